@@ -376,6 +376,108 @@ int qraf_cuda_decoder_info(qraf_decoder_t d, uint32_t* vocab, uint32_t* hidden, 
 /* Free the decoder, its caches and its model. */
 int qraf_cuda_decoder_close(qraf_decoder_t d);
 
+/* ── KV-cache operators ────────────────────────────────────────────────── */
+/* The int8 KV cache of one layer as a plain descriptor (the layout and quantizer
+ * of the reference's QuantizedKVCache, include/nn/kv_cache_quant.h:16-94): row r
+ * of slot s holds, for each KV head h, head_dim int8 codes of K and of V at element
+ * ((s * slot_rows + r) * kv_heads + h) * head_dim and one fp32 scale of each at the
+ * same index without head_dim; a value is code * scale.  Nothing is owned. */
+typedef struct qraf_kv {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    uint64_t slot_rows;   /* rows from one slot's first row to the next slot's, at least `rows` */
+    uint32_t slots;
+    uint32_t rows;        /* rows of a slot */
+    uint32_t kv_heads;
+    uint32_t head_dim;    /* a multiple of 16, at most 256 */
+    int32_t device;       /* CUDA device that holds the codes */
+} qraf_kv_t;
+/* Describe a cache in device memory (nothing is copied).  Codes 16-byte aligned. */
+int qraf_cuda_kv_wrap(int8_t* k_dev, int8_t* v_dev, float* k_scale_dev, float* v_scale_dev, uint32_t slots, uint32_t rows,
+                      uint64_t slot_rows, uint32_t kv_heads, uint32_t head_dim, qraf_kv_t* out);
+
+/* Element types of the operators' activations. */
+#define QRAF_TYPE_F32  0u
+#define QRAF_TYPE_F16  1u
+#define QRAF_TYPE_BF16 2u
+
+/* Runs.  New rows come in `count` runs: rows cu_dev[b] .. cu_dev[b + 1] (of n) are
+ * run b's, consecutive in slot slots_dev[b].  cu_dev (count + 1 values, ascending,
+ * from 0 and at most n) may be NULL: one row a run, count == n.  Rows behind the
+ * last run and runs whose slot is -1 (a padded batch) are left as they were.
+ * Other slots out of range, and rows past the end of a slot, are not touched and
+ * raise the device status (qraf_cuda_device_status).  slots, starts, lens and cu
+ * are device int32 arrays, read by the kernels: a captured call may be replayed
+ * with other values in them. */
+
+/* Quantise rows of K and V as they are written: row i of run b goes to row
+ * starts_dev[b] + i of its slot, per KV head scale = max |x| / 127, codes
+ * clamp(round(x / scale), -127, 127) (QuantizedKVCache::store,
+ * include/nn/kv_cache_quant.h:61-94).  k_dev and v_dev: rows of kv_heads * head_dim
+ * elements of `type`, k_ld and v_ld elements apart.  Where two runs of one call
+ * write the same row, the later run's values stay. */
+int qraf_cuda_kv_store(const qraf_kv_t* kv, const void* k_dev, const void* v_dev, uint32_t type, uint64_t k_ld,
+                       uint64_t v_ld, uint32_t n, const int32_t* slots_dev, const int32_t* starts_dev,
+                       const int32_t* cu_dev, uint32_t count, void* stream);
+/* Read the same rows back as numbers: code * scale, rounded once to `type`. */
+int qraf_cuda_kv_load(const qraf_kv_t* kv, void* k_dev, void* v_dev, uint32_t type, uint64_t k_ld, uint64_t v_ld,
+                      uint32_t n, const int32_t* slots_dev, const int32_t* starts_dev, const int32_t* cu_dev,
+                      uint32_t count, void* stream);
+
+/* Attention of new tokens over the cache: out[t] = softmax(scale q[t] K^T) V per
+ * head, heads / kv_heads query heads sharing a KV head (attention_forward,
+ * src/nn/attention.cpp:104-150, over codes as kv_cache_quant.h:113-123 reads them).
+ * A sequence's keys are first the prefix, rows 0 .. prefix_len of slot prefix_slot
+ * of `prefix` (read once for the whole batch; prefix_len 0: none, `prefix` may be
+ * NULL), then the rows of its own slot: run b's slot holds lens_dev[b] rows, its
+ * new tokens' among them, and token i of a run of m sees the first
+ * lens_dev[b] - m + 1 + i of them.  A token that sees no key gets zeros.  q_dev and
+ * out_dev: n rows of heads * head_dim elements of `type`, q_ld and out_ld elements
+ * apart; they may not overlap.  max_len: no lens_dev[b] is larger (at most kv->rows;
+ * one that is raises the device status and leaves its rows as they were); the work
+ * is cut for that length.  Sums, maxima and the running output are fp32 and the
+ * products at fp32 accuracy whatever the type.
+ * workspace_dev: qraf_cuda_kv_attention_workspace's bytes for the same shape
+ * (16-byte aligned; NULL where that is 0), written by the call: calls that may run
+ * at the same time, replays of captured ones among them, need one each. */
+int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_t prefix_slot, uint32_t prefix_len,
+                           const void* q_dev, void* out_dev, uint32_t type, uint64_t q_ld, uint64_t out_ld, uint32_t n,
+                           uint32_t heads, const int32_t* slots_dev, const int32_t* lens_dev, const int32_t* cu_dev,
+                           uint32_t count, uint32_t max_len, float scale, void* workspace_dev, uint64_t workspace_bytes,
+                           void* stream);
+/* ragged: whether the call has a cu_dev. */
+int qraf_cuda_kv_attention_workspace(const qraf_kv_t* kv, uint32_t prefix_len, uint32_t n, uint32_t heads, uint32_t count,
+                                     int ragged, uint32_t max_len, uint64_t* bytes);
+
+/* ── from logits to accepted tokens ─────────────────────────────────────── */
+/* probs[r] = softmax(logits[r] / temperature) for rows of `vocab` values, rows
+ * logits_ld and probs_ld apart (the temperature step of Sampler::sample,
+ * src/sampling/sampler.cpp:56-130).  temperature > 0.  Logits of -inf give 0; a row
+ * of nothing else gives zeros.  probs may be logits itself (same stride). */
+int qraf_cuda_token_probs(const float* logits_dev, uint64_t logits_ld, float* probs_dev, uint64_t probs_ld, uint32_t rows,
+                          uint32_t vocab, float temperature, void* stream);
+/* Verify drafted tokens against the target's probabilities (the draft / verify
+ * step of src/runtime/speculative.cpp, in its sampling form).  Per sequence b:
+ * target has drafts + 1 rows of vocab probabilities (row i: after the first i
+ * drafts), draft has `drafts` rows, tokens_dev[b][drafts] the drafted tokens,
+ * u_dev[b][drafts] and u_last_dev[b] uniform numbers in [0, 1).  Draft i stands while
+ * u_i q_i(x_i) < p_i(x_i); the first that falls is replaced by a draw from
+ * max(p_i - q_i, 0) (from p_i where that is zero everywhere), and when all stand
+ * one more token is drawn from the last row.  A draw takes the smallest token whose
+ * running sum of weights exceeds u_last times their total; products, differences
+ * and sums are taken in 64 bits.  out_tokens_dev[b][drafts + 1]: the standing drafts,
+ * the drawn token, then -1; accepted_dev[b]: how many stand.  counts_dev[b] (NULL:
+ * drafts): sequence b has that many; -1 leaves its outputs as they were.  The
+ * strides are in elements (sequence to sequence, row to row).  A token outside the
+ * vocabulary falls, a count above `drafts` is cut, a row without any weight gives
+ * token -1: each raises the device status.  At most 256 drafts. */
+int qraf_cuda_verify_drafts(const float* target_dev, uint64_t target_seq, uint64_t target_row, const float* draft_dev,
+                            uint64_t draft_seq, uint64_t draft_row, const int32_t* tokens_dev, const float* u_dev,
+                            const float* u_last_dev, const int32_t* counts_dev, uint32_t seqs, uint32_t drafts,
+                            uint32_t vocab, int32_t* out_tokens_dev, int32_t* accepted_dev, void* stream);
+
 /* ── host utility ───────────────────────────────────────────────────────── */
 /* Seeded synthetic data with the reference's idiom: std::mt19937(seed) and
  * std::normal_distribution<float>(mean, stddev) (tools/dummy_model.cpp:12-16). */

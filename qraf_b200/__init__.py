@@ -13,6 +13,7 @@ built.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -64,11 +65,26 @@ class qraf_weight_t(C.Structure):
     ]
 
 
+class qraf_kv_t(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("slot_rows", C.c_uint64),
+        ("slots", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("device", C.c_int32),
+    ]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: run `python -m qraf_b200.build` (nvcc, sm_100a) first")
     lib = C.CDLL(LIB_PATH)
-    W = C.POINTER(qraf_weight_t)
+    W, KV = C.POINTER(qraf_weight_t), C.POINTER(qraf_kv_t)
     vp, u32, u64, i32, f32p = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.POINTER(C.c_float)
     sig = {
         "qraf_cuda_version": (C.c_char_p, []),
@@ -113,6 +129,14 @@ def _load() -> C.CDLL:
         "qraf_cuda_decoder_kv_read": (i32, [vp, u32, u32, u32, vp, vp, f32p, f32p]),
         "qraf_cuda_model_open_ex": (i32, [C.c_char_p, u32, C.POINTER(vp)]),
         "qraf_cuda_model_tensor_f32": (i32, [vp, C.c_char_p, C.POINTER(vp), C.POINTER(u64)]),
+        "qraf_cuda_kv_wrap": (i32, [vp, vp, vp, vp, u32, u32, u64, u32, u32, KV]),
+        "qraf_cuda_kv_store": (i32, [KV, vp, vp, u32, u64, u64, u32, vp, vp, vp, u32, vp]),
+        "qraf_cuda_kv_load": (i32, [KV, vp, vp, u32, u64, u64, u32, vp, vp, vp, u32, vp]),
+        "qraf_cuda_kv_attention": (i32, [KV, KV, u32, u32, vp, vp, u32, u64, u64, u32, u32, vp, vp, vp, u32, u32,
+                                         C.c_float, vp, u64, vp]),
+        "qraf_cuda_kv_attention_workspace": (i32, [KV, u32, u32, u32, u32, i32, u32, C.POINTER(u64)]),
+        "qraf_cuda_token_probs": (i32, [vp, u64, vp, u64, u32, u32, C.c_float, vp]),
+        "qraf_cuda_verify_drafts": (i32, [vp, u64, u64, vp, u64, u64, vp, vp, vp, vp, u32, u32, u32, vp, vp, vp]),
         "qraf_fill_normal": (None, [u32, C.c_float, C.c_float, f32p, u64]),
         "qraf_cuda_comm_create": (i32, [i32, i32, u64, C.POINTER(vp)]),
         "qraf_cuda_comm_handle": (i32, [vp, vp]),
@@ -518,6 +542,288 @@ def dequantize(dtype: int, q, count: int, block_size: int = 32, stream=None):
     check(_get_lib().qraf_cuda_dequantize(dtype, C.c_void_p(q.data_ptr()), count, block_size, C.c_void_p(out.data_ptr()),
                                    _stream(stream)))
     return out
+
+
+# ── KV-cache operators ───────────────────────────────────────────────────
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+
+
+def _type_of(dtype) -> int:
+    torch = _torch()
+    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if dtype not in types:
+        raise ValueError(f"{dtype}: float32, float16 or bfloat16")
+    return types[dtype]
+
+
+def _check_ints(device, **tensors) -> None:
+    """Contiguous int32 tensors on `device` (None entries are skipped)."""
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != torch.int32 or t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+
+
+def _allocating_on(stream, device):
+    """Where what a call allocates belongs to the stream it runs on: memory that the current
+    stream has just let go may still be in use there."""
+    if stream is None:
+        return contextlib.nullcontext()
+    torch = _torch()
+    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
+                             torch.cuda.ExternalStream(int(stream), device=device))
+
+
+def _runs_of(firsts, slots, cu, n: int, device, firsts_name: str) -> int:
+    """The number of runs, their arrays checked."""
+    _check_ints(device, slots=slots, cu=cu, **{firsts_name: firsts})
+    count = slots.numel()
+    if firsts.numel() != count:
+        raise ValueError(f"{count} slots and {firsts.numel()} {firsts_name}")
+    if cu is None:
+        if count != n:
+            raise ValueError(f"{count} slots and {n} rows: without cu each row is a run")
+    elif cu.numel() != count + 1:
+        raise ValueError(f"cu needs {count + 1} values, has {cu.numel()}")
+    return count
+
+
+def _row_stride(t, inner: tuple, name: str) -> int:
+    """Elements from row to row of [n, *inner] (or [n, product of inner]) with contiguous rows."""
+    width = 1
+    for d in inner:
+        width *= d
+    if t.dim() == 1 + len(inner) and tuple(t.shape[1:]) == inner:
+        at = 1
+        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if size != 1 and stride != at:
+                raise ValueError(f"{name}: the values of a row must be contiguous")
+            at *= size
+    elif not (t.dim() == 2 and t.shape[1] == width and (width == 1 or t.stride(1) == 1)):
+        raise ValueError(f"{name} must be [n, {', '.join(map(str, inner))}] with contiguous rows")
+    if t.shape[0] > 1 and t.stride(0) < width:
+        raise ValueError(f"{name}: rows overlap")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+class KvCache:
+    """The int8 KV cache of one layer: row r of slot s holds, per KV head, head_dim
+    int8 codes of K and of V and one fp32 scale of each (the reference's
+    QuantizedKVCache layout); a value is code * scale.
+
+    k, v: int8 [slots, rows, kv_heads, head_dim]; k_scale, v_scale: float32
+    [slots, rows, kv_heads], all on one device.  Slots may lie further apart than
+    their rows (a view of a larger tensor), by the same number of rows in all four."""
+
+    def __init__(self, slots: int, rows: int, kv_heads: int, head_dim: int, device=None):
+        torch = _torch()
+        shape = (slots, rows, kv_heads)
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        self._set(*(torch.zeros(*shape, head_dim, dtype=torch.int8, device=dev) for _ in range(2)),
+                  *(torch.zeros(shape, dtype=torch.float32, device=dev) for _ in range(2)))
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale) -> "KvCache":
+        """A cache in the caller's tensors (nothing is copied)."""
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale)
+        return self
+
+    def _set(self, k, v, k_scale, v_scale) -> None:
+        torch = _torch()
+        if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8 or v.shape != k.shape:
+            raise ValueError("k and v must be int8 tensors of one shape [slots, rows, kv_heads, head_dim]")
+        if any(s.shape != k.shape[:3] or s.dtype != torch.float32 for s in (k_scale, v_scale)):
+            raise ValueError("k_scale and v_scale must be float32 [slots, rows, kv_heads]")
+        if any(not t.is_cuda or t.device != k.device for t in (k, v, k_scale, v_scale)):
+            raise ValueError("the cache's tensors must be on one CUDA device")
+        slots, rows, heads, dim = k.shape
+        if 0 in k.shape:
+            raise ValueError("the cache is empty")
+        apart = set()
+        for t, width in ((k, heads * dim), (v, heads * dim), (k_scale, heads), (v_scale, heads)):
+            if not t[0].is_contiguous():
+                raise ValueError("the rows of a slot must be contiguous")
+            if slots > 1:
+                if t.stride(0) % width:
+                    raise ValueError("slots must lie a whole number of rows apart")
+                apart.add(t.stride(0) // width)
+        if len(apart) > 1:
+            raise ValueError("codes and scales must have their slots the same number of rows apart")
+        d = qraf_kv_t()
+        check(_get_lib().qraf_cuda_kv_wrap(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots,
+                                           rows, apart.pop() if apart else rows, heads, dim, C.byref(d)))
+        self.desc, self.k, self.v, self.k_scale, self.v_scale = d, k, v, k_scale, v_scale
+        self.device = k.device
+        self.slots, self.rows, self.kv_heads, self.head_dim = slots, rows, heads, dim
+        self._workspace = {}
+
+
+def kv_store(cache: KvCache, k, v, slots, starts, cu=None, stream=None) -> None:
+    """Quantise rows of K and V into `cache` as they are written (qraf_cuda_kv_store).
+
+    k, v: float32, float16 or bfloat16 [n, kv_heads, head_dim] (or [n, kv_heads * head_dim]),
+    rows contiguous, any stride between them.  Rows cu[b] .. cu[b + 1] go to rows starts[b] ..
+    of slot slots[b] (int32 CUDA tensors; without cu, one row each); slot -1 and rows behind
+    the last run are left out, and where two runs write one row the later one stays."""
+    inner = (cache.kv_heads, cache.head_dim)
+    if k.device != cache.device or v.device != cache.device or v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        raise ValueError(f"k and v must have one type and length and be on {cache.device}")
+    ld_k, ld_v, n = _row_stride(k, inner, "k"), _row_stride(v, inner, "v"), k.shape[0]
+    count = _runs_of(starts, slots, cu, n, cache.device, "starts")
+    check(_get_lib().qraf_cuda_kv_store(C.byref(cache.desc), k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n,
+                                        slots.data_ptr(), starts.data_ptr(), None if cu is None else cu.data_ptr(), count,
+                                        _stream(stream)))
+
+
+def kv_load(cache: KvCache, slots, starts, cu=None, n=None, dtype=None, k=None, v=None, stream=None) -> tuple:
+    """Rows of K and V read back as numbers (qraf_cuda_kv_load), the runs as in kv_store.
+
+    n: the number of rows (needed with cu, unless k and v are given to be written);
+    dtype: float32 (default), float16 or bfloat16.  Returns (k, v) [n, kv_heads, head_dim]."""
+    torch = _torch()
+    inner = (cache.kv_heads, cache.head_dim)
+    if (k is None) != (v is None):
+        raise ValueError("k and v go together")
+    if k is None:
+        n = slots.numel() if n is None and cu is None else n
+        if n is None:
+            raise ValueError("n, the number of rows, is needed with cu")
+        with _allocating_on(stream, cache.device):
+            k, v = (torch.empty((n, *inner), dtype=dtype or torch.float32, device=cache.device) for _ in range(2))
+    elif k.device != cache.device or v.device != cache.device or v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        raise ValueError(f"k and v must have one type and length and be on {cache.device}")
+    ld_k, ld_v, n = _row_stride(k, inner, "k"), _row_stride(v, inner, "v"), k.shape[0]
+    count = _runs_of(starts, slots, cu, n, cache.device, "starts")
+    check(_get_lib().qraf_cuda_kv_load(C.byref(cache.desc), k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n,
+                                       slots.data_ptr(), starts.data_ptr(), None if cu is None else cu.data_ptr(), count,
+                                       _stream(stream)))
+    return k, v
+
+
+def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_slot: int = 0, prefix_len: int = 0,
+                 max_len=None, scale=None, out=None, stream=None):
+    """Attention of new tokens over the int8 cache, behind a prefix that the whole batch
+    shares (qraf_cuda_kv_attention).
+
+    q: float32, float16 or bfloat16 [n, heads, head_dim] (or [n, heads * head_dim]), heads a
+    multiple of the cache's kv_heads.  Tokens cu[b] .. cu[b + 1] are sequence b's new ones
+    (without cu, one each); its slot slots[b] holds lens[b] rows, theirs included, and token
+    i of m sees the first lens[b] - m + 1 + i of them after the prefix_len rows of slot
+    prefix_slot of the KvCache `prefix`.  A token that sees nothing gets zeros; tokens of
+    slot -1 or behind the last sequence keep what `out` holds.  max_len: no lens[b] is larger
+    (default: the cache's rows).  scale: default head_dim ** -0.5.  Returns out, shaped like q."""
+    torch = _torch()
+    if q.device != cache.device or q.dim() < 2:
+        raise ValueError(f"q must be [n, heads, head_dim] on {cache.device}")
+    dim = cache.head_dim
+    heads = q.shape[1] if q.dim() == 3 else q.shape[1] // dim
+    q_ld, n = _row_stride(q, (heads, dim), "q"), q.shape[0]
+    out_ld = heads * dim
+    if out is not None:
+        if out.dtype != q.dtype or out.device != q.device or out.shape[0] != n:
+            raise ValueError("out must have q's type, device and length")
+        out_ld = _row_stride(out, (heads, dim), "out")
+    count = _runs_of(lens, slots, cu, n, cache.device, "lens")
+    if prefix_len < 0 or prefix_slot < 0:
+        raise ValueError("prefix_len and prefix_slot cannot be negative")
+    if prefix_len and prefix is None:
+        raise ValueError("prefix_len without a prefix")
+    max_len = cache.rows if max_len is None else max_len
+    if max_len < 0:
+        raise ValueError("max_len cannot be negative")
+    lib, d = _get_lib(), C.byref(cache.desc)
+    key = (prefix_len, n, heads, count, cu is None, max_len)
+    size = cache._workspace.get(key)
+    if size is None:   # bytes by shape; the memory itself belongs to the call
+        b = C.c_uint64()
+        check(lib.qraf_cuda_kv_attention_workspace(d, prefix_len, n, heads, count, cu is not None, max_len, C.byref(b)))
+        if len(cache._workspace) > 4096:
+            cache._workspace.clear()
+        size = cache._workspace[key] = b.value
+    with _allocating_on(stream, q.device):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(lib.qraf_cuda_kv_attention(d, C.byref(prefix.desc) if prefix_len else None, prefix_slot, prefix_len,
+                                     q.data_ptr(), out.data_ptr(), _type_of(q.dtype), q_ld, out_ld, n, heads,
+                                     slots.data_ptr(), lens.data_ptr(), None if cu is None else cu.data_ptr(), count,
+                                     max_len, dim ** -0.5 if scale is None else scale,
+                                     None if ws is None else ws.data_ptr(), size, _stream(stream)))
+    return out
+
+
+# ── from logits to accepted tokens ───────────────────────────────────────
+def token_probs(logits, temperature: float = 1.0, out=None, stream=None):
+    """softmax(logits / temperature) over the last dimension (qraf_cuda_token_probs) of a
+    float32 CUDA tensor [rows, vocab] or [vocab]; -inf gives 0, a row of nothing else
+    zeros.  out may be logits itself."""
+    torch = _torch()
+    x = logits.reshape(1, -1) if logits.dim() == 1 else logits
+    if x.dim() != 2 or x.dtype != torch.float32 or not x.is_cuda:
+        raise ValueError("logits must be a CUDA float32 tensor [rows, vocab]")
+    _check_current(x.device)
+    if out is None:
+        with _allocating_on(stream, x.device):
+            out = torch.empty(logits.shape, dtype=torch.float32, device=x.device)
+    y = out.reshape(1, -1) if out.dim() == 1 else out
+    if y.dtype != torch.float32 or y.device != x.device or y.shape != x.shape:
+        raise ValueError("out must be float32, shaped like logits, on its device")
+    x_ld, y_ld = _row_stride(x, (x.shape[1],), "logits"), _row_stride(y, (x.shape[1],), "out")
+    check(_get_lib().qraf_cuda_token_probs(x.data_ptr(), x_ld, y.data_ptr(), y_ld, x.shape[0], x.shape[1], temperature,
+                                           _stream(stream)))
+    return out
+
+
+def verify_drafts(target, draft, tokens, u, u_last, counts=None, stream=None) -> tuple:
+    """Verify drafted tokens against the target's probabilities from given uniform random
+    numbers (qraf_cuda_verify_drafts).
+
+    target: float32 [B, K + 1, vocab] probabilities (row i: after the first i drafts); draft:
+    float32 [B, K, vocab]; tokens: int32 [B, K]; u: float32 [B, K]; u_last: float32 [B];
+    counts: int32 [B], the drafts of each sequence (default K; -1: its outputs are left as
+    they were, here uninitialised).  Rows of the vocabulary are contiguous, other strides free.
+    Draft i stands while u_i q_i(x_i) < p_i(x_i); the first that falls is replaced by a draw from
+    max(p_i - q_i, 0), and when all stand one more token is drawn from the next row.  Returns
+    (int32 [B, K + 1]: the standing drafts, the drawn token, then -1; int32 [B]: how many stand)."""
+    torch = _torch()
+    dev = target.device
+    if target.dim() != 3 or draft.dim() != 3 or tokens.dim() != 2:
+        raise ValueError("target [B, K + 1, vocab], draft [B, K, vocab], tokens [B, K]")
+    b, k1, vocab = target.shape
+    k = k1 - 1
+    if k < 0 or tuple(draft.shape) != (b, k, vocab) or tuple(tokens.shape) != (b, k) or tuple(u.shape) != (b, k) or \
+            tuple(u_last.shape) != (b,) or (counts is not None and tuple(counts.shape) != (b,)):
+        raise ValueError(f"shapes do not fit {b} sequences of {k} drafts over {vocab} tokens")
+    for name, t in (("target", target), ("draft", draft), ("u", u), ("u_last", u_last)):
+        if t.dtype != torch.float32 or t.device != dev or not t.is_cuda:
+            raise ValueError(f"{name} must be a float32 tensor on target's CUDA device")
+    if not u.is_contiguous() or not u_last.is_contiguous():
+        raise ValueError("u and u_last must be contiguous")
+    if any(t.numel() and vocab > 1 and t.stride(2) != 1 for t in (target, draft)):
+        raise ValueError("rows of target and draft must be contiguous")
+    _check_ints(dev, tokens=tokens, counts=counts)
+    _check_current(dev)
+    with _allocating_on(stream, dev):
+        out = torch.empty((b, k + 1), dtype=torch.int32, device=dev)
+        accepted = torch.empty(b, dtype=torch.int32, device=dev)
+
+    def strides(t):   # a dimension of one has any stride
+        return max(t.stride(0), vocab) if t.shape[0] <= 1 else t.stride(0), \
+            max(t.stride(1), vocab) if t.shape[1] <= 1 else t.stride(1)
+
+    check(_get_lib().qraf_cuda_verify_drafts(target.data_ptr(), *strides(target), draft.data_ptr(), *strides(draft),
+                                             tokens.data_ptr(), u.data_ptr(), u_last.data_ptr(),
+                                             None if counts is None else counts.data_ptr(), b, k, vocab, out.data_ptr(),
+                                             accepted.data_ptr(), _stream(stream)))
+    return out, accepted
+
+
+def _check_current(device) -> None:
+    if device.index != _torch().cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, the current device is {_torch().cuda.current_device()}")
 
 
 # ── host side: the reference-facing entry ────────────────────────────────

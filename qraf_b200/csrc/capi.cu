@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cudaTypedefs.h>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -17,12 +18,15 @@
 #include <vector>
 
 #include "common.cuh"
+#include "kv_attention.cuh"
+#include "kv_cache.cuh"
 #include "matmul_tc.cuh"
 #include "matvec_generic.cuh"
 #include "matvec_rows.cuh"
 #include "matvec_stream.cuh"
 #include "matvec_tc1.cuh"
 #include "quantize.cuh"
+#include "sampling.cuh"
 
 using namespace qraf_dev;
 
@@ -129,6 +133,10 @@ int ensure_device(int* dev_out, DeviceInfo** info_out) {
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 16>, lim));
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 32>, lim));
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 64>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<64>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<128>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<256>, lim));
+        QRAF_CUDA_TRY(allow_smem(token_probs_kernel, lim));
         d.ready = true;
     }
     if (dev_out) *dev_out = dev;
@@ -1981,4 +1989,5 @@ void qraf_fill_normal(uint32_t seed, float mean, float stddev, float* out_host, 
 }  // extern "C"
 
 #include "model_store.cuh"
+#include "kv_api.cuh"
 #include "decoder.cuh"

@@ -121,16 +121,6 @@ __device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(gmem) : "memory");
 }
 
-// QuantizedKVCache::store for one value (include/nn/kv_cache_quant.h:61-94):
-// clamp(round(x * inv), -127, 127), inv = 1 / (max |x| / 127) (0 when the max is 0).
-__device__ __forceinline__ int8_t kvq_code(float x, float inv) {
-    return static_cast<int8_t>(fmaxf(-127.0f, fminf(127.0f, roundf(__fmul_rn(x, inv)))));
-}
-__device__ __forceinline__ float4 i8x4_to_f4(uint32_t w) {
-    return make_float4(static_cast<float>(static_cast<int8_t>(w)), static_cast<float>(static_cast<int8_t>(w >> 8)),
-                       static_cast<float>(static_cast<int8_t>(w >> 16)), static_cast<float>(static_cast<int8_t>(w >> 24)));
-}
-
 // Attention of one step, fused with RoPE and the KV-cache store
 // (attention_forward, src/nn/attention.cpp:104-150).  CTA (s, kvh, m) takes slot
 // m's KV head kvh and the G = heads / kv_heads query heads that share it (the
