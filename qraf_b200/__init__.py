@@ -13,7 +13,6 @@ built.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 
@@ -192,10 +191,16 @@ def fill_normal(seed: int, mean: float, std: float, n: int) -> np.ndarray:
 
 
 # ── device side (torch tensors as device memory) ─────────────────────────
-def _torch():
-    import torch
+_TORCH = None
 
-    return torch
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
 
 
 def _stream(stream) -> C.c_void_p:
@@ -551,34 +556,28 @@ TYPE_BF16 = 2
 
 
 def _type_of(dtype) -> int:
-    torch = _torch()
-    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-    if dtype not in types:
+    global _TYPES
+    if _TYPES is None:
+        torch = _torch()
+        _TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    t = _TYPES.get(dtype)
+    if t is None:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16")
-    return types[dtype]
+    return t
 
 
-def _check_ints(device, **tensors) -> None:
-    """Contiguous int32 tensors on `device` (None entries are skipped)."""
-    torch = _torch()
-    for name, t in tensors.items():
-        if t is not None and (t.dtype != torch.int32 or t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+_TYPES = None
 
 
-def _allocating_on(stream, device):
-    """Where what a call allocates belongs to the stream it runs on: memory that the current
-    stream has just let go may still be in use there."""
-    if stream is None:
-        return contextlib.nullcontext()
-    torch = _torch()
-    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
-                             torch.cuda.ExternalStream(int(stream), device=device))
+def _ints(t, index: int, name: str) -> int:
+    """Address of a contiguous int32 tensor on device `index`."""
+    if t.dtype != _torch().int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor on cuda:{index}")
+    return t.data_ptr()
 
 
-def _runs_of(firsts, slots, cu, n: int, device, firsts_name: str) -> int:
-    """The number of runs, their arrays checked."""
-    _check_ints(device, slots=slots, cu=cu, **{firsts_name: firsts})
+def _runs_of(slots, firsts, cu, n: int, index: int, firsts_name: str) -> tuple:
+    """(slots, firsts, cu, number of runs) for the library, checked."""
     count = slots.numel()
     if firsts.numel() != count:
         raise ValueError(f"{count} slots and {firsts.numel()} {firsts_name}")
@@ -587,25 +586,51 @@ def _runs_of(firsts, slots, cu, n: int, device, firsts_name: str) -> int:
             raise ValueError(f"{count} slots and {n} rows: without cu each row is a run")
     elif cu.numel() != count + 1:
         raise ValueError(f"cu needs {count + 1} values, has {cu.numel()}")
-    return count
+    return (_ints(slots, index, "slots"), _ints(firsts, index, firsts_name),
+            None if cu is None else _ints(cu, index, "cu"), count)
 
 
-def _row_stride(t, inner: tuple, name: str) -> int:
-    """Elements from row to row of [n, *inner] (or [n, product of inner]) with contiguous rows."""
-    width = 1
-    for d in inner:
-        width *= d
-    if t.dim() == 1 + len(inner) and tuple(t.shape[1:]) == inner:
-        at = 1
-        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if size != 1 and stride != at:
-                raise ValueError(f"{name}: the values of a row must be contiguous")
-            at *= size
-    elif not (t.dim() == 2 and t.shape[1] == width and (width == 1 or t.stride(1) == 1)):
-        raise ValueError(f"{name} must be [n, {', '.join(map(str, inner))}] with contiguous rows")
-    if t.shape[0] > 1 and t.stride(0) < width:
+def _rows_of(t, heads: int, dim: int, index: int, name: str) -> tuple:
+    """(rows, elements from row to row) of [n, heads, dim] or [n, heads * dim] with contiguous rows."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}")
+    shape, width = t.shape, heads * dim
+    d = len(shape)
+    if not (d == 3 and shape[1] == heads and shape[2] == dim or d == 2 and shape[1] == width):
+        raise ValueError(f"{name} must be [n, {heads}, {dim}] or [n, {width}], is {list(shape)}")
+    if t.is_contiguous():
+        return shape[0], width
+    stride = t.stride()
+    if (dim if d == 3 else width) > 1 and stride[-1] != 1 or d == 3 and heads > 1 and stride[1] != dim:
+        raise ValueError(f"{name}: the values of a row must be contiguous")
+    if shape[0] <= 1:
+        return shape[0], width
+    if stride[0] < width:
         raise ValueError(f"{name}: rows overlap")
-    return t.stride(0) if t.shape[0] > 1 else width
+    return shape[0], stride[0]
+
+
+def _allocating_on(stream, device):
+    """Where what a call allocates belongs to the stream it runs on: memory that the current
+    stream has just let go may still be in use there."""
+    torch = _torch()
+    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
+                             torch.cuda.ExternalStream(int(stream), device=device))
+
+
+def _empty(shape, dtype, like, stream):
+    """A tensor on `like`'s device for a call on `stream`."""
+    if stream is None:
+        return _torch().empty(shape, dtype=dtype, device=like.device)
+    with _allocating_on(stream, like.device):
+        return _torch().empty(shape, dtype=dtype, device=like.device)
+
+
+def _stream_on(stream, index: int):
+    """The stream's handle; the current stream of device `index` when it is None."""
+    if stream is None:
+        return _torch()._C._cuda_getCurrentRawStream(index)
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
 class KvCache:
@@ -656,7 +681,7 @@ class KvCache:
         check(_get_lib().qraf_cuda_kv_wrap(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots,
                                            rows, apart.pop() if apart else rows, heads, dim, C.byref(d)))
         self.desc, self.k, self.v, self.k_scale, self.v_scale = d, k, v, k_scale, v_scale
-        self.device = k.device
+        self.device, self._index, self._ref = k.device, k.device.index, C.byref(d)
         self.slots, self.rows, self.kv_heads, self.head_dim = slots, rows, heads, dim
         self._workspace = {}
 
@@ -668,14 +693,14 @@ def kv_store(cache: KvCache, k, v, slots, starts, cu=None, stream=None) -> None:
     rows contiguous, any stride between them.  Rows cu[b] .. cu[b + 1] go to rows starts[b] ..
     of slot slots[b] (int32 CUDA tensors; without cu, one row each); slot -1 and rows behind
     the last run are left out, and where two runs write one row the later one stays."""
-    inner = (cache.kv_heads, cache.head_dim)
-    if k.device != cache.device or v.device != cache.device or v.dtype != k.dtype or v.shape[0] != k.shape[0]:
-        raise ValueError(f"k and v must have one type and length and be on {cache.device}")
-    ld_k, ld_v, n = _row_stride(k, inner, "k"), _row_stride(v, inner, "v"), k.shape[0]
-    count = _runs_of(starts, slots, cu, n, cache.device, "starts")
-    check(_get_lib().qraf_cuda_kv_store(C.byref(cache.desc), k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n,
-                                        slots.data_ptr(), starts.data_ptr(), None if cu is None else cu.data_ptr(), count,
-                                        _stream(stream)))
+    heads, dim, index = cache.kv_heads, cache.head_dim, cache._index
+    n, ld_k = _rows_of(k, heads, dim, index, "k")
+    m, ld_v = _rows_of(v, heads, dim, index, "v")
+    if m != n or v.dtype != k.dtype:
+        raise ValueError("k and v must have one type and length")
+    slots_p, starts_p, cu_p, count = _runs_of(slots, starts, cu, n, index, "starts")
+    check(_get_lib().qraf_cuda_kv_store(cache._ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
+                                        starts_p, cu_p, count, _stream_on(stream, index)))
 
 
 def kv_load(cache: KvCache, slots, starts, cu=None, n=None, dtype=None, k=None, v=None, stream=None) -> tuple:
@@ -683,23 +708,24 @@ def kv_load(cache: KvCache, slots, starts, cu=None, n=None, dtype=None, k=None, 
 
     n: the number of rows (needed with cu, unless k and v are given to be written);
     dtype: float32 (default), float16 or bfloat16.  Returns (k, v) [n, kv_heads, head_dim]."""
-    torch = _torch()
-    inner = (cache.kv_heads, cache.head_dim)
+    heads, dim, index = cache.kv_heads, cache.head_dim, cache._index
     if (k is None) != (v is None):
         raise ValueError("k and v go together")
     if k is None:
         n = slots.numel() if n is None and cu is None else n
         if n is None:
             raise ValueError("n, the number of rows, is needed with cu")
-        with _allocating_on(stream, cache.device):
-            k, v = (torch.empty((n, *inner), dtype=dtype or torch.float32, device=cache.device) for _ in range(2))
-    elif k.device != cache.device or v.device != cache.device or v.dtype != k.dtype or v.shape[0] != k.shape[0]:
-        raise ValueError(f"k and v must have one type and length and be on {cache.device}")
-    ld_k, ld_v, n = _row_stride(k, inner, "k"), _row_stride(v, inner, "v"), k.shape[0]
-    count = _runs_of(starts, slots, cu, n, cache.device, "starts")
-    check(_get_lib().qraf_cuda_kv_load(C.byref(cache.desc), k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n,
-                                       slots.data_ptr(), starts.data_ptr(), None if cu is None else cu.data_ptr(), count,
-                                       _stream(stream)))
+        dtype = _torch().float32 if dtype is None else dtype
+        k, v = (_empty((n, heads, dim), dtype, cache.k, stream) for _ in range(2))
+        ld_k = ld_v = heads * dim
+    else:
+        n, ld_k = _rows_of(k, heads, dim, index, "k")
+        m, ld_v = _rows_of(v, heads, dim, index, "v")
+        if m != n or v.dtype != k.dtype:
+            raise ValueError("k and v must have one type and length")
+    slots_p, starts_p, cu_p, count = _runs_of(slots, starts, cu, n, index, "starts")
+    check(_get_lib().qraf_cuda_kv_load(cache._ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
+                                       starts_p, cu_p, count, _stream_on(stream, index)))
     return k, v
 
 
@@ -715,18 +741,18 @@ def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_sl
     prefix_slot of the KvCache `prefix`.  A token that sees nothing gets zeros; tokens of
     slot -1 or behind the last sequence keep what `out` holds.  max_len: no lens[b] is larger
     (default: the cache's rows).  scale: default head_dim ** -0.5.  Returns out, shaped like q."""
-    torch = _torch()
-    if q.device != cache.device or q.dim() < 2:
-        raise ValueError(f"q must be [n, heads, head_dim] on {cache.device}")
-    dim = cache.head_dim
+    dim, index = cache.head_dim, cache._index
+    if q.dim() not in (2, 3):
+        raise ValueError("q must be [n, heads, head_dim] or [n, heads * head_dim]")
     heads = q.shape[1] if q.dim() == 3 else q.shape[1] // dim
-    q_ld, n = _row_stride(q, (heads, dim), "q"), q.shape[0]
-    out_ld = heads * dim
-    if out is not None:
-        if out.dtype != q.dtype or out.device != q.device or out.shape[0] != n:
-            raise ValueError("out must have q's type, device and length")
-        out_ld = _row_stride(out, (heads, dim), "out")
-    count = _runs_of(lens, slots, cu, n, cache.device, "lens")
+    n, q_ld = _rows_of(q, heads, dim, index, "q")
+    if out is None:
+        out, out_ld = _empty(q.shape, q.dtype, q, stream), heads * dim
+    else:
+        m, out_ld = _rows_of(out, heads, dim, index, "out")
+        if m != n or out.dtype != q.dtype:
+            raise ValueError("out must have q's type and length")
+    slots_p, lens_p, cu_p, count = _runs_of(slots, lens, cu, n, index, "lens")
     if prefix_len < 0 or prefix_slot < 0:
         raise ValueError("prefix_len and prefix_slot cannot be negative")
     if prefix_len and prefix is None:
@@ -734,24 +760,21 @@ def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_sl
     max_len = cache.rows if max_len is None else max_len
     if max_len < 0:
         raise ValueError("max_len cannot be negative")
-    lib, d = _get_lib(), C.byref(cache.desc)
+    lib = _get_lib()
     key = (prefix_len, n, heads, count, cu is None, max_len)
     size = cache._workspace.get(key)
     if size is None:   # bytes by shape; the memory itself belongs to the call
         b = C.c_uint64()
-        check(lib.qraf_cuda_kv_attention_workspace(d, prefix_len, n, heads, count, cu is not None, max_len, C.byref(b)))
+        check(lib.qraf_cuda_kv_attention_workspace(cache._ref, prefix_len, n, heads, count, cu is not None, max_len,
+                                                   C.byref(b)))
         if len(cache._workspace) > 4096:
             cache._workspace.clear()
         size = cache._workspace[key] = b.value
-    with _allocating_on(stream, q.device):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    check(lib.qraf_cuda_kv_attention(d, C.byref(prefix.desc) if prefix_len else None, prefix_slot, prefix_len,
-                                     q.data_ptr(), out.data_ptr(), _type_of(q.dtype), q_ld, out_ld, n, heads,
-                                     slots.data_ptr(), lens.data_ptr(), None if cu is None else cu.data_ptr(), count,
-                                     max_len, dim ** -0.5 if scale is None else scale,
-                                     None if ws is None else ws.data_ptr(), size, _stream(stream)))
+    ws = _empty(size, _torch().uint8, q, stream) if size else None
+    check(lib.qraf_cuda_kv_attention(cache._ref, prefix._ref if prefix_len else None, prefix_slot, prefix_len, q.data_ptr(),
+                                     out.data_ptr(), _type_of(q.dtype), q_ld, out_ld, n, heads, slots_p, lens_p, cu_p, count,
+                                     max_len, dim ** -0.5 if scale is None else scale, ws.data_ptr() if size else None, size,
+                                     _stream_on(stream, index)))
     return out
 
 
@@ -762,18 +785,21 @@ def token_probs(logits, temperature: float = 1.0, out=None, stream=None):
     zeros.  out may be logits itself."""
     torch = _torch()
     x = logits.reshape(1, -1) if logits.dim() == 1 else logits
-    if x.dim() != 2 or x.dtype != torch.float32 or not x.is_cuda:
+    index = x.get_device()
+    if x.dim() != 2 or x.dtype != torch.float32 or index < 0:
         raise ValueError("logits must be a CUDA float32 tensor [rows, vocab]")
-    _check_current(x.device)
+    rows, vocab = x.shape
+    _, x_ld = _rows_of(x, 1, vocab, index, "logits")
+    _check_current(index)
     if out is None:
-        with _allocating_on(stream, x.device):
-            out = torch.empty(logits.shape, dtype=torch.float32, device=x.device)
-    y = out.reshape(1, -1) if out.dim() == 1 else out
-    if y.dtype != torch.float32 or y.device != x.device or y.shape != x.shape:
-        raise ValueError("out must be float32, shaped like logits, on its device")
-    x_ld, y_ld = _row_stride(x, (x.shape[1],), "logits"), _row_stride(y, (x.shape[1],), "out")
-    check(_get_lib().qraf_cuda_token_probs(x.data_ptr(), x_ld, y.data_ptr(), y_ld, x.shape[0], x.shape[1], temperature,
-                                           _stream(stream)))
+        out, y_ld = _empty(logits.shape, torch.float32, x, stream), vocab
+    else:
+        y = out.reshape(1, -1) if out.dim() == 1 else out
+        m, y_ld = _rows_of(y, 1, vocab, index, "out")
+        if m != rows or y.dtype != torch.float32:
+            raise ValueError("out must be float32 and shaped like logits")
+    check(_get_lib().qraf_cuda_token_probs(x.data_ptr(), x_ld, out.data_ptr(), y_ld, rows, vocab, temperature,
+                                           _stream_on(stream, index)))
     return out
 
 
@@ -788,42 +814,42 @@ def verify_drafts(target, draft, tokens, u, u_last, counts=None, stream=None) ->
     Draft i stands while u_i q_i(x_i) < p_i(x_i); the first that falls is replaced by a draw from
     max(p_i - q_i, 0), and when all stand one more token is drawn from the next row.  Returns
     (int32 [B, K + 1]: the standing drafts, the drawn token, then -1; int32 [B]: how many stand)."""
-    torch = _torch()
-    dev = target.device
-    if target.dim() != 3 or draft.dim() != 3 or tokens.dim() != 2:
-        raise ValueError("target [B, K + 1, vocab], draft [B, K, vocab], tokens [B, K]")
+    f32 = _torch().float32
+    index = target.get_device()
+    if target.dim() != 3:
+        raise ValueError("target must be [B, K + 1, vocab]")
     b, k1, vocab = target.shape
     k = k1 - 1
-    if k < 0 or tuple(draft.shape) != (b, k, vocab) or tuple(tokens.shape) != (b, k) or tuple(u.shape) != (b, k) or \
-            tuple(u_last.shape) != (b,) or (counts is not None and tuple(counts.shape) != (b,)):
+    if k < 0 or draft.shape != (b, k, vocab) or tokens.shape != (b, k) or u.shape != (b, k) or u_last.shape != (b,) or \
+            (counts is not None and counts.shape != (b,)):
         raise ValueError(f"shapes do not fit {b} sequences of {k} drafts over {vocab} tokens")
-    for name, t in (("target", target), ("draft", draft), ("u", u), ("u_last", u_last)):
-        if t.dtype != torch.float32 or t.device != dev or not t.is_cuda:
-            raise ValueError(f"{name} must be a float32 tensor on target's CUDA device")
+    for t in (target, draft, u, u_last):
+        if t.dtype != f32 or t.get_device() != index or index < 0:
+            raise ValueError("target, draft, u and u_last must be float32 tensors on one CUDA device")
     if not u.is_contiguous() or not u_last.is_contiguous():
         raise ValueError("u and u_last must be contiguous")
-    if any(t.numel() and vocab > 1 and t.stride(2) != 1 for t in (target, draft)):
-        raise ValueError("rows of target and draft must be contiguous")
-    _check_ints(dev, tokens=tokens, counts=counts)
-    _check_current(dev)
-    with _allocating_on(stream, dev):
-        out = torch.empty((b, k + 1), dtype=torch.int32, device=dev)
-        accepted = torch.empty(b, dtype=torch.int32, device=dev)
-
-    def strides(t):   # a dimension of one has any stride
-        return max(t.stride(0), vocab) if t.shape[0] <= 1 else t.stride(0), \
-            max(t.stride(1), vocab) if t.shape[1] <= 1 else t.stride(1)
-
-    check(_get_lib().qraf_cuda_verify_drafts(target.data_ptr(), *strides(target), draft.data_ptr(), *strides(draft),
-                                             tokens.data_ptr(), u.data_ptr(), u_last.data_ptr(),
-                                             None if counts is None else counts.data_ptr(), b, k, vocab, out.data_ptr(),
-                                             accepted.data_ptr(), _stream(stream)))
+    strides = []
+    for t in (target, draft):
+        seq, row, one = t.stride()
+        if one != 1 and vocab > 1 and t.numel():
+            raise ValueError("rows of target and draft must be contiguous")
+        # a dimension of one has any stride
+        strides += [seq if b > 1 else max(seq, vocab), row if t.shape[1] > 1 else max(row, vocab)]
+    _check_current(index)
+    counts_p = None if counts is None else _ints(counts, index, "counts")
+    i32 = _torch().int32
+    out, accepted = _empty((b, k1), i32, target, stream), _empty(b, i32, target, stream)
+    check(_get_lib().qraf_cuda_verify_drafts(target.data_ptr(), strides[0], strides[1], draft.data_ptr(), strides[2],
+                                             strides[3], _ints(tokens, index, "tokens"), u.data_ptr(), u_last.data_ptr(),
+                                             counts_p, b, k, vocab, out.data_ptr(), accepted.data_ptr(),
+                                             _stream_on(stream, index)))
     return out, accepted
 
 
-def _check_current(device) -> None:
-    if device.index != _torch().cuda.current_device():
-        raise ValueError(f"the tensors are on {device}, the current device is {_torch().cuda.current_device()}")
+def _check_current(index: int) -> None:
+    current = _torch().cuda.current_device()
+    if index != current:
+        raise ValueError(f"the tensors are on cuda:{index}, the current device is cuda:{current}")
 
 
 # ── host side: the reference-facing entry ────────────────────────────────

@@ -20,6 +20,7 @@
 #include "common.cuh"
 #include "kv_attention.cuh"
 #include "kv_cache.cuh"
+#include "kv_prefix.cuh"
 #include "matmul_tc.cuh"
 #include "matvec_generic.cuh"
 #include "matvec_rows.cuh"
@@ -136,6 +137,12 @@ int ensure_device(int* dev_out, DeviceInfo** info_out) {
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<64>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<128>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<256>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 1, 1>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 1, 2>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 2, 2>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 1, 1>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 1, 2>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 2, 2>, lim));
         QRAF_CUDA_TRY(allow_smem(token_probs_kernel, lim));
         d.ready = true;
     }

@@ -104,8 +104,15 @@ int kv_io(const qraf_kv_t* kv, const void* k, const void* v, uint32_t type, uint
     return QRAF_OK;
 }
 
+#ifndef PRE_MIN_ROWS
+#define PRE_MIN_ROWS 17
+#endif
+bool prefix_on_tiles(uint64_t rows, uint32_t hd, uint32_t prefix_len) {
+    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 128u;
+}
+
 struct KvaPlan {
-    uint32_t row_tiles = 0, p_chunks = 0, p_chunk = 0, own_tiles = 0, splits = 0, own_wide = 0;
+    uint32_t row_tiles = 0, p_chunks = 0, p_chunk = 0, own_tiles = 0, splits = 0, own_wide = 0, pre_ctas = 0;
     uint64_t items = 0, part_bytes = 0;
 };
 
@@ -131,7 +138,15 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         items += groups * pl->splits;
     }
     pl->own_tiles = static_cast<uint32_t>(own_tiles);
-    if (prefix_len) {
+    if (prefix_len && prefix_on_tiles(rows, hd, prefix_len)) {
+        pl->row_tiles = static_cast<uint32_t>((rows + kPreRows - 1u) / kPreRows);
+        const uint64_t units = static_cast<uint64_t>(pl->row_tiles) * kv_heads;
+        const uint64_t work = units * ((prefix_len + kPreKeys - 1u) / kPreKeys);
+        pl->pre_ctas = static_cast<uint32_t>(std::min<uint64_t>(work, static_cast<uint64_t>(sm_count)));
+        // a unit's tiles start inside one CTA's range and end inside another's
+        const uint64_t T = work / units;
+        pl->p_chunks = static_cast<uint32_t>(std::min<uint64_t>(T, (T * pl->pre_ctas + work - 1u) / work + 1u));
+    } else if (prefix_len) {
         pl->row_tiles = static_cast<uint32_t>((rows + 15u) / 16u);
         const uint64_t units = static_cast<uint64_t>(pl->row_tiles) * kv_heads;
         const uint64_t by_len = (prefix_len + kKvaMinChunk - 1ull) / kKvaMinChunk;
@@ -141,23 +156,46 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         pl->p_chunks = (prefix_len + pl->p_chunk - 1u) / pl->p_chunk;
         items += units * pl->p_chunks;
     }
-    if (items == 0 || items > 0x7FFFFFFFull) {
-        if (items) return fail(QRAF_ERR_UNSUPPORTED, "the call has too many work items");
+    if (items > 0x7FFFFFFFull) return fail(QRAF_ERR_UNSUPPORTED, "the call has too many work items");
+    if (items == 0 && !pl->pre_ctas) {
         pl->splits = 1;   // no keys at all: one item a row tile writes the zeros
         items = own_tiles * kv_heads;
     }
     pl->items = items;
-    if (pl->p_chunks + pl->splits > 1u)
+    if (pl->p_chunks + pl->splits > 1u || pl->pre_ctas)
         pl->part_bytes = static_cast<uint64_t>(n) * heads * (pl->p_chunks + pl->splits) * (hd + 4u) * sizeof(float);
     return QRAF_OK;
 }
 
+template <typename K>
+cudaError_t launch_kv(K kernel, uint64_t grid, uint32_t threads, uint32_t smem, bool dependent, const KvAttnParams& p,
+                      cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    return counted(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
 template <uint32_t HDP>
 cudaError_t launch_kva(const KvAttnParams& p, uint64_t items, cudaStream_t st) {
-    constexpr uint32_t wide = KvaShape<HDP, true>::kSmem, narrow = KvaShape<HDP, false>::kSmem;
-    const uint32_t smem = (p.p_chunks || p.own_wide) ? wide : narrow;
-    (kv_attention_kernel<HDP><<<static_cast<unsigned>(items), kKvaThreads, smem, st>>>(p), count_launch());
-    return cudaGetLastError();
+    const bool wide = (p.p_chunks && !p.pre_ctas) || p.own_wide;
+    return launch_kv(kv_attention_kernel<HDP>, items, kKvaThreads,
+                     wide ? KvaShape<HDP, true>::kSmem : KvaShape<HDP, false>::kSmem, p.chained != 0u, p, st);
+}
+
+template <uint32_t HDP>
+cudaError_t launch_prefix(const KvAttnParams& p, cudaStream_t st) {
+    constexpr uint32_t one = PreShape<HDP, 1>::kSmem, two = PreShape<HDP, 2>::kSmem;
+    if (p.type == QRAF_TYPE_F32) return launch_kv(kv_prefix_kernel<HDP, 2, 2>, p.pre_ctas, kPreThreads, two, false, p, st);
+    if (p.type == QRAF_TYPE_F16) return launch_kv(kv_prefix_kernel<HDP, 1, 2>, p.pre_ctas, kPreThreads, one, false, p, st);
+    return launch_kv(kv_prefix_kernel<HDP, 1, 1>, p.pre_ctas, kPreThreads, one, false, p, st);
 }
 
 }  // namespace
@@ -302,24 +340,19 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     p.own_tiles = pl.own_tiles;
     p.splits = pl.splits;
     p.own_wide = pl.own_wide;
+    p.pre_ctas = pl.pre_ctas;
+    p.chained = pl.pre_ctas ? 1u : 0u;
     p.part = pl.part_bytes ? static_cast<float*>(workspace_dev) : nullptr;
     const uint32_t hd = kv->head_dim;
-    QRAF_CUDA_TRY(hd <= 64u ? launch_kva<64>(p, pl.items, st)
-                            : hd <= 128u ? launch_kva<128>(p, pl.items, st) : launch_kva<256>(p, pl.items, st));
+    if (p.pre_ctas) QRAF_CUDA_TRY(hd <= 64u ? launch_prefix<64>(p, st) : launch_prefix<128>(p, st));
+    if (pl.items)
+        QRAF_CUDA_TRY(hd <= 64u ? launch_kva<64>(p, pl.items, st)
+                                : hd <= 128u ? launch_kva<128>(p, pl.items, st) : launch_kva<256>(p, pl.items, st));
     if (!p.part) return QRAF_OK;
     const uint64_t out_rows = static_cast<uint64_t>(n) * heads;
     const bool few = pl.p_chunks + pl.splits <= 4u;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(few ? (out_rows + kKvaWarps - 1) / kKvaWarps : out_rows));
-    cfg.blockDim = dim3(kKvaThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    QRAF_CUDA_TRY(counted(few ? cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<1>, p)
-                              : cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<4>, p)));
+    QRAF_CUDA_TRY(few ? launch_kv(kv_attention_join_kernel<1>, (out_rows + kKvaWarps - 1) / kKvaWarps, kKvaThreads, 0, true, p, st)
+                      : launch_kv(kv_attention_join_kernel<4>, out_rows, kKvaThreads, 0, true, p, st));
     return QRAF_OK;
 }
 

@@ -37,6 +37,18 @@ constexpr uint32_t kKvaMinChunk = 128;      // keys per chunk, at least: one ste
 constexpr uint32_t kKvaMaxHeadDim = 256;
 constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own rows together
 
+constexpr uint32_t kPreRows = 128;          // kv_prefix.cuh: query rows of a tile = MMA M
+constexpr uint32_t kPreKeys = 128;          // and keys of a tile
+
+// The range of (unit, key tile) pairs of CTA c of C, unit-major.
+__host__ __device__ __forceinline__ uint64_t pre_start(uint64_t work, uint32_t c, uint32_t C) {
+    return work * c / C;
+}
+// The CTA that has pair x.
+__host__ __device__ __forceinline__ uint32_t pre_owner(uint64_t work, uint64_t x, uint32_t C) {
+    return static_cast<uint32_t>(((x + 1u) * C - 1u) / work);
+}
+
 struct KvAttnParams {
     KvView kv;
     KvRuns runs;             // firsts = visible rows of each slot
@@ -52,7 +64,10 @@ struct KvAttnParams {
     uint32_t group, heads;   // query heads per KV head; all query heads
     float scale_log2;        // scale * log2(e)
     uint32_t max_len;        // the longest visible length allowed
-    uint32_t row_tiles, p_chunks, p_chunk;   // prefix: 16-row tiles of a KV head, chunks and keys in one
+    uint32_t row_tiles;      // prefix: tiles of 16 rows (pre_ctas: of 128) of a KV head
+    uint32_t p_chunks, p_chunk;   // its chunks (pre_ctas: records of a row at most) and keys in one
+    uint32_t pre_ctas;       // CTAs of kv_prefix_kernel, which has the prefix then; 0: kv_attention_kernel has it
+    uint32_t chained;        // kv_attention_kernel was launched as kv_prefix_kernel's dependent
     uint32_t own_tiles, splits;              // own rows: row tiles over all runs (at most), chunks of each (at most)
     uint32_t own_wide;       // own rows in tiles of 16 rows, else 8
     float* part;             // [n * heads][p_chunks + splits][hd + 4]: output, max (log2), sum; nullptr: one chunk a row
@@ -548,16 +563,13 @@ __device__ __forceinline__ bool find_tile(const KvAttnParams& p, uint32_t idx, u
 }
 
 template <uint32_t HDP>
-__global__ void __launch_bounds__(kKvaThreads, 2) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
-    extern __shared__ __align__(16) uint8_t kva_smem[];
-    __shared__ float s_rf[16];
-    pdl_launch_dependents();
+__device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem, float* s_rf) {
     const uint32_t H = p.kv.kv_heads;
     KvaItem it;
     it.sstride = H;
     it.stride = static_cast<uint64_t>(H) * p.kv.hd;
     uint32_t idx = blockIdx.x;
-    const uint32_t p_items = p.row_tiles * H * p.p_chunks;
+    const uint32_t p_items = p.pre_ctas ? 0u : p.row_tiles * H * p.p_chunks;
     if (idx < p_items) {
         const uint32_t q = idx / p.row_tiles, rt = idx - q * p.row_tiles;
         it.chunk = q / H;
@@ -604,6 +616,16 @@ __global__ void __launch_bounds__(kKvaThreads, 2) kv_attention_kernel(const __gr
     else kva_item<HDP, false>(p, it, kva_smem, s_rf);
 }
 
+template <uint32_t HDP>
+__global__ void __launch_bounds__(kKvaThreads, 2) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
+    extern __shared__ __align__(16) uint8_t kva_smem[];
+    __shared__ float s_rf[16];
+    pdl_launch_dependents();
+    kva_cta<HDP>(p, kva_smem, s_rf);
+    // not to end before the prefix's kernel has: the joining kernel waits for this one alone
+    if (p.chained && blockIdx.x == 0u) pdl_wait();
+}
+
 // out = sum_c w_c o_c / sum_c w_c l_c with w_c = 2^(m_c - max m) over a row's chunks,
 // in chunk order.  WPR warps a row: one where a row has few chunks (then a CTA
 // joins four rows), else four, each with every fourth chunk.
@@ -625,20 +647,27 @@ __global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __
         live = b >= 0 && run_ok(p, static_cast<uint32_t>(b), &slot, &len);
         if (live && p.splits) own_chunk(len, p.splits, &own);
     }
-    const uint32_t chunks = live ? p.p_chunks + own : 0u;
+    uint32_t pre = p.p_chunks;
+    if (p.pre_ctas) {   // the CTAs whose ranges meet this row's unit
+        const uint64_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys, work = static_cast<uint64_t>(p.row_tiles) * p.kv.kv_heads * T;
+        const uint32_t h = head / p.group, unit = h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows;
+        pre = pre_owner(work, unit * T + T - 1u, p.pre_ctas) - pre_owner(work, unit * T, p.pre_ctas) + 1u;
+    }
+    const uint32_t chunks = live ? pre + own : 0u;
+    auto at = [&](uint32_t i) { return i < pre ? i : p.p_chunks + (i - pre); };   // record of chunk i
     const uint64_t ld = hd + 4u;
     const float* rec = p.part + row * (p.p_chunks + p.splits) * ld;
     float* w = s_w[warp / WPR];
     float m = -INFINITY;
-    for (uint32_t i = lane; i < chunks; i += 32u) m = fmaxf(m, __ldcg(rec + i * ld + hd));
+    for (uint32_t i = lane; i < chunks; i += 32u) m = fmaxf(m, __ldcg(rec + at(i) * ld + hd));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     float l = 0.0f;
     for (uint32_t i = sub + WPR * lane; i < chunks; i += 32u * WPR) {
-        const float mi = __ldcg(rec + i * ld + hd);
+        const float mi = __ldcg(rec + at(i) * ld + hd);
         const float wi = mi == -INFINITY ? 0.0f : ex2(__fsub_rn(mi, m));
         w[i] = wi;
-        l = fmaf(wi, __ldcg(rec + i * ld + hd + 1u), l);
+        l = fmaf(wi, __ldcg(rec + at(i) * ld + hd + 1u), l);
     }
     l = warp_sum(l);
     __syncwarp();
@@ -650,7 +679,7 @@ __global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __
         for (uint32_t j = 0; j < 2u; ++j) {
             const uint32_t d = 4u * lane + 128u * j;
             if (d >= hd) continue;
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(rec + i * ld + d));
+            const float4 a = __ldcg(reinterpret_cast<const float4*>(rec + at(i) * ld + d));
             if (wi == 0.0f) continue;
             y[j].x = fmaf(wi, a.x, y[j].x);
             y[j].y = fmaf(wi, a.y, y[j].y);
