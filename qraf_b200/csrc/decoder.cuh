@@ -89,14 +89,6 @@ struct AttnParams {
     float scale;               // 1 / sqrt(head_dim)
 };
 
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
-    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Floats of dynamic shared memory: q rotated [G][hd], the new k and v [hd] each,
 // two stages of K and V tiles [kAttnTile][hd + 4] each, probabilities [G][kAttnTile].
 __host__ __device__ constexpr size_t attn_smem_floats(uint32_t G, uint32_t hd) {

@@ -330,6 +330,7 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     p.out_ld = out_ld;
     p.type = type;
     p.wide = wide_rows(out_dev, out_ld, type);
+    p.q_wide = wide_rows(q_dev, q_ld, type);
     p.group = heads / kv->kv_heads;
     p.heads = heads;
     p.scale_log2 = scale * 1.44269504088896340736f;

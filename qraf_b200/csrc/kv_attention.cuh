@@ -61,6 +61,7 @@ struct KvAttnParams {
     void* out;               // [n][heads * hd], rows out_ld elements apart
     uint64_t q_ld, out_ld;
     uint32_t type, wide;     // element type of q and out; every four elements of out aligned for one store
+    uint32_t q_wide;         // and of q for one load
     uint32_t group, heads;   // query heads per KV head; all query heads
     float scale_log2;        // scale * log2(e)
     uint32_t max_len;        // the longest visible length allowed
@@ -111,6 +112,11 @@ __device__ __forceinline__ float load_any(const void* p, uint32_t type, uint64_t
     if (type == QRAF_TYPE_F32) return static_cast<const float*>(p)[i];
     if (type == QRAF_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ float4 load4_any(const void* p, uint32_t type, uint64_t i, bool wide) {
+    if (type == QRAF_TYPE_F32) return load4(static_cast<const float*>(p) + i, wide);
+    if (type == QRAF_TYPE_F16) return load4(static_cast<const __half*>(p) + i, wide);
+    return load4(static_cast<const __nv_bfloat16*>(p) + i, wide);
 }
 __device__ __forceinline__ void store4_any(void* p, uint32_t type, uint64_t i, float4 x, bool wide) {
     if (type == QRAF_TYPE_F32) store4(static_cast<float*>(p) + i, x, wide);

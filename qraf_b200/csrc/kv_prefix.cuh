@@ -15,7 +15,7 @@
 // its own, so that the tensor cores work on one while the other's S becomes P (in
 // place: a thread owns a row, so it overwrites only what it has read).  The maximum
 // that weights refer to moves only when a row exceeds it by 2^4 (then the O row is
-// scaled in TMEM); weights stay below 2^15.  Four warps turn the codes into the
+// scaled in TMEM); weights stay below 2^15.  Eight warps turn the codes into the
 // MMA's shared-memory layout (K as it lies, V transposed, both K-major with the
 // 128-byte swizzle), with the next tile's loads in flight.
 //
@@ -33,8 +33,8 @@
 
 namespace qraf_dev {
 
-constexpr uint32_t kPreThreads = 416;   // two softmax warpgroups, four transform warps, one MMA warp
-constexpr uint32_t kPreWarpXf = 8, kPreWarpMma = 12;
+constexpr uint32_t kPreThreads = 544;   // two softmax warpgroups, eight transform warps, one MMA warp
+constexpr uint32_t kPreWarpXf = 8, kPreWarpMma = 16, kPreXfThreads = 256;
 constexpr float kPreLag = 4.0f;         // log2 of how far a row may exceed the maximum it refers to
 constexpr int32_t kPreUp = 11;          // weights of p = 1 are below 2^11
 
@@ -43,14 +43,17 @@ struct PreShape {
     static constexpr uint32_t kAtoms = HDP / 64u;                      // 64-element (128-byte) column blocks of Q and K
     static constexpr uint32_t kQPart = kPreRows * HDP * 2u;            // one part of Q
     static constexpr uint32_t kKTile = kPreKeys * HDP * 2u;            // one K or V tile in fp16
-    static constexpr uint32_t kQ = 0, kK = kQ + QP * kQPart, kV = kK + 2u * kKTile, kEnd = kV + 2u * kKTile;
+    static constexpr uint32_t kRaw = kPreKeys * HDP;                   // one K or V tile in codes
+    static constexpr uint32_t kStages = 2;                             // of each in flight
+    static constexpr uint32_t kQ = 0, kK = kQ + QP * kQPart, kV = kK + kKTile;
+    static constexpr uint32_t kRawK = kV + kKTile, kRawV = kRawK + kStages * kRaw, kEnd = kRawV + kStages * kRaw;
     static constexpr uint32_t kScales = kEnd;                          // [2][2][128] floats: K and V scales of a slot's tile
     static constexpr uint32_t kRf = kScales + 2048u;                   // [128] row factors
     static constexpr uint32_t kMl = kRf + 512u;                        // [2][2][128]: max and sum of each warpgroup's rows
     static constexpr uint32_t kBars = kMl + 2048u;
     static constexpr uint32_t kSmem = kBars + 128u + 1024u;            // + alignment of the tiles
     static constexpr uint32_t kJoinLd = HDP + 4u;                      // floats per row where the two outputs meet (over K and V)
-    static_assert(kPreRows * kJoinLd * 4u <= 4u * kKTile, "the joined output must fit over the K and V tiles");
+    static_assert(kPreRows * kJoinLd * 4u <= 2u * kKTile + 4u * kRaw, "the joined output must fit over the K and V tiles");
 };
 
 __device__ __forceinline__ void pre_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -94,21 +97,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
         : "memory");
 }
 
-// 32 scores of a row starting at key `c0` of the tile -> weights.  MASK: keys from
-// `valid` on are not there.
-template <bool MASK>
-__device__ __forceinline__ float2 pre_scaled(const float* v, uint32_t j, const float* ks, uint32_t c0, uint32_t valid) {
-    float2 y = f2_mul(make_float2(v[j], v[j + 1u]), *reinterpret_cast<const float2*>(ks + c0 + j));
-    if constexpr (MASK) {
-        if (c0 + j >= valid) y.x = -INFINITY;
-        if (c0 + j + 1u >= valid) y.y = -INFINITY;
-    }
-    return y;
-}
-
 // One tile's softmax for one row (thread): S at TMEM column s_col becomes P in
 // place, the row's maximum and sum move on, O at o_col is scaled where the maximum
-// moved.  `first`: the warpgroup's first tile of the stretch (O is written anew).
+// moved.  ks, vs: the scales of the tile's keys; MASK: keys from `valid` on are not
+// there; `first`: the warpgroup's first tile of the stretch (O is written anew).
 template <uint32_t HDP, uint32_t PP, bool MASK>
 __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, const float* ks, const float* vs, uint32_t valid,
                                             float rf, bool first, float& m, float& l) {
@@ -119,9 +111,17 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
         tmem_ld32(s_col + 32u * c, v);
         tmem_wait_ld();
 #pragma unroll
-        for (uint32_t j = 0; j < 32u; j += 2u) {
-            const float2 y = pre_scaled<MASK>(v, j, ks, 32u * c, valid);
-            ymax = fmaxf(ymax, fmaxf(y.x, y.y));
+        for (uint32_t j = 0; j < 32u; j += 4u) {
+            const float4 k4 = *reinterpret_cast<const float4*>(ks + 32u * c + j);
+            float2 y = f2_mul(make_float2(v[j], v[j + 1u]), make_float2(k4.x, k4.y));
+            float2 z = f2_mul(make_float2(v[j + 2u], v[j + 3u]), make_float2(k4.z, k4.w));
+            if constexpr (MASK) {
+                if (32u * c + j >= valid) y.x = -INFINITY;
+                if (32u * c + j + 1u >= valid) y.y = -INFINITY;
+                if (32u * c + j + 2u >= valid) z.x = -INFINITY;
+                if (32u * c + j + 3u >= valid) z.y = -INFINITY;
+            }
+            ymax = fmaxf(fmaxf(ymax, fmaxf(y.x, y.y)), fmaxf(z.x, z.y));
         }
     }
     const float mt = __fmul_rn(ymax, rf);
@@ -151,21 +151,28 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
         tmem_wait_ld();
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (uint32_t j = 0; j < 32u; j += 2u) {
-            float2 x = f2_fma(pre_scaled<false>(v, j, ks, 32u * c, valid), rf2, m2);
-            if constexpr (MASK) {
-                if (32u * c + j >= valid) x.x = -INFINITY;
-                if (32u * c + j + 1u >= valid) x.y = -INFINITY;
-            }
-            const float2 p = make_float2(ex2(x.x), ex2(x.y));
-            sum = f2_add(sum, p);
-            const float2 w = f2_mul(p, *reinterpret_cast<const float2*>(vs + 32u * c + j));
-            const __half2 h = __floats2half2_rn(w.x, w.y);
-            hi[j / 2u] = *reinterpret_cast<const uint32_t*>(&h);
-            if constexpr (PP == 2u) {
-                const float2 d = f2_fma(__half22float2(h), neg, w);
-                const __half2 r = __floats2half2_rn(d.x, d.y);
-                lo[j / 2u] = *reinterpret_cast<const uint32_t*>(&r);
+        for (uint32_t j = 0; j < 32u; j += 4u) {
+            const float4 k4 = *reinterpret_cast<const float4*>(ks + 32u * c + j);
+            const float4 v4 = *reinterpret_cast<const float4*>(vs + 32u * c + j);
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i += 2u) {
+                const float2 kk = i ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
+                const float2 vv = i ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                float2 x = f2_fma(f2_mul(make_float2(v[j + i], v[j + i + 1u]), kk), rf2, m2);
+                if constexpr (MASK) {
+                    if (32u * c + j + i >= valid) x.x = -INFINITY;
+                    if (32u * c + j + i + 1u >= valid) x.y = -INFINITY;
+                }
+                const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                sum = f2_add(sum, p);
+                const float2 w = f2_mul(p, vv);
+                const __half2 h = __floats2half2_rn(w.x, w.y);
+                hi[(j + i) / 2u] = *reinterpret_cast<const uint32_t*>(&h);
+                if constexpr (PP == 2u) {
+                    const float2 d = f2_fma(__half22float2(h), neg, w);
+                    const __half2 r = __floats2half2_rn(d.x, d.y);
+                    lo[(j + i) / 2u] = *reinterpret_cast<const uint32_t*>(&r);
+                }
             }
         }
         tmem_st16(s_col + 32u * c, hi);   // the chunk's hi parts, then its lo parts
@@ -180,12 +187,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     using S = PreShape<HDP, QP>;
     extern __shared__ uint8_t pre_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pre_smem_raw) + 1023u) & ~uintptr_t(1023));
-    __shared__ uint32_t s_tmem, s_unit, s_fail;
+    __shared__ uint32_t s_tmem, s_fail, s_unit[8];
     float* s_scales = reinterpret_cast<float*>(smem + S::kScales);
     float* s_rf = reinterpret_cast<float*>(smem + S::kRf);
     float* s_ml = reinterpret_cast<float*>(smem + S::kMl);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t *k_ready = bars, *v_ready = bars + 2, *s_ready = bars + 4, *p_ready = bars + 6, *pv_done = bars + 8, *drain = bars + 10;
+    uint64_t *k_ready = bars, *v_ready = bars + 2, *s_ready = bars + 4, *p_ready = bars + 6, *pv_done = bars + 8,
+             *q_ready = bars + 10, *drain = bars + 11;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t hd = p.kv.hd, H = p.kv.kv_heads, G = p.group;
     const uint32_t rows = p.runs.n * G;
@@ -194,12 +202,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     pdl_launch_dependents();
     if (tid == 0) {
         for (uint32_t i = 0; i < 2u; ++i) {
-            mbar_init(&k_ready[i], 4);
-            mbar_init(&v_ready[i], 4);
+            mbar_init(&k_ready[i], kPreXfThreads / 32u);
+            mbar_init(&v_ready[i], kPreXfThreads / 32u);
             mbar_init(&s_ready[i], 1);
             mbar_init(&p_ready[i], 4);
             mbar_init(&pv_done[i], 1);
         }
+        mbar_init(q_ready, 8);
         mbar_init(drain, 1);
         fence_mbar_init();
         s_fail = 0u;
@@ -218,65 +227,58 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     const uint64_t work = static_cast<uint64_t>(p.row_tiles) * H * T;
     const uint64_t w1 = pre_start(work, blockIdx.x + 1u, gridDim.x);
     uint32_t used[2] = {0u, 0u};   // tiles that each slot has had, over the CTA's stretches
+    uint32_t q_phase = 0u;
     bool ok = true;
     for (uint64_t w = pre_start(work, blockIdx.x, gridDim.x); w < w1;) {
         const uint32_t unit = static_cast<uint32_t>(w / T), tile0 = static_cast<uint32_t>(w - static_cast<uint64_t>(unit) * T);
         const uint32_t n = static_cast<uint32_t>(min(static_cast<uint64_t>(T - tile0), w1 - w));
         const uint32_t h = unit / p.row_tiles, row0 = (unit - h * p.row_tiles) * kPreRows;
         const uint32_t key0 = tile0 * kPreKeys, key1 = min(p.prefix_len, (tile0 + n) * kPreKeys);
-        const int8_t* pk = p.pk + static_cast<uint64_t>(h) * hd;
-        const int8_t* pv = p.pv + static_cast<uint64_t>(h) * hd;
-        const float* pks = p.pks + h;
-        const float* pvs = p.pvs + h;
-
-        // ── the query rows (softmax warps) and the unit of the V scales (transform warps) ──
-        if (tid == 0) s_unit = 0u;
-        __syncthreads();
-        if (warp < kPreWarpXf) {
-            const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-            constexpr uint32_t LPR = HDP / 4u, RPW = 32u / LPR;   // lanes per row, rows per warp access
-            const uint32_t l = lane % LPR;
-#pragma unroll 4
-            for (uint32_t i = 0; i < 16u / RPW; ++i) {
-                const uint32_t r = warp * 16u + i * RPW + lane / LPR, row = row0 + r;
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                if (row < rows && 4u * l < hd) {
-                    const uint32_t t = row / G;
-                    const uint64_t at = static_cast<uint64_t>(t) * p.q_ld + static_cast<uint64_t>(h * G + (row - t * G)) * hd + 4u * l;
-#pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) x[k] = __fmul_rn(load_any(p.q, p.type, at + k), sign);
-                }
-                float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-                for (uint32_t o = LPR / 2u; o > 0u; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-                // the largest becomes 2^10 .. 2^11, as in kva_item
-                const int32_t e = max(exponent_bits(m), 11);
-                const float up = pow2_bits(264 - e);
-                if (l == 0u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
-                uint32_t hi[2], lo[2];
-                split_f16(__fmul_rn(x[0], up), __fmul_rn(x[1], up), hi[0], lo[0]);
-                split_f16(__fmul_rn(x[2], up), __fmul_rn(x[3], up), hi[1], lo[1]);
-                const uint32_t off = (l >> 4) * (kPreRows * 128u) + tc_sw128_off(r, (l & 15u) >> 1) + 8u * (l & 1u);
-                *reinterpret_cast<uint2*>(smem + S::kQ + off) = make_uint2(hi[0], hi[1]);
-                if constexpr (QP == 2u) *reinterpret_cast<uint2*>(smem + S::kQ + S::kQPart + off) = make_uint2(lo[0], lo[1]);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        } else if (warp < kPreWarpMma) {
-            uint32_t most = 0u;
-            for (uint32_t key = key0 + tid - kPreWarpXf * 32u; key < key1; key += 128u) {
-                const uint32_t e = static_cast<uint32_t>(exponent_bits(__ldg(pvs + static_cast<uint64_t>(key) * H)));
-                if (e < 255u) most = max(most, e);
-            }
-            most = __reduce_max_sync(0xFFFFFFFFu, most);
-            if (lane == 0u) atomicMax(&s_unit, most);
-        }
-        __syncthreads();
-        // every V scale is below 2^(eb - 126); scaled by 2^(kPreUp + 126 - eb) they are below 2^kPreUp
-        const int32_t eb = max(static_cast<int32_t>(s_unit), 14);
         float m = -INFINITY, l = 0.0f;
         const uint32_t slot = warp >> 2;   // of a softmax warp
 
         if (warp < kPreWarpXf) {
+            // ── the query rows: 16 a warp, eight loads in flight ──
+            constexpr uint32_t LPR = HDP / 4u, RPW = 32u / LPR, RB = 8u / RPW;   // lanes per row, rows per access, accesses per batch
+            const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+            const uint32_t ql = lane % LPR;
+#pragma unroll 1
+            for (uint32_t half = 0; half < 2u; ++half) {
+                float4 x[RB];
+#pragma unroll
+                for (uint32_t i = 0; i < RB; ++i) {
+                    const uint32_t row = row0 + warp * 16u + half * 8u + i * RPW + lane / LPR;
+                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (row < rows && 4u * ql < hd) {
+                        const uint32_t t = row / G;
+                        x[i] = load4_any(p.q, p.type,
+                                         static_cast<uint64_t>(t) * p.q_ld + static_cast<uint64_t>(h * G + (row - t * G)) * hd + 4u * ql,
+                                         p.q_wide);
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < RB; ++i) {
+                    const uint32_t r = warp * 16u + half * 8u + i * RPW + lane / LPR;
+                    float mx = absmax4(x[i], 0.0f);
+#pragma unroll
+                    for (uint32_t o = LPR / 2u; o > 0u; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+                    // the largest becomes 2^10 .. 2^11, as in kva_item
+                    const int32_t e = max(exponent_bits(mx), 11);
+                    const float up = __fmul_rn(pow2_bits(264 - e), sign);
+                    if (ql == 0u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
+                    uint32_t hi[2], lo[2];
+                    split_f16(__fmul_rn(x[i].x, up), __fmul_rn(x[i].y, up), hi[0], lo[0]);
+                    split_f16(__fmul_rn(x[i].z, up), __fmul_rn(x[i].w, up), hi[1], lo[1]);
+                    const uint32_t off = (ql >> 4) * (kPreRows * 128u) + tc_sw128_off(r, (ql & 15u) >> 1) + 8u * (ql & 1u);
+                    *reinterpret_cast<uint2*>(smem + S::kQ + off) = make_uint2(hi[0], hi[1]);
+                    if constexpr (QP == 2u) *reinterpret_cast<uint2*>(smem + S::kQ + S::kQPart + off) = make_uint2(lo[0], lo[1]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(q_ready);
+            asm volatile("bar.sync 2, 256;" ::: "memory");   // the row factors, across warps
+
             // ── softmax ──
             const uint32_t lane_row = (warp & 3u) * 32u;   // TMEM lanes of this warp
             const uint32_t s_col = tmem + (lane_row << 16) + slot * 128u, o_col = tmem + (lane_row << 16) + 256u + slot * 128u;
@@ -295,106 +297,194 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             }
         } else if (warp < kPreWarpMma) {
             // ── codes -> fp16 tiles ──
+            // The MMAs run ... PV(t) S(t+2) PV(t+1) S(t+3) ...: V(t) is made while S(t+1)
+            // runs and K(t+2) while PV(t) does, so one fp16 tile of each is enough; two
+            // tiles of codes of each are in flight behind them (cp.async).
             const uint32_t xw = warp - kPreWarpXf, xt = tid - kPreWarpXf * 32u;
-            const float vup = pow2_bits(kPreUp + 253 - eb);
-            constexpr uint32_t KL = HDP / 16u;    // 16-byte loads of K a thread
-            constexpr uint32_t VB = HDP / 32u;    // 32-dim blocks of V
-            uint4 kr[KL];
-            uint32_t vr[VB][8];
-            float ksc = 0.0f, vsc = 0.0f;
-            // K: lane (unit a of 16 codes, key) so that eight consecutive lanes store to
-            // eight different 16-byte columns of the swizzled rows
-            const uint32_t ka = lane & 3u;
-            auto k_place = [&](uint32_t i, uint32_t& key, uint32_t& u) {   // key of the tile, 16-code unit of its row
-                if constexpr (HDP == 128u) {
-                    key = xw * 32u + i * 4u + ((lane >> 2) & 1u) + 2u * (lane >> 4);
-                    u = ka + 4u * ((lane >> 3) & 1u);
-                } else {
-                    key = xw * 32u + i * 8u + (lane >> 2);
-                    u = ka;
+            constexpr uint32_t U = HDP / 16u;                      // 16-byte units of a row
+            constexpr uint32_t KL = kPreKeys * U / kPreXfThreads;  // units of a tile a thread
+            constexpr uint32_t VB = HDP / 64u;                     // 32-dim blocks of V a warp
+            const int8_t* pk = p.pk + static_cast<uint64_t>(h) * hd;
+            const int8_t* pv = p.pv + static_cast<uint64_t>(h) * hd;
+            const float* my_scale = (xt < kPreKeys ? p.pks : p.pvs) + h;   // threads 0-127: K's, 128-255: V's
+            const uint32_t last = key1 - 1u;
+            // K: lane (unit of 16 codes, key), so that eight consecutive lanes load from and
+            // store to eight different 16-byte columns; a thread loads what it converts.
+            // Access i is key k_key + KI i of the tile, at raw offset k_src + i KI HDP.
+            constexpr uint32_t KI = 32u / U;   // keys per access
+            const uint32_t k_kk = HDP == 128u ? ((lane >> 2) & 1u) + 2u * (lane >> 4) : lane >> 2;
+            const uint32_t k_u = HDP == 128u ? (lane & 3u) + 4u * ((lane >> 3) & 1u) : lane & 3u;
+            const uint32_t k_key = xw * 16u + k_kk;
+            const uint32_t k_src = k_key * HDP + 16u * (HDP == 128u ? k_u ^ (4u * (k_kk & 1u)) : k_u);
+            // fp16 row of key 16 xw + i KI + k_kk: 8-row atom 2 xw + (i KI) / 8, row (i KI & 7) + k_kk
+            const uint32_t k_dst = (k_u >> 2) * (kPreKeys * 128u) + xw * 2048u + k_kk * 128u;
+            const uint32_t k_col = (2u * (k_u & 3u)) ^ k_kk;   // its 16-byte column, ^ (i KI & 7), ^ 1 for the second eight codes
+            const bool k_in = 16u * k_u < hd;
+            // V: unit u of key k lies at unit u ^ 2 (k / 8) so that a lane's four-byte reads of
+            // four octets of keys meet four groups of banks
+            const uint32_t vf_u = xt % U, vf_key = xt / U;   // fetch: unit, first key; keys kPreXfThreads / U apart
+            const bool vf_in = 16u * vf_u < hd;
+            // conversion: lane (4 dims dq, octet of keys ko) of 32 keys x 32 dims
+            const uint32_t dq = (lane & 1u) + 2u * (lane >> 3), ko = (lane >> 1) & 3u, kb = xw & 3u, vb0 = xw >> 2;
+            const uint32_t v_src = (32u * kb + 8u * ko) * HDP + 4u * dq;   // + i HDP + 32 (block ^ ko)
+            // transposed row 32 block + 4 dq + j, 64 keys per 128-byte row: 16-byte column = octet of keys
+            const uint32_t v_dst = (kb >> 1) * (HDP * 128u) + (dq >> 1) * 1024u + (dq & 1u) * 512u;
+            const uint32_t v_col = (4u * (kb & 1u) + ko) ^ (4u * (dq & 1u));   // ^ j
+            auto fetch_k = [&](uint32_t t) {
+                if (t < n && k_in) {
+                    uint8_t* dst = smem + S::kRawK + (t & 1u) * S::kRaw + k_src;
+                    const uint32_t k0 = key0 + t * kPreKeys + k_key;
+#pragma unroll
+                    for (uint32_t i = 0; i < KL; ++i)
+                        cp_async16(dst + i * KI * HDP, pk + static_cast<uint64_t>(min(k0 + i * KI, last)) * stride + 16u * k_u);
                 }
+                cp_async_commit();
             };
-            // V: lane (4 dims, octet of keys), likewise
-            const uint32_t dq = (lane & 1u) + 2u * (lane >> 3), ko = (lane >> 1) & 3u;
-            auto load = [&](uint32_t t) {
-                const uint32_t k0 = key0 + t * kPreKeys, last = key1 - 1u;
+            auto fetch_v = [&](uint32_t t) {
+                if (t < n && vf_in) {
+                    uint8_t* dst = smem + S::kRawV + (t & 1u) * S::kRaw;
+                    const uint32_t k0 = key0 + t * kPreKeys;
 #pragma unroll
-                for (uint32_t i = 0; i < KL; ++i) {
-                    uint32_t key, u;
-                    k_place(i, key, u);
-                    kr[i] = 16u * u < hd ? __ldg(reinterpret_cast<const uint4*>(
-                                               pk + static_cast<uint64_t>(min(k0 + key, last)) * stride + 16u * u))
-                                         : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-                for (uint32_t b = 0; b < VB; ++b)
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) {
-                        const uint32_t d = 32u * b + 4u * dq;
-                        vr[b][i] = d < hd ? __ldg(reinterpret_cast<const uint32_t*>(
-                                                pv + static_cast<uint64_t>(min(k0 + 32u * xw + 8u * ko + i, last)) * stride + d))
-                                          : 0u;
+                    for (uint32_t i = 0; i < KL; ++i) {
+                        const uint32_t key = vf_key + i * (kPreXfThreads / U);
+                        cp_async16(dst + key * HDP + 16u * (vf_u ^ (2u * ((key >> 3) & (U / 2u - 1u)))),
+                                   pv + static_cast<uint64_t>(min(k0 + key, last)) * stride + 16u * vf_u);
                     }
-                const uint32_t key = k0 + xt;
-                ksc = key < key1 ? __ldg(pks + static_cast<uint64_t>(key) * H) : 0.0f;
-                vsc = key < key1 ? __fmul_rn(__ldg(pvs + static_cast<uint64_t>(key) * H), vup) : 0.0f;
+                }
+                cp_async_commit();
             };
-            load(0);
-            for (uint32_t t = 0; ok && t < n; ++t) {
+            // a barrier of these warps that tells whether all of them are fine, so that they
+            // give up together when a wait runs out
+            auto all_xf = [](bool fine) {
+                uint32_t r;
+                asm volatile(
+                    "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                    "bar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                    : "=r"(r)
+                    : "r"(fine ? 1u : 0u)
+                    : "memory");
+                return r != 0u;
+            };
+            // groups in order K0 K1 V0 V1 K2 K3 V2 K4 V3 K5 ..., one each even past the last tile
+            fetch_k(0);
+            fetch_k(1);
+            fetch_v(0);
+            fetch_v(1);
+            // the unit of the weights: every V scale of the stretch is below 2^(eb - 126)
+            // (an infinity or NaN has no say)
+            uint32_t most = 0u;
+            for (uint32_t key = key0 + xt; key < key1; key += 4u * kPreXfThreads) {
+                float v[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i)
+                    v[i] = __ldg(p.pvs + h + static_cast<uint64_t>(min(key + i * kPreXfThreads, last)) * H);
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i) {
+                    const uint32_t e = static_cast<uint32_t>(exponent_bits(v[i]));
+                    if (e < 255u) most = max(most, e);
+                }
+            }
+            most = __reduce_max_sync(0xFFFFFFFFu, most);
+            if (lane == 0u) s_unit[xw] = most;
+            all_xf(true);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
+            const float up = xt < kPreKeys ? 1.0f : pow2_bits(kPreUp + 253 - max(static_cast<int32_t>(most), 14));
+            float scale = 0.0f;   // this thread's scale of the next K tile's key xt & 127
+            auto fetch_scale = [&](uint32_t t) {
+                const uint32_t key = key0 + t * kPreKeys + (xt & (kPreKeys - 1u));
+                scale = t < n && key < key1 ? __ldg(my_scale + static_cast<uint64_t>(key) * H) : 0.0f;
+            };
+            auto make_k = [&](uint32_t t) {
                 const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
-                // the slot's K tile, scales and V tile are free once its previous tile's
-                // S is there, its P is written and its O is done
-                if (j > 0u) ok = warp_wait(&s_ready[sl], (j - 1u) & 1u) && warp_wait(&p_ready[sl], (j - 1u) & 1u);
-                if (!ok) break;
-                uint8_t* kt = smem + S::kK + sl * S::kKTile;
+                if (t == 2u) cp_async_wait<2>();   // behind K2 came K3 and V2 only
+                else cp_async_wait<3>();
+                const uint8_t* raw = smem + S::kRawK + sl * S::kRaw + k_src;
+                uint4 c[KL];
+#pragma unroll
+                for (uint32_t i = 0; i < KL; ++i)
+                    c[i] = k_in ? *reinterpret_cast<const uint4*>(raw + i * KI * HDP) : make_uint4(0u, 0u, 0u, 0u);
+                if (t > 0u) {   // the K tile is free once the previous tile's S is there
+                    const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
+                    if (!warp_wait(&s_ready[ps], pj & 1u)) return false;
+                }
+                // and the slot's scales once its previous P is written
+                if (j > 0u && !warp_wait(&p_ready[sl], (j - 1u) & 1u)) return false;
+                uint8_t* dst = smem + S::kK + k_dst;
 #pragma unroll
                 for (uint32_t i = 0; i < KL; ++i) {
-                    uint32_t key, u;
-                    k_place(i, key, u);
-                    uint8_t* atom = kt + (u >> 2) * (kPreKeys * 128u);
-                    const uint32_t a0 = kr[i].x ^ 0x80808080u, a1 = kr[i].y ^ 0x80808080u, a2 = kr[i].z ^ 0x80808080u,
-                                   a3 = kr[i].w ^ 0x80808080u;
-                    *reinterpret_cast<uint4*>(atom + tc_sw128_off(key, 2u * (u & 3u))) =
+                    uint8_t* row = dst + (i * KI >> 3) * 1024u + (i * KI & 7u) * 128u;
+                    const uint32_t col = k_col ^ (i * KI & 7u);
+                    const uint32_t a0 = c[i].x ^ 0x80808080u, a1 = c[i].y ^ 0x80808080u, a2 = c[i].z ^ 0x80808080u,
+                                   a3 = c[i].w ^ 0x80808080u;
+                    *reinterpret_cast<uint4*>(row + (col << 4)) =
                         make_uint4(codes_f16<0x4140u>(a0), codes_f16<0x4342u>(a0), codes_f16<0x4140u>(a1), codes_f16<0x4342u>(a1));
-                    *reinterpret_cast<uint4*>(atom + tc_sw128_off(key, 2u * (u & 3u) + 1u)) =
+                    *reinterpret_cast<uint4*>(row + ((col ^ 1u) << 4)) =
                         make_uint4(codes_f16<0x4140u>(a2), codes_f16<0x4342u>(a2), codes_f16<0x4140u>(a3), codes_f16<0x4342u>(a3));
                 }
-                s_scales[sl * 256u + xt] = ksc;
-                s_scales[sl * 256u + 128u + xt] = vsc;
+                s_scales[sl * 256u + xt] = __fmul_rn(scale, up);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&k_ready[sl]);
-                if (j > 0u) ok = warp_wait(&pv_done[sl], (j - 1u) & 1u);
-                if (!ok) break;
-                // V transposed: row = dim, 64 keys per 128-byte row; eight keys are one 16-byte column
-                uint8_t* vt = smem + S::kV + sl * S::kKTile + (xw >> 1) * (HDP * 128u);
-                const uint32_t chunk = 4u * (xw & 1u) + ko;
+                fetch_k(t + 2u);
+                fetch_scale(t + 1u);
+                return true;
+            };
+            auto make_v = [&](uint32_t t, bool fine) {
+                const uint32_t sl = t & 1u;
+                cp_async_wait<3>();
+                if (!all_xf(fine)) return false;   // the other threads' pieces have come too
+                const uint8_t* raw = smem + S::kRawV + sl * S::kRaw + v_src;
+                uint32_t x[VB][8];
 #pragma unroll
                 for (uint32_t b = 0; b < VB; ++b) {
-                    uint32_t x[8];
+                    const uint32_t block = vb0 + 2u * b;
+                    const bool in = 32u * block + 4u * dq < hd;
+                    const uint8_t* src = raw + 32u * (block ^ (ko & (U / 2u - 1u)));
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) x[i] = vr[b][i] ^ 0x80808080u;
+                    for (uint32_t i = 0; i < 8u; ++i) x[b][i] = in ? *reinterpret_cast<const uint32_t*>(src + i * HDP) ^ 0x80808080u : 0x80808080u;
+                }
+                if (t > 0u) {   // the V tile is free once the previous tile's O is done
+                    const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
+                    fine = warp_wait(&pv_done[ps], pj & 1u);
+                }
+#pragma unroll
+                for (uint32_t b = 0; b < VB; ++b) {
+                    if (!fine) break;
+                    uint8_t* dst = smem + S::kV + v_dst + (vb0 + 2u * b) * 4096u;
                     uint32_t c01[4], c23[4];   // keys 2 i and 2 i + 1, byte-interleaved: dims 0-1 and 2-3
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) {
-                        c01[i] = __byte_perm(x[2u * i], x[2u * i + 1u], 0x5140u);
-                        c23[i] = __byte_perm(x[2u * i], x[2u * i + 1u], 0x7362u);
+                        c01[i] = __byte_perm(x[b][2u * i], x[b][2u * i + 1u], 0x5140u);
+                        c23[i] = __byte_perm(x[b][2u * i], x[b][2u * i + 1u], 0x7362u);
                     }
-                    const uint32_t d = 32u * b + 4u * dq;
-                    *reinterpret_cast<uint4*>(vt + tc_sw128_off(d, chunk)) =
+                    *reinterpret_cast<uint4*>(dst + (v_col << 4)) =
                         make_uint4(codes_f16<0x4140u>(c01[0]), codes_f16<0x4140u>(c01[1]), codes_f16<0x4140u>(c01[2]), codes_f16<0x4140u>(c01[3]));
-                    *reinterpret_cast<uint4*>(vt + tc_sw128_off(d + 1u, chunk)) =
+                    *reinterpret_cast<uint4*>(dst + 128u + ((v_col ^ 1u) << 4)) =
                         make_uint4(codes_f16<0x4342u>(c01[0]), codes_f16<0x4342u>(c01[1]), codes_f16<0x4342u>(c01[2]), codes_f16<0x4342u>(c01[3]));
-                    *reinterpret_cast<uint4*>(vt + tc_sw128_off(d + 2u, chunk)) =
+                    *reinterpret_cast<uint4*>(dst + 256u + ((v_col ^ 2u) << 4)) =
                         make_uint4(codes_f16<0x4140u>(c23[0]), codes_f16<0x4140u>(c23[1]), codes_f16<0x4140u>(c23[2]), codes_f16<0x4140u>(c23[3]));
-                    *reinterpret_cast<uint4*>(vt + tc_sw128_off(d + 3u, chunk)) =
+                    *reinterpret_cast<uint4*>(dst + 384u + ((v_col ^ 3u) << 4)) =
                         make_uint4(codes_f16<0x4342u>(c23[0]), codes_f16<0x4342u>(c23[1]), codes_f16<0x4342u>(c23[2]), codes_f16<0x4342u>(c23[3]));
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0u) mbar_arrive(&v_ready[sl]);
-                if (t + 1u < n) load(t + 1u);
+                if (lane == 0u && fine) mbar_arrive(&v_ready[sl]);
+                if (!all_xf(fine)) return false;   // every piece of the stage has been read
+                fetch_v(t + 2u);
+                return true;
+            };
+            fetch_scale(0);
+            ok = make_k(0);
+            if (ok && n > 1u) ok = make_k(1);
+            else cp_async_commit();
+            for (uint32_t t = 0; t < n; ++t) {
+                ok = make_v(t, ok);
+                if (!ok) break;   // all of these warps
+                if (t + 2u < n) ok = make_k(t + 2u);
+                else cp_async_commit();
             }
+            cp_async_wait<0>();
         } else {
             // ── MMA issue ──
             const uint32_t base = smem_u32(smem);
@@ -411,14 +501,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                         for (uint32_t k = 0; k < HDP / 16u; ++k)
                             tc_mma_f16(tmem + sl * 128u,
                                        tc_smem_desc(base + S::kQ + part * S::kQPart + (k >> 2) * (kPreRows * 128u) + (k & 3u) * 32u),
-                                       tc_smem_desc(base + S::kK + sl * S::kKTile + (k >> 2) * (kPreKeys * 128u) + (k & 3u) * 32u),
+                                       tc_smem_desc(base + S::kK + (k >> 2) * (kPreKeys * 128u) + (k & 3u) * 32u),
                                        idesc_s, part + k > 0u);
                     tc_commit(&s_ready[sl]);
                 }
                 __syncwarp();
                 return true;
             };
-            ok = scores(0);
+            ok = warp_wait(q_ready, q_phase) && scores(0);
             if (ok && n > 1u) ok = scores(1);
             for (uint32_t t = 0; ok && t < n; ++t) {
                 const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
@@ -431,7 +521,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
 #pragma unroll
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
                             pre_mma_ts(tmem + 256u + sl * 128u, tmem + sl * 128u + 32u * (k >> 1) + 16u * part + 8u * (k & 1u),
-                                       tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
+                                       tc_smem_desc(base + S::kV + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
                                        t >= 2u || part + k > 0u);
                     tc_commit(&pv_done[sl]);
                 }
@@ -442,12 +532,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         }
         used[0] += (n + 1u) / 2u;
         used[1] += n / 2u;
-        // ── both outputs of a row meet in shared memory (over K and V) and leave as one record ──
-        if (warp < kPreWarpXf && ok && slot < n) {
-            ok = warp_wait(&pv_done[slot], (used[slot] - 1u) & 1u);
+        q_phase ^= 1u;
+        // ── the two outputs of a row join in shared memory (over K and V) and leave as one record ──
+        const bool both = n > 1u;
+        if (warp < kPreWarpXf && ok) {
+            ok = warp_wait(&pv_done[0], (used[0] - 1u) & 1u) && (!both || warp_wait(&pv_done[1], (used[1] - 1u) & 1u));
             tc_fence_after();
             const uint32_t r = (warp & 3u) * 32u + lane;
-            s_ml[slot * 256u + r] = m;
+            s_ml[slot * 256u + r] = m;   // -inf and 0 where the slot had no tile
             s_ml[slot * 256u + 128u + r] = l;
         }
         if (!ok) s_fail = 1u;
@@ -461,54 +553,62 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             break;
         }
         float* jo = reinterpret_cast<float*>(smem + S::kK);   // [128][HDP + 4]
-        const float unit_f = pow2_bits(eb - kPreUp + 1);
-        const bool both = n > 1u;
-        for (uint32_t turn = both ? 1u : 0u;; --turn) {   // slot 1 stores, slot 0 adds
-            if (warp < kPreWarpXf && slot == turn) {
-                const uint32_t r = (warp & 3u) * 32u + lane;
-                const float m_all = both ? fmaxf(s_ml[r], s_ml[256u + r]) : m;
-                const float f = __fmul_rn(ex2(__fsub_rn(m, m_all)), unit_f);
-                const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 256u + slot * 128u;
-                float* dst = jo + r * S::kJoinLd;
+        if (warp < kPreWarpXf) {   // each warpgroup has half of the columns
+            uint32_t most = 14u;
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
+            const uint32_t r = (warp & 3u) * 32u + lane;
+            const float m0 = s_ml[r], m1 = s_ml[256u + r], m_all = fmaxf(m0, m1);
+            const float e0 = ex2(__fsub_rn(m0, m_all)), e1 = both ? ex2(__fsub_rn(m1, m_all)) : 0.0f;
+            const float unit_f = pow2_bits(static_cast<int32_t>(most) - kPreUp + 1);
+            const float2 f0 = make_float2(__fmul_rn(e0, unit_f), __fmul_rn(e0, unit_f));
+            const float2 f1 = make_float2(__fmul_rn(e1, unit_f), __fmul_rn(e1, unit_f));
+            const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 256u;
+            float* dst = jo + r * S::kJoinLd;
 #pragma unroll 1
-                for (uint32_t c = 0; c < HDP; c += 32u) {
-                    float v[32];
-                    tmem_ld32(o_col + c, v);
+            for (uint32_t c = slot * (HDP / 2u); c < (slot + 1u) * (HDP / 2u); c += 32u) {
+                float v[32];
+                tmem_ld32(o_col + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (uint32_t k = 0; k < 32u; k += 2u) {
+                    const float2 y = f2_mul(make_float2(v[k], v[k + 1u]), f0);
+                    v[k] = y.x;
+                    v[k + 1u] = y.y;
+                }
+                if (both) {
+                    float z[32];
+                    tmem_ld32(o_col + 128u + c, z);
                     tmem_wait_ld();
 #pragma unroll
-                    for (uint32_t k = 0; k < 32u; k += 4u) {
-                        float4 y = make_float4(__fmul_rn(v[k], f), __fmul_rn(v[k + 1u], f), __fmul_rn(v[k + 2u], f),
-                                               __fmul_rn(v[k + 3u], f));
-                        float4* at = reinterpret_cast<float4*>(dst + c + k);
-                        if (both && turn == 0u) {
-                            const float4 z = *at;
-                            y = make_float4(__fadd_rn(y.x, z.x), __fadd_rn(y.y, z.y), __fadd_rn(y.z, z.z), __fadd_rn(y.w, z.w));
-                        }
-                        *at = y;
+                    for (uint32_t k = 0; k < 32u; k += 2u) {
+                        const float2 y = f2_fma(make_float2(z[k], z[k + 1u]), f1, make_float2(v[k], v[k + 1u]));
+                        v[k] = y.x;
+                        v[k + 1u] = y.y;
                     }
                 }
-                if (turn == 0u) {
-                    float l_all = l;
-                    if (both)
-                        l_all = __fadd_rn(__fmul_rn(l, ex2(__fsub_rn(m, m_all))),
-                                          __fmul_rn(s_ml[256u + 128u + r], ex2(__fsub_rn(s_ml[256u + r], m_all))));
-                    dst[HDP] = m_all;
-                    dst[HDP + 1u] = l_all;
-                }
+#pragma unroll
+                for (uint32_t k = 0; k < 32u; k += 4u)
+                    *reinterpret_cast<float4*>(dst + c + k) = make_float4(v[k], v[k + 1u], v[k + 2u], v[k + 3u]);
+            }
+            if (slot == 0u) {
+                dst[HDP] = m_all;
+                dst[HDP + 1u] = fmaf(e0, s_ml[128u + r], both ? __fmul_rn(e1, s_ml[256u + 128u + r]) : 0.0f);
             }
             tc_fence_before();
-            __syncthreads();
-            if (turn == 0u) break;
         }
+        __syncthreads();
         const uint32_t chunk = blockIdx.x - pre_owner(work, static_cast<uint64_t>(unit) * T, gridDim.x);
+#pragma unroll 4
         for (uint32_t r = warp; r < kPreRows; r += kPreThreads / 32u) {
             const uint32_t row = row0 + r;
-            if (row >= rows) break;
-            const uint32_t t = row / G, head = h * G + (row - t * G);
-            float* rec = p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + chunk) * (hd + 4u);
-            const float* src = jo + r * S::kJoinLd;
-            if (4u * lane < hd) *reinterpret_cast<float4*>(rec + 4u * lane) = *reinterpret_cast<const float4*>(src + 4u * lane);
-            if (lane == 0u) *reinterpret_cast<float2*>(rec + hd) = *reinterpret_cast<const float2*>(src + HDP);
+            if (row < rows) {
+                const uint32_t t = row / G, head = h * G + (row - t * G);
+                float* rec = p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + chunk) * (hd + 4u);
+                const float* src = jo + r * S::kJoinLd;
+                if (4u * lane < hd) *reinterpret_cast<float4*>(rec + 4u * lane) = *reinterpret_cast<const float4*>(src + 4u * lane);
+                if (lane == 0u) *reinterpret_cast<float2*>(rec + hd) = *reinterpret_cast<const float2*>(src + HDP);
+            }
         }
         w += n;
         if (w < w1) {
