@@ -137,12 +137,12 @@ int ensure_device(int* dev_out, DeviceInfo** info_out) {
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<64>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<128>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<256>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 1, 1>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 1, 2>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, 2, 2>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 1, 1>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 1, 2>, lim));
-        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, 2, 2>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, float>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, __half>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<64, __nv_bfloat16>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, float>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, __half>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_prefix_kernel<128, __nv_bfloat16>, lim));
         QRAF_CUDA_TRY(allow_smem(token_probs_kernel, lim));
         d.ready = true;
     }

@@ -107,12 +107,14 @@ int kv_io(const qraf_kv_t* kv, const void* k, const void* v, uint32_t type, uint
 #ifndef PRE_MIN_ROWS
 #define PRE_MIN_ROWS 17
 #endif
-bool prefix_on_tiles(uint64_t rows, uint32_t hd, uint32_t prefix_len) {
-    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 128u;
+bool prefix_on_tiles(uint64_t rows, uint64_t kv_heads, uint32_t hd, uint64_t prefix_len) {
+    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 128u &&
+           (rows / kPreRows + 1u) * kv_heads * (prefix_len / kPreKeys + 1u) < (1ull << 31);   // 32-bit ranges
 }
 
 struct KvaPlan {
     uint32_t row_tiles = 0, p_chunks = 0, p_chunk = 0, own_tiles = 0, splits = 0, own_wide = 0, pre_ctas = 0;
+    uint32_t pre_base = 0, pre_extra = 0;
     uint64_t items = 0, part_bytes = 0;
 };
 
@@ -138,14 +140,24 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         items += groups * pl->splits;
     }
     pl->own_tiles = static_cast<uint32_t>(own_tiles);
-    if (prefix_len && prefix_on_tiles(rows, hd, prefix_len)) {
+    if (prefix_len && prefix_on_tiles(rows, kv_heads, hd, prefix_len)) {
         pl->row_tiles = static_cast<uint32_t>((rows + kPreRows - 1u) / kPreRows);
-        const uint64_t units = static_cast<uint64_t>(pl->row_tiles) * kv_heads;
-        const uint64_t work = units * ((prefix_len + kPreKeys - 1u) / kPreKeys);
-        pl->pre_ctas = static_cast<uint32_t>(std::min<uint64_t>(work, static_cast<uint64_t>(sm_count)));
-        // a unit's tiles start inside one CTA's range and end inside another's
-        const uint64_t T = work / units;
-        pl->p_chunks = static_cast<uint32_t>(std::min<uint64_t>(T, (T * pl->pre_ctas + work - 1u) / work + 1u));
+        const uint32_t T = (prefix_len + kPreKeys - 1u) / kPreKeys, work = pl->row_tiles * kv_heads * T;
+        // One CTA an SM, each with two tiles at least (its two warpgroups).  Beginning and
+        // ending a stretch of one unit takes about as long as 2.5 tiles, so ranges that
+        // meet two units are worth it only where whole numbers of CTAs a unit would be
+        // much longer.
+        const uint32_t units = pl->row_tiles * kv_heads, sms = static_cast<uint32_t>(sm_count);
+        pl->pre_ctas = std::min(std::max(1u, (work + 1u) / 2u), sms);
+        if (units <= sms) {
+            const uint32_t per = std::max(1u, std::min(sms / units, (T + 1u) / 2u));
+            const uint32_t alone = 2u * ((T + per - 1u) / per) + 5u, shared = 2u * ((work + pl->pre_ctas - 1u) / pl->pre_ctas) + 10u;
+            if (alone <= shared) pl->pre_ctas = units * per;
+        }
+        pl->pre_base = work / pl->pre_ctas;
+        pl->pre_extra = work % pl->pre_ctas;
+        // a unit's T tiles may start inside one CTA's range and end inside another's
+        pl->p_chunks = std::min(T, (T + pl->pre_base - 1u) / pl->pre_base + 1u);
     } else if (prefix_len) {
         pl->row_tiles = static_cast<uint32_t>((rows + 15u) / 16u);
         const uint64_t units = static_cast<uint64_t>(pl->row_tiles) * kv_heads;
@@ -193,9 +205,9 @@ cudaError_t launch_kva(const KvAttnParams& p, uint64_t items, cudaStream_t st) {
 template <uint32_t HDP>
 cudaError_t launch_prefix(const KvAttnParams& p, cudaStream_t st) {
     constexpr uint32_t one = PreShape<HDP, 1>::kSmem, two = PreShape<HDP, 2>::kSmem;
-    if (p.type == QRAF_TYPE_F32) return launch_kv(kv_prefix_kernel<HDP, 2, 2>, p.pre_ctas, kPreThreads, two, false, p, st);
-    if (p.type == QRAF_TYPE_F16) return launch_kv(kv_prefix_kernel<HDP, 1, 2>, p.pre_ctas, kPreThreads, one, false, p, st);
-    return launch_kv(kv_prefix_kernel<HDP, 1, 1>, p.pre_ctas, kPreThreads, one, false, p, st);
+    if (p.type == QRAF_TYPE_F32) return launch_kv(kv_prefix_kernel<HDP, float>, p.pre_ctas, kPreThreads, two, false, p, st);
+    if (p.type == QRAF_TYPE_F16) return launch_kv(kv_prefix_kernel<HDP, __half>, p.pre_ctas, kPreThreads, one, false, p, st);
+    return launch_kv(kv_prefix_kernel<HDP, __nv_bfloat16>, p.pre_ctas, kPreThreads, one, false, p, st);
 }
 
 }  // namespace
@@ -342,6 +354,8 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     p.splits = pl.splits;
     p.own_wide = pl.own_wide;
     p.pre_ctas = pl.pre_ctas;
+    p.pre_base = pl.pre_base;
+    p.pre_extra = pl.pre_extra;
     p.chained = pl.pre_ctas ? 1u : 0u;
     p.part = pl.part_bytes ? static_cast<float*>(workspace_dev) : nullptr;
     const uint32_t hd = kv->head_dim;

@@ -40,13 +40,15 @@ constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own
 constexpr uint32_t kPreRows = 128;          // kv_prefix.cuh: query rows of a tile = MMA M
 constexpr uint32_t kPreKeys = 128;          // and keys of a tile
 
-// The range of (unit, key tile) pairs of CTA c of C, unit-major.
-__host__ __device__ __forceinline__ uint64_t pre_start(uint64_t work, uint32_t c, uint32_t C) {
-    return work * c / C;
+// kv_prefix_kernel's (unit, key tile) pairs, unit-major, are dealt out in contiguous
+// ranges of `base` pairs a CTA, one more for the first `extra`: the first pair of CTA c,
+__host__ __device__ __forceinline__ uint32_t pre_start(uint32_t base, uint32_t extra, uint32_t c) {
+    return c * base + (c < extra ? c : extra);
 }
-// The CTA that has pair x.
-__host__ __device__ __forceinline__ uint32_t pre_owner(uint64_t work, uint64_t x, uint32_t C) {
-    return static_cast<uint32_t>(((x + 1u) * C - 1u) / work);
+// and the CTA that has pair x.
+__host__ __device__ __forceinline__ uint32_t pre_owner(uint32_t base, uint32_t extra, uint32_t x) {
+    const uint32_t split = extra * (base + 1u);
+    return x < split ? x / (base + 1u) : extra + (x - split) / base;
 }
 
 struct KvAttnParams {
@@ -68,6 +70,7 @@ struct KvAttnParams {
     uint32_t row_tiles;      // prefix: tiles of 16 rows (pre_ctas: of 128) of a KV head
     uint32_t p_chunks, p_chunk;   // its chunks (pre_ctas: records of a row at most) and keys in one
     uint32_t pre_ctas;       // CTAs of kv_prefix_kernel, which has the prefix then; 0: kv_attention_kernel has it
+    uint32_t pre_base, pre_extra;   // its ranges
     uint32_t chained;        // kv_attention_kernel was launched as kv_prefix_kernel's dependent
     uint32_t own_tiles, splits;              // own rows: row tiles over all runs (at most), chunks of each (at most)
     uint32_t own_wide;       // own rows in tiles of 16 rows, else 8
@@ -655,9 +658,9 @@ __global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __
     }
     uint32_t pre = p.p_chunks;
     if (p.pre_ctas) {   // the CTAs whose ranges meet this row's unit
-        const uint64_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys, work = static_cast<uint64_t>(p.row_tiles) * p.kv.kv_heads * T;
-        const uint32_t h = head / p.group, unit = h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows;
-        pre = pre_owner(work, unit * T + T - 1u, p.pre_ctas) - pre_owner(work, unit * T, p.pre_ctas) + 1u;
+        const uint32_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys, h = head / p.group;
+        const uint32_t unit = h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows;
+        pre = pre_owner(p.pre_base, p.pre_extra, unit * T + T - 1u) - pre_owner(p.pre_base, p.pre_extra, unit * T) + 1u;
     }
     const uint32_t chunks = live ? pre + own : 0u;
     auto at = [&](uint32_t i) { return i < pre ? i : p.p_chunks + (i - pre); };   // record of chunk i

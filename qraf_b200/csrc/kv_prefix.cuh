@@ -27,6 +27,8 @@
 // 8 x 73 for O (N = 128, K = 16 each).
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv_attention.cuh"
 #include "matmul_tc.cuh"
@@ -37,6 +39,12 @@ constexpr uint32_t kPreThreads = 544;   // two softmax warpgroups, eight transfo
 constexpr uint32_t kPreWarpXf = 8, kPreWarpMma = 16, kPreXfThreads = 256;
 constexpr float kPreLag = 4.0f;         // log2 of how far a row may exceed the maximum it refers to
 constexpr int32_t kPreUp = 11;          // weights of p = 1 are below 2^11
+
+// Parts of the queries (16-bit ones are exact in one) and of the weights.
+template <typename Q>
+constexpr uint32_t pre_q_parts() { return sizeof(Q) == 4u ? 2u : 1u; }
+template <typename Q>
+constexpr uint32_t pre_p_parts() { return std::is_same<Q, __nv_bfloat16>::value ? 1u : 2u; }
 
 template <uint32_t HDP, uint32_t QP>
 struct PreShape {
@@ -99,14 +107,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
 
 // One tile's softmax for one row (thread): S at TMEM column s_col becomes P in
 // place, the row's maximum and sum move on, O at o_col is scaled where the maximum
-// moved.  ks, vs: the scales of the tile's keys; MASK: keys from `valid` on are not
+// moved.  The loops stay rolled: five kinds of code share the instruction caches here,
+// and unrolled (1500 instructions a tile) fetching them took a quarter of the issue
+// slots' waits.  ks, vs: the scales of the tile's keys; MASK: keys from `valid` on are not
 // there; `first`: the warpgroup's first tile of the stretch (O is written anew).
 template <uint32_t HDP, uint32_t PP, bool MASK>
 __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, const float* ks, const float* vs, uint32_t valid,
                                             float rf, bool first, float& m, float& l) {
     float v[32];
     float ymax = -INFINITY;
-#pragma unroll
+#pragma unroll 1
     for (uint32_t c = 0; c < 4u; ++c) {
         tmem_ld32(s_col + 32u * c, v);
         tmem_wait_ld();
@@ -139,13 +149,17 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
             tmem_ld32(o_col + c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (uint32_t j = 0; j < 32u; ++j) v[j] = __fmul_rn(v[j], alpha);
+            for (uint32_t j = 0; j < 32u; j += 2u) {
+                const float2 y = f2_mul(make_float2(v[j], v[j + 1u]), make_float2(alpha, alpha));
+                v[j] = y.x;
+                v[j + 1u] = y.y;
+            }
             tmem_st32(o_col + c, v);
         }
     }
     const float2 rf2 = make_float2(rf, rf), m2 = make_float2(-m, -m), neg = make_float2(-1.0f, -1.0f);
     float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
+#pragma unroll 1
     for (uint32_t c = 0; c < 4u; ++c) {
         tmem_ld32(s_col + 32u * c, v);
         tmem_wait_ld();
@@ -182,8 +196,10 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
     tmem_wait_st();
 }
 
-template <uint32_t HDP, uint32_t QP, uint32_t PP>
+// Q: the type of q and out.
+template <uint32_t HDP, typename Q>
 __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_constant__ KvAttnParams p) {
+    constexpr uint32_t QP = pre_q_parts<Q>(), PP = pre_p_parts<Q>();
     using S = PreShape<HDP, QP>;
     extern __shared__ uint8_t pre_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pre_smem_raw) + 1023u) & ~uintptr_t(1023));
@@ -202,8 +218,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     pdl_launch_dependents();
     if (tid == 0) {
         for (uint32_t i = 0; i < 2u; ++i) {
-            mbar_init(&k_ready[i], kPreXfThreads / 32u);
-            mbar_init(&v_ready[i], kPreXfThreads / 32u);
+            mbar_init(&k_ready[i], 4);
+            mbar_init(&v_ready[i], 4);
             mbar_init(&s_ready[i], 1);
             mbar_init(&p_ready[i], 4);
             mbar_init(&pv_done[i], 1);
@@ -224,54 +240,53 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     const uint32_t tmem = s_tmem;   // columns: S of slots 0 and 1 [0, 256), O of slots 0 and 1 [256, 512)
 
     const uint32_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys;
-    const uint64_t work = static_cast<uint64_t>(p.row_tiles) * H * T;
-    const uint64_t w1 = pre_start(work, blockIdx.x + 1u, gridDim.x);
+    const uint32_t w1 = pre_start(p.pre_base, p.pre_extra, blockIdx.x + 1u);
     uint32_t used[2] = {0u, 0u};   // tiles that each slot has had, over the CTA's stretches
     uint32_t q_phase = 0u;
     bool ok = true;
-    for (uint64_t w = pre_start(work, blockIdx.x, gridDim.x); w < w1;) {
-        const uint32_t unit = static_cast<uint32_t>(w / T), tile0 = static_cast<uint32_t>(w - static_cast<uint64_t>(unit) * T);
-        const uint32_t n = static_cast<uint32_t>(min(static_cast<uint64_t>(T - tile0), w1 - w));
+    for (uint32_t w = pre_start(p.pre_base, p.pre_extra, blockIdx.x); w < w1;) {
+        const uint32_t unit = w / T, tile0 = w - unit * T, n = min(T - tile0, w1 - w);
         const uint32_t h = unit / p.row_tiles, row0 = (unit - h * p.row_tiles) * kPreRows;
         const uint32_t key0 = tile0 * kPreKeys, key1 = min(p.prefix_len, (tile0 + n) * kPreKeys);
         float m = -INFINITY, l = 0.0f;
         const uint32_t slot = warp >> 2;   // of a softmax warp
 
         if (warp < kPreWarpXf) {
-            // ── the query rows: 16 a warp, eight loads in flight ──
-            constexpr uint32_t LPR = HDP / 4u, RPW = 32u / LPR, RB = 8u / RPW;   // lanes per row, rows per access, accesses per batch
-            const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-            const uint32_t ql = lane % LPR;
-#pragma unroll 1
-            for (uint32_t half = 0; half < 2u; ++half) {
-                float4 x[RB];
+            // ── the query rows: two lanes a row, all of a lane's loads in flight ──
+            {
+                constexpr uint32_t C = HDP / 16u;   // 16-byte columns of fp16 (8 elements) a lane
+                const uint32_t r = warp * 16u + (lane & 15u), c0 = (lane >> 4) * C, row = row0 + r;
+                const uint32_t t = row / G;
+                const Q* src = static_cast<const Q*>(p.q) + static_cast<uint64_t>(t) * p.q_ld +
+                               static_cast<uint64_t>(h * G + (row - t * G)) * hd + 8u * c0;
+                float4 x[2u * C];
 #pragma unroll
-                for (uint32_t i = 0; i < RB; ++i) {
-                    const uint32_t row = row0 + warp * 16u + half * 8u + i * RPW + lane / LPR;
-                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (row < rows && 4u * ql < hd) {
-                        const uint32_t t = row / G;
-                        x[i] = load4_any(p.q, p.type,
-                                         static_cast<uint64_t>(t) * p.q_ld + static_cast<uint64_t>(h * G + (row - t * G)) * hd + 4u * ql,
-                                         p.q_wide);
-                    }
+                for (uint32_t c = 0; c < 2u * C; ++c)
+                    x[c] = row < rows && 8u * c0 + 4u * c < hd && p.q_wide ? load4(src + 4u * c, true) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!p.q_wide && row < rows) {
+#pragma unroll
+                    for (uint32_t c = 0; c < 2u * C; ++c)
+                        if (8u * c0 + 4u * c < hd) x[c] = load4(src + 4u * c, false);
                 }
+                float mx = 0.0f;
 #pragma unroll
-                for (uint32_t i = 0; i < RB; ++i) {
-                    const uint32_t r = warp * 16u + half * 8u + i * RPW + lane / LPR;
-                    float mx = absmax4(x[i], 0.0f);
+                for (uint32_t c = 0; c < 2u * C; ++c) mx = absmax4(x[c], mx);
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+                // the largest becomes 2^10 .. 2^11, as in kva_item
+                const int32_t e = max(exponent_bits(mx), 11);
+                const float up = __fmul_rn(pow2_bits(264 - e), p.scale_log2 < 0.0f ? -1.0f : 1.0f);
+                if (lane < 16u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
 #pragma unroll
-                    for (uint32_t o = LPR / 2u; o > 0u; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-                    // the largest becomes 2^10 .. 2^11, as in kva_item
-                    const int32_t e = max(exponent_bits(mx), 11);
-                    const float up = __fmul_rn(pow2_bits(264 - e), sign);
-                    if (ql == 0u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
-                    uint32_t hi[2], lo[2];
-                    split_f16(__fmul_rn(x[i].x, up), __fmul_rn(x[i].y, up), hi[0], lo[0]);
-                    split_f16(__fmul_rn(x[i].z, up), __fmul_rn(x[i].w, up), hi[1], lo[1]);
-                    const uint32_t off = (ql >> 4) * (kPreRows * 128u) + tc_sw128_off(r, (ql & 15u) >> 1) + 8u * (ql & 1u);
-                    *reinterpret_cast<uint2*>(smem + S::kQ + off) = make_uint2(hi[0], hi[1]);
-                    if constexpr (QP == 2u) *reinterpret_cast<uint2*>(smem + S::kQ + S::kQPart + off) = make_uint2(lo[0], lo[1]);
+                for (uint32_t c = 0; c < C; ++c) {
+                    uint32_t hi[4], lo[4];
+                    split_f16(__fmul_rn(x[2u * c].x, up), __fmul_rn(x[2u * c].y, up), hi[0], lo[0]);
+                    split_f16(__fmul_rn(x[2u * c].z, up), __fmul_rn(x[2u * c].w, up), hi[1], lo[1]);
+                    split_f16(__fmul_rn(x[2u * c + 1u].x, up), __fmul_rn(x[2u * c + 1u].y, up), hi[2], lo[2]);
+                    split_f16(__fmul_rn(x[2u * c + 1u].z, up), __fmul_rn(x[2u * c + 1u].w, up), hi[3], lo[3]);
+                    const uint32_t off = ((c0 + c) >> 3) * (kPreRows * 128u) + tc_sw128_off(r, (c0 + c) & 7u);
+                    *reinterpret_cast<uint4*>(smem + S::kQ + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (QP == 2u)
+                        *reinterpret_cast<uint4*>(smem + S::kQ + S::kQPart + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -299,14 +314,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             // ── codes -> fp16 tiles ──
             // The MMAs run ... PV(t) S(t+2) PV(t+1) S(t+3) ...: V(t) is made while S(t+1)
             // runs and K(t+2) while PV(t) does, so one fp16 tile of each is enough; two
-            // tiles of codes of each are in flight behind them (cp.async).
-            const uint32_t xw = warp - kPreWarpXf, xt = tid - kPreWarpXf * 32u;
-            constexpr uint32_t U = HDP / 16u;                      // 16-byte units of a row
-            constexpr uint32_t KL = kPreKeys * U / kPreXfThreads;  // units of a tile a thread
-            constexpr uint32_t VB = HDP / 64u;                     // 32-dim blocks of V a warp
-            const int8_t* pk = p.pk + static_cast<uint64_t>(h) * hd;
-            const int8_t* pv = p.pv + static_cast<uint64_t>(h) * hd;
-            const float* my_scale = (xt < kPreKeys ? p.pks : p.pvs) + h;   // threads 0-127: K's, 128-255: V's
+            // tiles of codes of each are in flight behind them (cp.async).  Four warps make
+            // K, four V: one chain of waits, loads and stores each.
+            const uint32_t xw = warp & 3u, xt = tid & 127u;
+            const bool for_k = warp < kPreWarpXf + 4u;
+            constexpr uint32_t U = HDP / 16u;            // 16-byte units of a row
+            constexpr uint32_t KL = kPreKeys * U / 128u; // units of a tile a thread
+            constexpr uint32_t VB = HDP / 32u;           // 32-dim blocks of V
+            const int8_t* src_codes = (for_k ? p.pk : p.pv) + static_cast<uint64_t>(h) * hd;
             const uint32_t last = key1 - 1u;
             // K: lane (unit of 16 codes, key), so that eight consecutive lanes load from and
             // store to eight different 16-byte columns; a thread loads what it converts.
@@ -314,29 +329,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             constexpr uint32_t KI = 32u / U;   // keys per access
             const uint32_t k_kk = HDP == 128u ? ((lane >> 2) & 1u) + 2u * (lane >> 4) : lane >> 2;
             const uint32_t k_u = HDP == 128u ? (lane & 3u) + 4u * ((lane >> 3) & 1u) : lane & 3u;
-            const uint32_t k_key = xw * 16u + k_kk;
+            const uint32_t k_key = xw * 32u + k_kk;
             const uint32_t k_src = k_key * HDP + 16u * (HDP == 128u ? k_u ^ (4u * (k_kk & 1u)) : k_u);
-            // fp16 row of key 16 xw + i KI + k_kk: 8-row atom 2 xw + (i KI) / 8, row (i KI & 7) + k_kk
-            const uint32_t k_dst = (k_u >> 2) * (kPreKeys * 128u) + xw * 2048u + k_kk * 128u;
+            // fp16 row of key 32 xw + i KI + k_kk: 8-row atom 4 xw + (i KI) / 8, row (i KI & 7) + k_kk
+            const uint32_t k_dst = (k_u >> 2) * (kPreKeys * 128u) + xw * 4096u + k_kk * 128u;
             const uint32_t k_col = (2u * (k_u & 3u)) ^ k_kk;   // its 16-byte column, ^ (i KI & 7), ^ 1 for the second eight codes
             const bool k_in = 16u * k_u < hd;
             // V: unit u of key k lies at unit u ^ 2 (k / 8) so that a lane's four-byte reads of
             // four octets of keys meet four groups of banks
-            const uint32_t vf_u = xt % U, vf_key = xt / U;   // fetch: unit, first key; keys kPreXfThreads / U apart
+            const uint32_t vf_u = xt % U, vf_key = xt / U;   // fetch: unit, first key; keys 128 / U apart
             const bool vf_in = 16u * vf_u < hd;
             // conversion: lane (4 dims dq, octet of keys ko) of 32 keys x 32 dims
-            const uint32_t dq = (lane & 1u) + 2u * (lane >> 3), ko = (lane >> 1) & 3u, kb = xw & 3u, vb0 = xw >> 2;
-            const uint32_t v_src = (32u * kb + 8u * ko) * HDP + 4u * dq;   // + i HDP + 32 (block ^ ko)
+            const uint32_t dq = (lane & 1u) + 2u * (lane >> 3), ko = (lane >> 1) & 3u;
+            const uint32_t v_src = (32u * xw + 8u * ko) * HDP + 4u * dq;   // + i HDP + 32 (block ^ ko)
             // transposed row 32 block + 4 dq + j, 64 keys per 128-byte row: 16-byte column = octet of keys
-            const uint32_t v_dst = (kb >> 1) * (HDP * 128u) + (dq >> 1) * 1024u + (dq & 1u) * 512u;
-            const uint32_t v_col = (4u * (kb & 1u) + ko) ^ (4u * (dq & 1u));   // ^ j
+            const uint32_t v_dst = (xw >> 1) * (HDP * 128u) + (dq >> 1) * 1024u + (dq & 1u) * 512u;
+            const uint32_t v_col = (4u * (xw & 1u) + ko) ^ (4u * (dq & 1u));   // ^ j
             auto fetch_k = [&](uint32_t t) {
                 if (t < n && k_in) {
                     uint8_t* dst = smem + S::kRawK + (t & 1u) * S::kRaw + k_src;
                     const uint32_t k0 = key0 + t * kPreKeys + k_key;
-#pragma unroll
+#pragma unroll 2
                     for (uint32_t i = 0; i < KL; ++i)
-                        cp_async16(dst + i * KI * HDP, pk + static_cast<uint64_t>(min(k0 + i * KI, last)) * stride + 16u * k_u);
+                        cp_async16(dst + i * KI * HDP, src_codes + static_cast<uint64_t>(min(k0 + i * KI, last)) * stride + 16u * k_u);
                 }
                 cp_async_commit();
             };
@@ -344,36 +359,31 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 if (t < n && vf_in) {
                     uint8_t* dst = smem + S::kRawV + (t & 1u) * S::kRaw;
                     const uint32_t k0 = key0 + t * kPreKeys;
-#pragma unroll
+#pragma unroll 2
                     for (uint32_t i = 0; i < KL; ++i) {
-                        const uint32_t key = vf_key + i * (kPreXfThreads / U);
+                        const uint32_t key = vf_key + i * (128u / U);
                         cp_async16(dst + key * HDP + 16u * (vf_u ^ (2u * ((key >> 3) & (U / 2u - 1u)))),
-                                   pv + static_cast<uint64_t>(min(k0 + key, last)) * stride + 16u * vf_u);
+                                   src_codes + static_cast<uint64_t>(min(k0 + key, last)) * stride + 16u * vf_u);
                     }
                 }
                 cp_async_commit();
             };
-            // a barrier of these warps that tells whether all of them are fine, so that they
+            // a barrier of V's warps that tells whether all of them are fine, so that they
             // give up together when a wait runs out
-            auto all_xf = [](bool fine) {
+            auto all_v = [](bool fine) {
                 uint32_t r;
                 asm volatile(
                     "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                    "bar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                    "bar.red.and.pred q, 3, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                     : "=r"(r)
                     : "r"(fine ? 1u : 0u)
                     : "memory");
                 return r != 0u;
             };
-            // groups in order K0 K1 V0 V1 K2 K3 V2 K4 V3 K5 ..., one each even past the last tile
-            fetch_k(0);
-            fetch_k(1);
-            fetch_v(0);
-            fetch_v(1);
             // the unit of the weights: every V scale of the stretch is below 2^(eb - 126)
-            // (an infinity or NaN has no say)
+            // (an infinity or NaN has no say); before the tiles' copies, which would hold its loads up
             uint32_t most = 0u;
-            for (uint32_t key = key0 + xt; key < key1; key += 4u * kPreXfThreads) {
+            for (uint32_t key = key0 + tid - kPreWarpXf * 32u; key < key1; key += 4u * kPreXfThreads) {
                 float v[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i)
@@ -384,26 +394,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     if (e < 255u) most = max(most, e);
                 }
             }
+            for (uint32_t t = 0; t < 2u; ++t) {   // a group a tile, even past the last
+                if (for_k) fetch_k(t);
+                else fetch_v(t);
+            }
             most = __reduce_max_sync(0xFFFFFFFFu, most);
-            if (lane == 0u) s_unit[xw] = most;
-            all_xf(true);
+            if (lane == 0u) s_unit[warp - kPreWarpXf] = most;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
-            const float up = xt < kPreKeys ? 1.0f : pow2_bits(kPreUp + 253 - max(static_cast<int32_t>(most), 14));
-            float scale = 0.0f;   // this thread's scale of the next K tile's key xt & 127
+            const float up = pow2_bits(kPreUp + 253 - max(static_cast<int32_t>(most), 14));
+            float ksc = 0.0f, vsc = 0.0f;   // the scales of key xt of the next K tile
             auto fetch_scale = [&](uint32_t t) {
-                const uint32_t key = key0 + t * kPreKeys + (xt & (kPreKeys - 1u));
-                scale = t < n && key < key1 ? __ldg(my_scale + static_cast<uint64_t>(key) * H) : 0.0f;
+                const uint32_t key = key0 + t * kPreKeys + xt;
+                const bool in = t < n && key < key1;
+                ksc = in ? __ldg(p.pks + h + static_cast<uint64_t>(key) * H) : 0.0f;
+                vsc = in ? __ldg(p.pvs + h + static_cast<uint64_t>(key) * H) : 0.0f;
             };
             auto make_k = [&](uint32_t t) {
                 const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
-                if (t == 2u) cp_async_wait<2>();   // behind K2 came K3 and V2 only
-                else cp_async_wait<3>();
+                cp_async_wait<1>();
                 const uint8_t* raw = smem + S::kRawK + sl * S::kRaw + k_src;
-                uint4 c[KL];
-#pragma unroll
-                for (uint32_t i = 0; i < KL; ++i)
-                    c[i] = k_in ? *reinterpret_cast<const uint4*>(raw + i * KI * HDP) : make_uint4(0u, 0u, 0u, 0u);
                 if (t > 0u) {   // the K tile is free once the previous tile's S is there
                     const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
                     if (!warp_wait(&s_ready[ps], pj & 1u)) return false;
@@ -411,18 +422,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 // and the slot's scales once its previous P is written
                 if (j > 0u && !warp_wait(&p_ready[sl], (j - 1u) & 1u)) return false;
                 uint8_t* dst = smem + S::kK + k_dst;
-#pragma unroll
+#pragma unroll 2
                 for (uint32_t i = 0; i < KL; ++i) {
+                    const uint4 c = k_in ? *reinterpret_cast<const uint4*>(raw + i * KI * HDP) : make_uint4(0u, 0u, 0u, 0u);
                     uint8_t* row = dst + (i * KI >> 3) * 1024u + (i * KI & 7u) * 128u;
                     const uint32_t col = k_col ^ (i * KI & 7u);
-                    const uint32_t a0 = c[i].x ^ 0x80808080u, a1 = c[i].y ^ 0x80808080u, a2 = c[i].z ^ 0x80808080u,
-                                   a3 = c[i].w ^ 0x80808080u;
+                    const uint32_t a0 = c.x ^ 0x80808080u, a1 = c.y ^ 0x80808080u, a2 = c.z ^ 0x80808080u, a3 = c.w ^ 0x80808080u;
                     *reinterpret_cast<uint4*>(row + (col << 4)) =
                         make_uint4(codes_f16<0x4140u>(a0), codes_f16<0x4342u>(a0), codes_f16<0x4140u>(a1), codes_f16<0x4342u>(a1));
                     *reinterpret_cast<uint4*>(row + ((col ^ 1u) << 4)) =
                         make_uint4(codes_f16<0x4140u>(a2), codes_f16<0x4342u>(a2), codes_f16<0x4140u>(a3), codes_f16<0x4342u>(a3));
                 }
-                s_scales[sl * 256u + xt] = __fmul_rn(scale, up);
+                s_scales[sl * 256u + xt] = ksc;
+                s_scales[sl * 256u + 128u + xt] = __fmul_rn(vsc, up);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&k_ready[sl]);
@@ -432,31 +444,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             };
             auto make_v = [&](uint32_t t, bool fine) {
                 const uint32_t sl = t & 1u;
-                cp_async_wait<3>();
-                if (!all_xf(fine)) return false;   // the other threads' pieces have come too
+                cp_async_wait<1>();
+                if (!all_v(fine)) return false;   // the other threads' pieces have come too
                 const uint8_t* raw = smem + S::kRawV + sl * S::kRaw + v_src;
-                uint32_t x[VB][8];
-#pragma unroll
-                for (uint32_t b = 0; b < VB; ++b) {
-                    const uint32_t block = vb0 + 2u * b;
-                    const bool in = 32u * block + 4u * dq < hd;
-                    const uint8_t* src = raw + 32u * (block ^ (ko & (U / 2u - 1u)));
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) x[b][i] = in ? *reinterpret_cast<const uint32_t*>(src + i * HDP) ^ 0x80808080u : 0x80808080u;
-                }
                 if (t > 0u) {   // the V tile is free once the previous tile's O is done
                     const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
                     fine = warp_wait(&pv_done[ps], pj & 1u);
                 }
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t b = 0; b < VB; ++b) {
                     if (!fine) break;
-                    uint8_t* dst = smem + S::kV + v_dst + (vb0 + 2u * b) * 4096u;
+                    const bool in = 32u * b + 4u * dq < hd;
+                    const uint8_t* src = raw + 32u * (b ^ (ko & (U / 2u - 1u)));
+                    uint32_t x[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) x[i] = in ? *reinterpret_cast<const uint32_t*>(src + i * HDP) ^ 0x80808080u : 0x80808080u;
+                    uint8_t* dst = smem + S::kV + v_dst + b * 4096u;
                     uint32_t c01[4], c23[4];   // keys 2 i and 2 i + 1, byte-interleaved: dims 0-1 and 2-3
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) {
-                        c01[i] = __byte_perm(x[b][2u * i], x[b][2u * i + 1u], 0x5140u);
-                        c23[i] = __byte_perm(x[b][2u * i], x[b][2u * i + 1u], 0x7362u);
+                        c01[i] = __byte_perm(x[2u * i], x[2u * i + 1u], 0x5140u);
+                        c23[i] = __byte_perm(x[2u * i], x[2u * i + 1u], 0x7362u);
                     }
                     *reinterpret_cast<uint4*>(dst + (v_col << 4)) =
                         make_uint4(codes_f16<0x4140u>(c01[0]), codes_f16<0x4140u>(c01[1]), codes_f16<0x4140u>(c01[2]), codes_f16<0x4140u>(c01[3]));
@@ -470,19 +478,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0u && fine) mbar_arrive(&v_ready[sl]);
-                if (!all_xf(fine)) return false;   // every piece of the stage has been read
+                if (!all_v(fine)) return false;   // every piece of the stage has been read
                 fetch_v(t + 2u);
                 return true;
             };
-            fetch_scale(0);
-            ok = make_k(0);
-            if (ok && n > 1u) ok = make_k(1);
-            else cp_async_commit();
-            for (uint32_t t = 0; t < n; ++t) {
-                ok = make_v(t, ok);
-                if (!ok) break;   // all of these warps
-                if (t + 2u < n) ok = make_k(t + 2u);
-                else cp_async_commit();
+            if (for_k) {
+                fetch_scale(0);
+                for (uint32_t t = 0; ok && t < n; ++t) ok = make_k(t);
+            } else {
+                for (uint32_t t = 0; ok && t < n; ++t) ok = make_v(t, ok);
             }
             cp_async_wait<0>();
         } else {
@@ -495,9 +499,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 if (!warp_wait(&k_ready[sl], j & 1u)) return false;
                 tc_fence_after();
                 if (tc_elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t part = 0; part < QP; ++part)
-#pragma unroll
+#pragma unroll 4
                         for (uint32_t k = 0; k < HDP / 16u; ++k)
                             tc_mma_f16(tmem + sl * 128u,
                                        tc_smem_desc(base + S::kQ + part * S::kQPart + (k >> 2) * (kPreRows * 128u) + (k & 3u) * 32u),
@@ -516,9 +520,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 if (!ok) break;
                 tc_fence_after();
                 if (tc_elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t part = 0; part < PP; ++part)
-#pragma unroll
+#pragma unroll 4
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
                             pre_mma_ts(tmem + 256u + sl * 128u, tmem + sl * 128u + 32u * (k >> 1) + 16u * part + 8u * (k & 1u),
                                        tc_smem_desc(base + S::kV + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             tc_fence_before();
         }
         __syncthreads();
-        const uint32_t chunk = blockIdx.x - pre_owner(work, static_cast<uint64_t>(unit) * T, gridDim.x);
+        const uint32_t chunk = blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T);
 #pragma unroll 4
         for (uint32_t r = warp; r < kPreRows; r += kPreThreads / 32u) {
             const uint32_t row = row0 + r;
