@@ -126,21 +126,25 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
     const uint64_t G = heads / kv_heads, rows = static_cast<uint64_t>(n) * G;
     if (rows > 0x7FFFFFFFull / 16u || static_cast<uint64_t>(n) * heads > 0x7FFFFFFFull)
         return fail(QRAF_ERR_UNSUPPORTED, "%u new rows of %u heads are too many for one call", n, heads);
-    pl->own_wide = ragged ? rows > 8ull * std::min(count, n) : G > 8u;
+    const bool tiles = prefix_len && prefix_on_tiles(rows, kv_heads, hd, prefix_len);
+    // rows by 16: wherever the prefix is among the kernel's items (it is read once for every
+    // tile of rows), or where a sequence's own rows do not fit 8
+    pl->own_wide = (prefix_len && !tiles) || (ragged ? rows > 8ull * std::min(count, n) : G > 8u);
     const uint32_t R = pl->own_wide ? 16u : 8u;
     const uint64_t own_tiles = ragged ? (rows + static_cast<uint64_t>(std::min(count, n)) * (R - 1u)) / R
                                       : static_cast<uint64_t>(count) * ((G + R - 1u) / R);
-    const uint64_t slots = 2ull * static_cast<uint64_t>(sm_count);   // CTAs that run at once
+    const uint64_t slots = (pl->own_wide ? 2ull : 3ull) * static_cast<uint64_t>(sm_count);   // CTAs that run at once
     uint64_t items = 0;
     if (max_len) {
-        const uint64_t groups = own_tiles * kv_heads;
+        // about two rounds of CTAs, counting the tiles that runs of equal lengths would have
+        const uint64_t groups = std::max<uint64_t>({1, rows / R, std::min(count, n)}) * kv_heads;
         const uint64_t by_len = (max_len + kKvaMinChunk - 1ull) / kKvaMinChunk;
         pl->splits = static_cast<uint32_t>(
-            std::max<uint64_t>(1, std::min<uint64_t>({(slots + groups - 1) / groups, by_len, kKvaMaxChunks / 2u})));
-        items += groups * pl->splits;
+            std::max<uint64_t>(1, std::min<uint64_t>({(2 * slots + groups - 1) / groups, by_len, kKvaMaxChunks / 2u})));
+        items += own_tiles * kv_heads * pl->splits;
     }
     pl->own_tiles = static_cast<uint32_t>(own_tiles);
-    if (prefix_len && prefix_on_tiles(rows, kv_heads, hd, prefix_len)) {
+    if (tiles) {
         pl->row_tiles = static_cast<uint32_t>((rows + kPreRows - 1u) / kPreRows);
         const uint32_t T = (prefix_len + kPreKeys - 1u) / kPreKeys, work = pl->row_tiles * kv_heads * T;
         // One CTA an SM, each with two tiles at least (its two warpgroups).  Beginning and
@@ -197,9 +201,9 @@ cudaError_t launch_kv(K kernel, uint64_t grid, uint32_t threads, uint32_t smem, 
 
 template <uint32_t HDP>
 cudaError_t launch_kva(const KvAttnParams& p, uint64_t items, cudaStream_t st) {
-    const bool wide = (p.p_chunks && !p.pre_ctas) || p.own_wide;
-    return launch_kv(kv_attention_kernel<HDP>, items, kKvaThreads,
-                     wide ? KvaShape<HDP, true>::kSmem : KvaShape<HDP, false>::kSmem, p.chained != 0u, p, st);
+    return p.own_wide
+               ? launch_kv(kv_attention_kernel<HDP, true>, items, kKvaThreads, KvaShape<HDP, true>::kSmem, p.chained != 0u, p, st)
+               : launch_kv(kv_attention_kernel<HDP, false>, items, kKvaThreads, KvaShape<HDP, false>::kSmem, p.chained != 0u, p, st);
 }
 
 template <uint32_t HDP>
@@ -365,7 +369,7 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
                                 : hd <= 128u ? launch_kva<128>(p, pl.items, st) : launch_kva<256>(p, pl.items, st));
     if (!p.part) return QRAF_OK;
     const uint64_t out_rows = static_cast<uint64_t>(n) * heads;
-    const bool few = pl.p_chunks + pl.splits <= 4u;
+    const bool few = pl.p_chunks + pl.splits <= kJoinFew;
     QRAF_CUDA_TRY(few ? launch_kv(kv_attention_join_kernel<1>, (out_rows + kKvaWarps - 1) / kKvaWarps, kKvaThreads, 0, true, p, st)
                       : launch_kv(kv_attention_join_kernel<4>, out_rows, kKvaThreads, 0, true, p, st));
     return QRAF_OK;

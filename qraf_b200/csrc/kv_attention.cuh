@@ -33,6 +33,7 @@ namespace qraf_dev {
 
 constexpr uint32_t kKvaThreads = 128;
 constexpr uint32_t kKvaWarps = kKvaThreads / 32u;
+constexpr uint32_t kKvaStages = 2;          // steps of codes that a warp has in shared memory
 constexpr uint32_t kKvaMinChunk = 128;      // keys per chunk, at least: one step of each warp
 constexpr uint32_t kKvaMaxHeadDim = 256;
 constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own rows together
@@ -73,7 +74,7 @@ struct KvAttnParams {
     uint32_t pre_base, pre_extra;   // its ranges
     uint32_t chained;        // kv_attention_kernel was launched as kv_prefix_kernel's dependent
     uint32_t own_tiles, splits;              // own rows: row tiles over all runs (at most), chunks of each (at most)
-    uint32_t own_wide;       // own rows in tiles of 16 rows, else 8
+    uint32_t own_wide;       // the kernel with tiles of 16 rows, else 8
     float* part;             // [n * heads][p_chunks + splits][hd + 4]: output, max (log2), sum; nullptr: one chunk a row
 };
 
@@ -180,8 +181,11 @@ struct KvaShape {
     static constexpr uint32_t kOut = HDP / 8u;                   // 8-column output tiles
     static constexpr uint32_t kRows = WIDE ? 16u : 8u;
     static constexpr uint32_t kQBytes = kSteps * 32u * 16u * (WIDE ? 2u : 1u);
+    static constexpr uint32_t kStage = 2u * kKeys * HDP;         // a step's codes of K and V
+    static constexpr uint32_t kRing = kKvaWarps * kKvaStages * kStage;
     static constexpr uint32_t kJoinBytes = kKvaWarps * kRows * (HDP + 4u) * 4u;
-    static constexpr uint32_t kSmem = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
+    static constexpr uint32_t kSmem = kQBytes + (kRing > kJoinBytes ? kRing : kJoinBytes);
+    static_assert(kSmem <= (HDP == 256u ? 113u : 75u) * 1024u, "two or three CTAs an SM");
 };
 
 // One work item.  WIDE: 16 rows, hi and lo parts as two products into one
@@ -190,60 +194,99 @@ struct KvaShape {
 //
 // Lane (g = lane / 4, c = lane % 4).  The codes' order in the products is free as
 // long as both operands agree, and is chosen so that every fragment comes from wide
-// loads without going through shared memory: of a K row a lane reads 16 bytes
-// (dims 64 j + 16 c ..), each of its four words one step's fragment; of V it reads
-// its columns (16 g ..) of the four keys that its score accumulators belong to, and
-// pairs their bytes.
+// reads: of a K row a lane reads 16 bytes (dims 64 j + 16 c ..), each of its four
+// words one step's fragment; of V it reads its columns (16 g ..) of the four keys
+// that its score accumulators belong to, and pairs their bytes.  Each warp copies
+// its own steps to shared memory (cp.async), one step ahead; the rows' 16-byte
+// units are exchanged so that both reads meet no bank twice.
 template <uint32_t HDP, bool WIDE>
 __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& it, uint8_t* smem, float* s_rf) {
     using S = KvaShape<HDP, WIDE>;
     constexpr uint32_t R = S::kRows, RT = WIDE ? 2u : 1u;   // RT: score rows of a thread
+    constexpr uint32_t U = HDP / 16u;                       // 16-byte units of a row
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, c = lane & 3u;
     const uint32_t hd = p.kv.hd, G = p.group;
     const uint32_t nrows = min(R, it.rows - it.row0);
 
-    // ── the query rows: powers of two, then the fragments in shared memory ──
-    auto q_at = [&](uint32_t r) {
-        const uint32_t row = it.row0 + r, i = row / G;
-        return static_cast<uint64_t>(it.t0 + static_cast<int32_t>(i)) * p.q_ld +
-               static_cast<uint64_t>(it.h * G + (row - i * G)) * hd;
-    };
-    for (uint32_t r = warp; r < R; r += kKvaWarps) {
-        float m = 0.0f;
-        if (r < nrows) {
-            const uint64_t at = q_at(r);
-            for (uint32_t d = lane; d < hd; d += 32u) m = fmaxf(m, fabsf(__fmul_rn(load_any(p.q, p.type, at + d), p.scale_log2)));
-        }
+    // ── the first steps' codes ──
+    uint8_t* ring = smem + S::kQBytes + warp * (kKvaStages * S::kStage);
+    const uint32_t last = it.key1 - 1u;
+    constexpr uint32_t KPA = 32u / U;   // keys per copy of the warp
+    const uint32_t cu = lane % U, ck = lane / U;
+    auto fetch = [&](uint32_t k0, uint32_t stage) {   // the step from key k0, a group even past the end
+        if (k0 < it.key1 && 16u * cu < hd) {
+            uint8_t* dst = ring + stage * S::kStage;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        // the largest becomes 2^10 .. 2^11: hi up to 2048, lo's last bit 2^-24
-        if (lane == 0) s_rf[r] = pow2_bits(max(exponent_bits(m), 11) - 10);
-    }
-    __syncthreads();
-    for (uint32_t j = tid; j < S::kSteps * 32u; j += kKvaThreads) {
-        const uint32_t l = j & 31u, st = j >> 5;
-        const uint32_t d = 64u * (st >> 2) + 16u * (l & 3u) + 4u * (st & 3u);
-        uint32_t hi[2][2] = {}, lo[2][2] = {};
-#pragma unroll
-        for (uint32_t e = 0; e < RT; ++e) {
-            const uint32_t r = (l >> 2) + 8u * e;
-            if (r < nrows && d < hd) {
-                const uint64_t at = q_at(r) + d;
-                const float up = pow2_bits(254 - exponent_bits(s_rf[r]));
-                float x[4];
-#pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k)
-                    x[k] = __fmul_rn(__fmul_rn(load_any(p.q, p.type, at + k), p.scale_log2), up);
-                split_f16(x[0], x[1], hi[e][0], lo[e][0]);
-                split_f16(x[2], x[3], hi[e][1], lo[e][1]);
+            for (uint32_t i = 0; i < S::kKeys / KPA; ++i) {
+                const uint32_t k = ck + i * KPA;
+                const uint64_t off = static_cast<uint64_t>(min(k0 + k, last)) * it.stride + 16u * cu;
+                cp_async16(dst + k * HDP + 16u * (cu ^ (4u * (k & 1u) & (U - 1u))), it.k + off);
+                cp_async16(dst + S::kKeys * HDP + k * HDP + 16u * (cu ^ (k & 6u & (U - 1u))), it.v + off);
             }
         }
-        uint4* dst = reinterpret_cast<uint4*>(smem);
-        if constexpr (WIDE) {
-            dst[j] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
-            dst[S::kSteps * 32u + j] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
-        } else {
-            dst[j] = make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1]);
+        cp_async_commit();
+    };
+    constexpr uint32_t step = S::kKeys * kKvaWarps;
+    uint32_t k0 = it.key0 + warp * S::kKeys;
+    fetch(k0, 0);
+    float sk = 0.0f, sv = 0.0f;   // K and V scale of key (lane) of the next step
+    auto fetch_scales = [&](uint32_t k) {
+        const uint32_t key = k + lane;
+        const bool in = lane < S::kKeys && key < it.key1;
+        sk = in ? __ldg(it.ks + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
+        sv = in ? __ldg(it.vs + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
+    };
+    fetch_scales(k0);
+
+    // ── the query rows: powers of two, then the fragments in shared memory ──
+    {
+        constexpr uint32_t TPR = kKvaThreads / R, QN = HDP / 4u / TPR;   // threads a row, quads (4 dims) a thread
+        const uint32_t r = tid / TPR, j0 = tid % TPR, row = it.row0 + r, i = row / G;
+        const uint64_t at = static_cast<uint64_t>(it.t0 + static_cast<int32_t>(i)) * p.q_ld +
+                            static_cast<uint64_t>(it.h * G + (row - i * G)) * hd;
+        float4 x[QN];
+        auto load = [&](const auto* q) {
+#pragma unroll
+            for (uint32_t j = 0; j < QN; ++j) {
+                const uint32_t d = 4u * (j0 + j * TPR);
+                x[j] = r < nrows && d < hd ? load4(q + at + d, p.q_wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        if (p.type == QRAF_TYPE_F32) load(static_cast<const float*>(p.q));
+        else if (p.type == QRAF_TYPE_F16) load(static_cast<const __half*>(p.q));
+        else load(static_cast<const __nv_bfloat16*>(p.q));
+        float m = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < QN; ++j) {
+            x[j] = make_float4(__fmul_rn(x[j].x, p.scale_log2), __fmul_rn(x[j].y, p.scale_log2), __fmul_rn(x[j].z, p.scale_log2),
+                               __fmul_rn(x[j].w, p.scale_log2));
+            m = absmax4(x[j], m);
+        }
+#pragma unroll
+        for (uint32_t o = TPR / 2u; o > 0u; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        // the largest becomes 2^10 .. 2^11: hi up to 2048, lo's last bit 2^-24
+        const int32_t e = max(exponent_bits(m), 11);
+        const float up = pow2_bits(264 - e);
+        if (j0 == 0u) s_rf[r] = pow2_bits(e - 10);
+        uint32_t* frag = reinterpret_cast<uint32_t*>(smem);
+#pragma unroll
+        for (uint32_t j = 0; j < QN; ++j) {
+            const uint32_t d = 4u * (j0 + j * TPR);
+            uint32_t hi[2], lo[2];
+            split_f16(__fmul_rn(x[j].x, up), __fmul_rn(x[j].y, up), hi[0], lo[0]);
+            split_f16(__fmul_rn(x[j].z, up), __fmul_rn(x[j].w, up), hi[1], lo[1]);
+            const uint32_t st = 4u * (d >> 6) + ((d >> 2) & 3u), l = 4u * (r & 7u) + ((d >> 4) & 3u);
+            uint32_t* f = frag + 4u * (st * 32u + l);
+            if constexpr (WIDE) {
+                f += r >> 3;
+                f[0] = hi[0];
+                f[2] = hi[1];
+                f += 4u * S::kSteps * 32u;
+                f[0] = lo[0];
+                f[2] = lo[1];
+            } else {
+                *reinterpret_cast<uint4*>(f) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+            }
         }
     }
     __syncthreads();
@@ -270,81 +313,50 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
 #pragma unroll
     for (uint32_t e = 0; e < RT; ++e) vref[e] = 14;
 
-    uint4 kr[S::kTiles][HDP / 64u];
-    float sk = 0.0f, sv = 0.0f;   // K and V scale of key (lane) of the step
-    const uint32_t last = it.key1 - 1u;
-    auto load_k = [&](uint32_t k0) {
-#pragma unroll
-        for (uint32_t t = 0; t < S::kTiles; ++t) {
-            const int8_t* row = it.k + static_cast<uint64_t>(min(k0 + 8u * t + g, last)) * it.stride;
-#pragma unroll
-            for (uint32_t j = 0; j < HDP / 64u; ++j)
-                kr[t][j] = 64u * j + 16u * c < hd ? __ldg(reinterpret_cast<const uint4*>(row + 64u * j + 16u * c))
-                                                  : make_uint4(0u, 0u, 0u, 0u);
-        }
-        const uint32_t key = k0 + lane;
-        const bool in = lane < S::kKeys && key < it.key1;
-        sk = in ? __ldg(it.ks + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
-        sv = in ? __ldg(it.vs + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
-    };
-    const uint32_t step = S::kKeys * kKvaWarps;
-    uint32_t k0 = it.key0 + warp * S::kKeys;
-    if (k0 < it.key1) load_k(k0);
-    for (; k0 < it.key1; k0 += step) {
-        // V of this step: in flight through the score product and the softmax
-        uint32_t vw[S::kKeys / 16u][4][S::kWords];
-#pragma unroll
-        for (uint32_t u = 0; u < S::kKeys / 16u; ++u) {
-#pragma unroll
-            for (uint32_t r = 0; r < 4u; ++r) {
-                const uint32_t key = min(k0 + 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1), last);
-                const int8_t* row = it.v + static_cast<uint64_t>(key) * it.stride;
-                if constexpr (HDP == 64u) {
-                    const uint2 w = 8u * g < hd ? __ldg(reinterpret_cast<const uint2*>(row + 8u * g)) : make_uint2(0u, 0u);
-                    vw[u][r][0] = w.x;
-                    vw[u][r][1] = w.y;
-                } else {
-#pragma unroll
-                    for (uint32_t h = 0; h < HDP / 128u; ++h) {
-                        const uint4 w = 128u * h + 16u * g < hd
-                                            ? __ldg(reinterpret_cast<const uint4*>(row + 128u * h + 16u * g))
-                                            : make_uint4(0u, 0u, 0u, 0u);
-                        vw[u][r][4u * h] = w.x;
-                        vw[u][r][4u * h + 1u] = w.y;
-                        vw[u][r][4u * h + 2u] = w.z;
-                        vw[u][r][4u * h + 3u] = w.w;
-                    }
-                }
-            }
-        }
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (; k0 < it.key1; k0 += step, stage ^= 1u) {
+        fetch(k0 + step, stage ^ 1u);   // that stage's step was read before the last __syncwarp
+        cp_async_wait<1>();
+        __syncwarp();   // the other lanes' copies
+        const uint8_t* kc = ring + stage * S::kStage;
+        const uint8_t* vc = kc + S::kKeys * HDP;
         // ── scores ──
         float s[S::kTiles][4];
 #pragma unroll
         for (uint32_t t = 0; t < S::kTiles; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-        for (uint32_t st = 0; st < S::kSteps; ++st) {
-            const uint4 qa = reinterpret_cast<const uint4*>(smem)[st * 32u + lane];
-            const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
-            uint32_t al[4];
-            if constexpr (WIDE) {
-                const uint4 ql = reinterpret_cast<const uint4*>(smem)[(S::kSteps + st) * 32u + lane];
-                al[0] = ql.x;
-                al[1] = ql.y;
-                al[2] = ql.z;
-                al[3] = ql.w;
-            }
+        for (uint32_t j = 0; j < HDP / 64u; ++j) {
+            uint4 kr[S::kTiles];
+            const bool in = 64u * j + 16u * c < hd;
 #pragma unroll
-            for (uint32_t t = 0; t < S::kTiles; ++t) {
-                const uint4 kk = kr[t][st >> 2];
-                const uint32_t w = ((st & 3u) == 0u ? kk.x : (st & 3u) == 1u ? kk.y : (st & 3u) == 2u ? kk.z : kk.w) ^ 0x80808080u;
-                const uint32_t b0 = codes_f16<0x4140u>(w), b1 = codes_f16<0x4342u>(w);
-                mma_f16(s[t], a, b0, b1);
-                if constexpr (WIDE) mma_f16(s[t], al, b0, b1);
+            for (uint32_t t = 0; t < S::kTiles; ++t)
+                kr[t] = in ? *reinterpret_cast<const uint4*>(kc + (8u * t + g) * HDP + 16u * ((4u * j + c) ^ (4u * (g & 1u) & (U - 1u))))
+                           : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint4 qa = reinterpret_cast<const uint4*>(smem)[(4u * j + i) * 32u + lane];
+                const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
+                uint32_t al[4];
+                if constexpr (WIDE) {
+                    const uint4 ql = reinterpret_cast<const uint4*>(smem)[(S::kSteps + 4u * j + i) * 32u + lane];
+                    al[0] = ql.x;
+                    al[1] = ql.y;
+                    al[2] = ql.z;
+                    al[3] = ql.w;
+                }
+#pragma unroll
+                for (uint32_t t = 0; t < S::kTiles; ++t) {
+                    const uint32_t w = (i == 0u ? kr[t].x : i == 1u ? kr[t].y : i == 2u ? kr[t].z : kr[t].w) ^ 0x80808080u;
+                    const uint32_t b0 = codes_f16<0x4140u>(w), b1 = codes_f16<0x4342u>(w);
+                    mma_f16(s[t], a, b0, b1);
+                    if constexpr (WIDE) mma_f16(s[t], al, b0, b1);
+                }
             }
         }
         const float sk_now = sk, sv_now = sv;
         const uint32_t k_now = k0;
-        if (k0 + step < it.key1) load_k(k0 + step);   // in flight through the rest of this step
+        fetch_scales(k0 + step);
 
         // ── softmax ──
         float x[RT][2u * S::kTiles], vsc[2u * S::kTiles];
@@ -418,6 +430,29 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         // ── weighted sum of V ──
 #pragma unroll
         for (uint32_t u = 0; u < S::kKeys / 16u; ++u) {
+            uint32_t vw[4][S::kWords];   // this lane's columns of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+#pragma unroll
+            for (uint32_t r = 0; r < 4u; ++r) {
+                const uint32_t k = 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1);
+                const uint8_t* row = vc + k * HDP;
+                if constexpr (HDP == 64u) {
+                    const uint2 w = 8u * g < hd ? *reinterpret_cast<const uint2*>(row + 16u * ((g >> 1) ^ (k & 6u & (U - 1u))) + 8u * (g & 1u))
+                                                : make_uint2(0u, 0u);
+                    vw[r][0] = w.x;
+                    vw[r][1] = w.y;
+                } else {
+#pragma unroll
+                    for (uint32_t h = 0; h < HDP / 128u; ++h) {
+                        const uint4 w = 128u * h + 16u * g < hd
+                                            ? *reinterpret_cast<const uint4*>(row + 16u * ((8u * h + g) ^ (k & 6u)))
+                                            : make_uint4(0u, 0u, 0u, 0u);
+                        vw[r][4u * h] = w.x;
+                        vw[r][4u * h + 1u] = w.y;
+                        vw[r][4u * h + 2u] = w.z;
+                        vw[r][4u * h + 3u] = w.w;
+                    }
+                }
+            }
             uint32_t a[4], al[4];
             if constexpr (WIDE) {
                 a[0] = ph[0][2u * u];
@@ -436,8 +471,8 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
             }
 #pragma unroll
             for (uint32_t w = 0; w < S::kWords; ++w) {
-                const uint32_t v0 = vw[u][0][w] ^ 0x80808080u, v1 = vw[u][1][w] ^ 0x80808080u;
-                const uint32_t v2 = vw[u][2][w] ^ 0x80808080u, v3 = vw[u][3][w] ^ 0x80808080u;
+                const uint32_t v0 = vw[0][w] ^ 0x80808080u, v1 = vw[1][w] ^ 0x80808080u;
+                const uint32_t v2 = vw[2][w] ^ 0x80808080u, v3 = vw[3][w] ^ 0x80808080u;
                 const uint32_t a01 = __byte_perm(v0, v1, 0x5140u), a23 = __byte_perm(v0, v1, 0x7362u);
                 const uint32_t b01 = __byte_perm(v2, v3, 0x5140u), b23 = __byte_perm(v2, v3, 0x7362u);
                 const uint32_t b[4][2] = {{codes_f16<0x4140u>(a01), codes_f16<0x4140u>(b01)},
@@ -451,7 +486,9 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                 }
             }
         }
+        __syncwarp();   // the stage has been read
     }
+    cp_async_wait<0>();
 
     // ── join the warps ──
 #pragma unroll
@@ -459,8 +496,8 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         run_l[e] = __fadd_rn(run_l[e], __shfl_xor_sync(0xFFFFFFFFu, run_l[e], 1));
         run_l[e] = __fadd_rn(run_l[e], __shfl_xor_sync(0xFFFFFFFFu, run_l[e], 2));
     }
-    __syncthreads();   // the query fragments have been read
-    float* jo = reinterpret_cast<float*>(smem);   // [warp][row][HDP + 4]: output, max, sum
+    __syncthreads();   // every ring has been read
+    float* jo = reinterpret_cast<float*>(smem + S::kQBytes);   // [warp][row][HDP + 4]: output, max, sum
     constexpr uint32_t LD = HDP + 4u;
 #pragma unroll
     for (uint32_t e = 0; e < RT; ++e) {
@@ -571,15 +608,16 @@ __device__ __forceinline__ bool find_tile(const KvAttnParams& p, uint32_t idx, u
     return false;
 }
 
-template <uint32_t HDP>
+// WIDE: prefix items and own rows in tiles of 16 rows, else own rows in tiles of 8.
+template <uint32_t HDP, bool WIDE>
 __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem, float* s_rf) {
     const uint32_t H = p.kv.kv_heads;
     KvaItem it;
     it.sstride = H;
     it.stride = static_cast<uint64_t>(H) * p.kv.hd;
     uint32_t idx = blockIdx.x;
-    const uint32_t p_items = p.pre_ctas ? 0u : p.row_tiles * H * p.p_chunks;
-    if (idx < p_items) {
+    const uint32_t p_items = !WIDE || p.pre_ctas ? 0u : p.row_tiles * H * p.p_chunks;
+    if (WIDE && idx < p_items) {
         const uint32_t q = idx / p.row_tiles, rt = idx - q * p.row_tiles;
         it.chunk = q / H;
         it.h = q - it.chunk * H;
@@ -593,11 +631,11 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
         it.rows = p.runs.n * p.group;
         it.t0 = 0;
         it.seen0 = INT32_MAX;
-        kva_item<HDP, true>(p, it, kva_smem, s_rf);
+        kva_item<HDP, WIDE>(p, it, kva_smem, s_rf);
         return;
     }
     idx -= p_items;
-    const uint32_t R = p.own_wide ? 16u : 8u;
+    constexpr uint32_t R = WIDE ? 16u : 8u;
     const uint32_t q = idx / p.splits, s = idx - q * p.splits;
     const uint32_t tile_idx = q / H;
     it.h = q - tile_idx * H;
@@ -621,34 +659,36 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
     it.t0 = t0;
     it.seen0 = static_cast<int32_t>(len) - static_cast<int32_t>(n) + 1;
     it.chunk = p.p_chunks + s;
-    if (p.own_wide) kva_item<HDP, true>(p, it, kva_smem, s_rf);
-    else kva_item<HDP, false>(p, it, kva_smem, s_rf);
+    kva_item<HDP, WIDE>(p, it, kva_smem, s_rf);
 }
 
-template <uint32_t HDP>
-__global__ void __launch_bounds__(kKvaThreads, 2) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
+template <uint32_t HDP, bool WIDE>
+__global__ void __launch_bounds__(kKvaThreads, WIDE || HDP == 256u ? 2 : 3) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
     extern __shared__ __align__(16) uint8_t kva_smem[];
     __shared__ float s_rf[16];
     pdl_launch_dependents();
-    kva_cta<HDP>(p, kva_smem, s_rf);
+    kva_cta<HDP, WIDE>(p, kva_smem, s_rf);
     // not to end before the prefix's kernel has: the joining kernel waits for this one alone
     if (p.chained && blockIdx.x == 0u) pdl_wait();
 }
 
 // out = sum_c w_c o_c / sum_c w_c l_c with w_c = 2^(m_c - max m) over a row's chunks,
-// in chunk order.  WPR warps a row: one where a row has few chunks (then a CTA
-// joins four rows), else four, each with every fourth chunk.
+// in chunk order.  WPR warps a row: one where a row has up to 16 chunks (then a CTA
+// joins four rows), else four, each with every fourth chunk.  The runs are looked up
+// before the dependency wait: nothing that they say is written by the kernels before.
+constexpr uint32_t kJoinFew = 16;
+
 template <uint32_t WPR>
 __global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __grid_constant__ KvAttnParams p) {
-    __shared__ float s_w[kKvaWarps / WPR][kKvaMaxChunks];
-    __shared__ float s_o[kKvaWarps][kKvaMaxHeadDim];
+    constexpr uint32_t kMost = WPR == 1u ? kJoinFew : kKvaMaxChunks;
+    __shared__ float s_w[kKvaWarps / WPR][kMost];
+    __shared__ float s_o[WPR == 1u ? 1u : kKvaWarps][kKvaMaxHeadDim];
     __shared__ float s_l[kKvaWarps];
-    pdl_wait();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = p.kv.hd;
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kKvaWarps / WPR) + warp / WPR;
     const uint32_t sub = warp % WPR;
     bool live = row < static_cast<uint64_t>(p.runs.n) * p.heads;
-    const uint32_t t = live ? static_cast<uint32_t>(row / p.heads) : 0u, head = static_cast<uint32_t>(row - static_cast<uint64_t>(t) * p.heads);
+    const uint32_t t = live ? static_cast<uint32_t>(row) / p.heads : 0u, head = static_cast<uint32_t>(row) - t * p.heads;
     uint32_t own = 0;
     if (live) {
         const int32_t b = find_run(p.runs, static_cast<int32_t>(t));
@@ -667,6 +707,7 @@ __global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __
     const uint64_t ld = hd + 4u;
     const float* rec = p.part + row * (p.p_chunks + p.splits) * ld;
     float* w = s_w[warp / WPR];
+    pdl_wait();
     float m = -INFINITY;
     for (uint32_t i = lane; i < chunks; i += 32u) m = fmaxf(m, __ldcg(rec + at(i) * ld + hd));
 #pragma unroll
