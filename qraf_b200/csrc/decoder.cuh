@@ -108,11 +108,6 @@ __host__ __device__ constexpr size_t attn_smem_bytes8(uint32_t G, uint32_t hd) {
     return 4u * static_cast<size_t>(G) * hd + 2u * hd + 2u * attn_stage8_bytes(hd) + 4u * static_cast<size_t>(G) * kAttnTile;
 }
 
-__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
-    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(gmem) : "memory");
-}
-
 // Attention of one step, fused with RoPE and the KV-cache store
 // (attention_forward, src/nn/attention.cpp:104-150).  CTA (s, kvh, m) takes slot
 // m's KV head kvh and the G = heads / kv_heads query heads that share it (the

@@ -133,14 +133,15 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
     const uint32_t R = pl->own_wide ? 16u : 8u;
     const uint64_t own_tiles = ragged ? (rows + static_cast<uint64_t>(std::min(count, n)) * (R - 1u)) / R
                                       : static_cast<uint64_t>(count) * ((G + R - 1u) / R);
-    const uint64_t slots = (pl->own_wide ? 2ull : 3ull) * static_cast<uint64_t>(sm_count);   // CTAs that run at once
+    // warps (CTAs) that run at once: 8 or 11 an SM by registers and shared memory
+    const uint64_t slots = (pl->own_wide || hd > 128u ? 8ull : 11ull) * static_cast<uint64_t>(sm_count);
     uint64_t items = 0;
     if (max_len) {
-        // about two rounds of CTAs, counting the tiles that runs of equal lengths would have
+        // about one round of them, counting the tiles that runs of equal lengths would have
         const uint64_t groups = std::max<uint64_t>({1, rows / R, std::min(count, n)}) * kv_heads;
         const uint64_t by_len = (max_len + kKvaMinChunk - 1ull) / kKvaMinChunk;
         pl->splits = static_cast<uint32_t>(
-            std::max<uint64_t>(1, std::min<uint64_t>({(2 * slots + groups - 1) / groups, by_len, kKvaMaxChunks / 2u})));
+            std::max<uint64_t>(1, std::min<uint64_t>({(slots + groups - 1) / groups, by_len, kKvaMaxChunks / 2u})));
         items += own_tiles * kv_heads * pl->splits;
     }
     pl->own_tiles = static_cast<uint32_t>(own_tiles);
@@ -167,7 +168,7 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         const uint64_t units = static_cast<uint64_t>(pl->row_tiles) * kv_heads;
         const uint64_t by_len = (prefix_len + kKvaMinChunk - 1ull) / kKvaMinChunk;
         uint64_t chunks = std::max<uint64_t>(
-            1, std::min<uint64_t>({(4 * slots + units - 1) / units, by_len, kKvaMaxChunks / 2u}));
+            1, std::min<uint64_t>({(slots + units - 1) / units, by_len, kKvaMaxChunks / 2u}));
         pl->p_chunk = static_cast<uint32_t>(((prefix_len + chunks - 1) / chunks + 31u) & ~31ull);
         pl->p_chunks = (prefix_len + pl->p_chunk - 1u) / pl->p_chunk;
         items += units * pl->p_chunks;
@@ -202,8 +203,8 @@ cudaError_t launch_kv(K kernel, uint64_t grid, uint32_t threads, uint32_t smem, 
 template <uint32_t HDP>
 cudaError_t launch_kva(const KvAttnParams& p, uint64_t items, cudaStream_t st) {
     return p.own_wide
-               ? launch_kv(kv_attention_kernel<HDP, true>, items, kKvaThreads, KvaShape<HDP, true>::kSmem, p.chained != 0u, p, st)
-               : launch_kv(kv_attention_kernel<HDP, false>, items, kKvaThreads, KvaShape<HDP, false>::kSmem, p.chained != 0u, p, st);
+               ? launch_kv(kv_attention_kernel<HDP, true>, items, 32u, KvaShape<HDP, true>::kSmem, p.chained != 0u, p, st)
+               : launch_kv(kv_attention_kernel<HDP, false>, items, 32u, KvaShape<HDP, false>::kSmem, p.chained != 0u, p, st);
 }
 
 template <uint32_t HDP>
@@ -370,8 +371,8 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     if (!p.part) return QRAF_OK;
     const uint64_t out_rows = static_cast<uint64_t>(n) * heads;
     const bool few = pl.p_chunks + pl.splits <= kJoinFew;
-    QRAF_CUDA_TRY(few ? launch_kv(kv_attention_join_kernel<1>, (out_rows + kKvaWarps - 1) / kKvaWarps, kKvaThreads, 0, true, p, st)
-                      : launch_kv(kv_attention_join_kernel<4>, out_rows, kKvaThreads, 0, true, p, st));
+    QRAF_CUDA_TRY(few ? launch_kv(kv_attention_join_kernel<1>, (out_rows + kJoinWarps - 1) / kJoinWarps, kJoinThreads, 0, true, p, st)
+                      : launch_kv(kv_attention_join_kernel<4>, out_rows, kJoinThreads, 0, true, p, st));
     return QRAF_OK;
 }
 

@@ -17,11 +17,12 @@
 //
 // Work.  The rows of a work item (up to 16 of one KV head) meet one chunk of keys:
 // a chunk of the prefix, with rows of any sequences, so the prefix is read once
-// for every 16 rows; or a chunk of one sequence's own rows.  The four warps of a
-// CTA take steps of 32 keys in turn and keep maximum, sum and output of their
-// own; they are joined in shared memory, and the chunks of a row by a second
-// kernel (in a fixed order: results do not depend on timing).  A call with one
-// chunk a row writes its output at once.
+// for every 16 rows (kv_prefix.cuh has it instead where there are rows enough for
+// the 5th-generation tensor cores); or a chunk of one sequence's own rows.  One
+// warp has an item and is a CTA of its own: it takes steps of 32 keys, keeps
+// maximum, sum and output in registers and leaves them as the chunk's record; a
+// second kernel joins the chunks of a row, in their order, so results do not
+// depend on timing.  A call with one chunk a row writes its output at once.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -31,10 +32,9 @@
 
 namespace qraf_dev {
 
-constexpr uint32_t kKvaThreads = 128;
-constexpr uint32_t kKvaWarps = kKvaThreads / 32u;
 constexpr uint32_t kKvaStages = 2;          // steps of codes that a warp has in shared memory
-constexpr uint32_t kKvaMinChunk = 128;      // keys per chunk, at least: one step of each warp
+constexpr uint32_t kJoinThreads = 128, kJoinWarps = kJoinThreads / 32u;
+constexpr uint32_t kKvaMinChunk = 64;       // keys per chunk, at least: two steps
 constexpr uint32_t kKvaMaxHeadDim = 256;
 constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own rows together
 
@@ -181,14 +181,11 @@ struct KvaShape {
     static constexpr uint32_t kOut = HDP / 8u;                   // 8-column output tiles
     static constexpr uint32_t kRows = WIDE ? 16u : 8u;
     static constexpr uint32_t kQBytes = kSteps * 32u * 16u * (WIDE ? 2u : 1u);
-    static constexpr uint32_t kStage = 2u * kKeys * HDP;         // a step's codes of K and V
-    static constexpr uint32_t kRing = kKvaWarps * kKvaStages * kStage;
-    static constexpr uint32_t kJoinBytes = kKvaWarps * kRows * (HDP + 4u) * 4u;
-    static constexpr uint32_t kSmem = kQBytes + (kRing > kJoinBytes ? kRing : kJoinBytes);
-    static_assert(kSmem <= (HDP == 256u ? 113u : 75u) * 1024u, "two or three CTAs an SM");
+    static constexpr uint32_t kStage = 2u * kKeys * HDP + 2u * kKeys * 4u;   // a step's codes of K and V, their scales
+    static constexpr uint32_t kSmem = kQBytes + kKvaStages * kStage;
 };
 
-// One work item.  WIDE: 16 rows, hi and lo parts as two products into one
+// One work item, one warp.  WIDE: 16 rows, hi and lo parts as two products into one
 // accumulator; else 8 rows, the tensor-core tile's rows 0-7 their hi parts and
 // rows 8-15 their lo parts, whose two results meet in one thread.
 //
@@ -196,131 +193,144 @@ struct KvaShape {
 // long as both operands agree, and is chosen so that every fragment comes from wide
 // reads: of a K row a lane reads 16 bytes (dims 64 j + 16 c ..), each of its four
 // words one step's fragment; of V it reads its columns (16 g ..) of the four keys
-// that its score accumulators belong to, and pairs their bytes.  Each warp copies
-// its own steps to shared memory (cp.async), one step ahead; the rows' 16-byte
-// units are exchanged so that both reads meet no bank twice.
+// that its score accumulators belong to, and pairs their bytes.  The codes come to
+// shared memory by cp.async, one step ahead; the rows' 16-byte units are exchanged
+// so that both reads meet no bank twice.
 template <uint32_t HDP, bool WIDE>
-__device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& it, uint8_t* smem, float* s_rf) {
+__device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& it, uint8_t* smem) {
     using S = KvaShape<HDP, WIDE>;
     constexpr uint32_t R = S::kRows, RT = WIDE ? 2u : 1u;   // RT: score rows of a thread
     constexpr uint32_t U = HDP / 16u;                       // 16-byte units of a row
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, c = lane & 3u;
+    const uint32_t lane = threadIdx.x, g = lane >> 2, c = lane & 3u;
     const uint32_t hd = p.kv.hd, G = p.group;
     const uint32_t nrows = min(R, it.rows - it.row0);
 
-    // ── the first steps' codes ──
-    uint8_t* ring = smem + S::kQBytes + warp * (kKvaStages * S::kStage);
+    // ── the first step's codes and scales ──
+    uint8_t* ring = smem + S::kQBytes;
     const uint32_t last = it.key1 - 1u;
-    constexpr uint32_t KPA = 32u / U;   // keys per copy of the warp
+    constexpr uint32_t KPA = 32u / U;   // keys per copy
     const uint32_t cu = lane % U, ck = lane / U;
+    const uint32_t k_at = ck * HDP, k_sw = 4u & (U - 1u), v_sw = 6u & (U - 1u);
     auto fetch = [&](uint32_t k0, uint32_t stage) {   // the step from key k0, a group even past the end
-        if (k0 < it.key1 && 16u * cu < hd) {
+        if (k0 < it.key1) {
             uint8_t* dst = ring + stage * S::kStage;
+            if (16u * cu < hd) {
 #pragma unroll
-            for (uint32_t i = 0; i < S::kKeys / KPA; ++i) {
-                const uint32_t k = ck + i * KPA;
-                const uint64_t off = static_cast<uint64_t>(min(k0 + k, last)) * it.stride + 16u * cu;
-                cp_async16(dst + k * HDP + 16u * (cu ^ (4u * (k & 1u) & (U - 1u))), it.k + off);
-                cp_async16(dst + S::kKeys * HDP + k * HDP + 16u * (cu ^ (k & 6u & (U - 1u))), it.v + off);
+                for (uint32_t i = 0; i < S::kKeys / KPA; ++i) {
+                    const uint32_t k = ck + i * KPA;
+                    const uint64_t off = static_cast<uint64_t>(min(k0 + k, last)) * it.stride + 16u * cu;
+                    cp_async16(dst + k_at + i * KPA * HDP + 16u * (cu ^ ((k & 1u) * k_sw)), it.k + off);
+                    cp_async16(dst + S::kKeys * HDP + k_at + i * KPA * HDP + 16u * (cu ^ (k & v_sw)), it.v + off);
+                }
+            }
+            if (lane < S::kKeys) {
+                const uint64_t off = static_cast<uint64_t>(min(k0 + lane, last)) * it.sstride;
+                cp_async4(dst + 2u * S::kKeys * HDP + 4u * lane, it.ks + off);
+                cp_async4(dst + 2u * S::kKeys * HDP + 4u * (S::kKeys + lane), it.vs + off);
             }
         }
         cp_async_commit();
     };
-    constexpr uint32_t step = S::kKeys * kKvaWarps;
-    uint32_t k0 = it.key0 + warp * S::kKeys;
+    uint32_t k0 = it.key0;
     fetch(k0, 0);
-    float sk = 0.0f, sv = 0.0f;   // K and V scale of key (lane) of the next step
-    auto fetch_scales = [&](uint32_t k) {
-        const uint32_t key = k + lane;
-        const bool in = lane < S::kKeys && key < it.key1;
-        sk = in ? __ldg(it.ks + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
-        sv = in ? __ldg(it.vs + static_cast<uint64_t>(key) * it.sstride) : 0.0f;
-    };
-    fetch_scales(k0);
 
     // ── the query rows: powers of two, then the fragments in shared memory ──
+    float rf[RT];
     {
-        constexpr uint32_t TPR = kKvaThreads / R, QN = HDP / 4u / TPR;   // threads a row, quads (4 dims) a thread
-        const uint32_t r = tid / TPR, j0 = tid % TPR, row = it.row0 + r, i = row / G;
+        constexpr uint32_t TPR = 32u / R, QN = HDP / 4u / TPR;   // lanes a row, quads (4 dims) a lane
+        constexpr uint32_t QB = QN > 16u ? 16u : QN;             // in flight at a time
+        const uint32_t r = lane / TPR, j0 = lane % TPR, row = it.row0 + r, i = row / G;
         const uint64_t at = static_cast<uint64_t>(it.t0 + static_cast<int32_t>(i)) * p.q_ld +
                             static_cast<uint64_t>(it.h * G + (row - i * G)) * hd;
-        float4 x[QN];
-        auto load = [&](const auto* q) {
+        float4 x[QB];
+        auto load = [&](uint32_t q0) {
+            auto typed = [&](const auto* q) {
 #pragma unroll
-            for (uint32_t j = 0; j < QN; ++j) {
-                const uint32_t d = 4u * (j0 + j * TPR);
-                x[j] = r < nrows && d < hd ? load4(q + at + d, p.q_wide) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+                for (uint32_t j = 0; j < QB; ++j) {
+                    const uint32_t d = 4u * (j0 + (q0 + j) * TPR);
+                    x[j] = r < nrows && d < hd ? load4(q + at + d, p.q_wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            };
+            if (p.type == QRAF_TYPE_F32) typed(static_cast<const float*>(p.q));
+            else if (p.type == QRAF_TYPE_F16) typed(static_cast<const __half*>(p.q));
+            else typed(static_cast<const __nv_bfloat16*>(p.q));
+#pragma unroll
+            for (uint32_t j = 0; j < QB; ++j)
+                x[j] = make_float4(__fmul_rn(x[j].x, p.scale_log2), __fmul_rn(x[j].y, p.scale_log2),
+                                   __fmul_rn(x[j].z, p.scale_log2), __fmul_rn(x[j].w, p.scale_log2));
         };
-        if (p.type == QRAF_TYPE_F32) load(static_cast<const float*>(p.q));
-        else if (p.type == QRAF_TYPE_F16) load(static_cast<const __half*>(p.q));
-        else load(static_cast<const __nv_bfloat16*>(p.q));
         float m = 0.0f;
+#pragma unroll 1
+        for (uint32_t q0 = 0; q0 < QN; q0 += QB) {
+            load(q0);
 #pragma unroll
-        for (uint32_t j = 0; j < QN; ++j) {
-            x[j] = make_float4(__fmul_rn(x[j].x, p.scale_log2), __fmul_rn(x[j].y, p.scale_log2), __fmul_rn(x[j].z, p.scale_log2),
-                               __fmul_rn(x[j].w, p.scale_log2));
-            m = absmax4(x[j], m);
+            for (uint32_t j = 0; j < QB; ++j) m = absmax4(x[j], m);
         }
 #pragma unroll
         for (uint32_t o = TPR / 2u; o > 0u; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         // the largest becomes 2^10 .. 2^11: hi up to 2048, lo's last bit 2^-24
         const int32_t e = max(exponent_bits(m), 11);
         const float up = pow2_bits(264 - e);
-        if (j0 == 0u) s_rf[r] = pow2_bits(e - 10);
-        uint32_t* frag = reinterpret_cast<uint32_t*>(smem);
 #pragma unroll
-        for (uint32_t j = 0; j < QN; ++j) {
-            const uint32_t d = 4u * (j0 + j * TPR);
-            uint32_t hi[2], lo[2];
-            split_f16(__fmul_rn(x[j].x, up), __fmul_rn(x[j].y, up), hi[0], lo[0]);
-            split_f16(__fmul_rn(x[j].z, up), __fmul_rn(x[j].w, up), hi[1], lo[1]);
-            const uint32_t st = 4u * (d >> 6) + ((d >> 2) & 3u), l = 4u * (r & 7u) + ((d >> 4) & 3u);
-            uint32_t* f = frag + 4u * (st * 32u + l);
-            if constexpr (WIDE) {
-                f += r >> 3;
-                f[0] = hi[0];
-                f[2] = hi[1];
-                f += 4u * S::kSteps * 32u;
-                f[0] = lo[0];
-                f[2] = lo[1];
-            } else {
-                *reinterpret_cast<uint4*>(f) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+        for (uint32_t n = 0; n < RT; ++n) rf[n] = __shfl_sync(0xFFFFFFFFu, pow2_bits(e - 10), (g + 8u * n) * TPR);
+        uint32_t* frag = reinterpret_cast<uint32_t*>(smem);
+#pragma unroll 1
+        for (uint32_t q0 = 0; q0 < QN; q0 += QB) {
+            if (QN > QB) load(q0);
+#pragma unroll
+            for (uint32_t j = 0; j < QB; ++j) {
+                const uint32_t d = 4u * (j0 + (q0 + j) * TPR);
+                uint32_t hi[2], lo[2];
+                split_f16(__fmul_rn(x[j].x, up), __fmul_rn(x[j].y, up), hi[0], lo[0]);
+                split_f16(__fmul_rn(x[j].z, up), __fmul_rn(x[j].w, up), hi[1], lo[1]);
+                const uint32_t st = 4u * (d >> 6) + ((d >> 2) & 3u), l = 4u * (r & 7u) + ((d >> 4) & 3u);
+                uint32_t* f = frag + 4u * (st * 32u + l);
+                if constexpr (WIDE) {
+                    f += r >> 3;
+                    f[0] = hi[0];
+                    f[2] = hi[1];
+                    f += 4u * S::kSteps * 32u;
+                    f[0] = lo[0];
+                    f[2] = lo[1];
+                } else {
+                    *reinterpret_cast<uint4*>(f) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+                }
             }
         }
     }
-    __syncthreads();
 
-    float rf[RT];
-    int32_t seen[RT];
+    uint32_t seen[RT];   // keys below this one are visible to the row
 #pragma unroll
     for (uint32_t e = 0; e < RT; ++e) {
         const uint32_t r = g + 8u * e, row = it.row0 + r;
-        rf[e] = s_rf[r];
-        seen[e] = it.seen0 == INT32_MAX ? INT32_MAX : it.seen0 + static_cast<int32_t>(row / G);
-        if (r >= nrows) seen[e] = 0;
-    }
+        seen[e] = it.key1;
+        if (it.seen0 != INT32_MAX && r < nrows) {
+            const int32_t n = it.seen0 + static_cast<int32_t>(row / G);
+            seen[e] = min(it.key1, static_cast<uint32_t>(max(n, 0)));
+        }
+    }   // rows past the tile's last are zeros that see every key; they are not written
+    const uint32_t all_see = __reduce_min_sync(0xFFFFFFFFu, RT == 2u ? min(seen[0], seen[RT - 1u]) : seen[0]);
     float o[S::kOut][4];
 #pragma unroll
     for (uint32_t i = 0; i < S::kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     float run_m[RT], run_l[RT];
+    int32_t vref[RT];   // the output's unit is 2^(vref - 140), every V scale seen is below 2^(vref - 126)
 #pragma unroll
     for (uint32_t e = 0; e < RT; ++e) {
         run_m[e] = -INFINITY;
         run_l[e] = 0.0f;
+        vref[e] = 14;
     }
-    int32_t vref[RT];   // the output's unit is 2^(vref - 140), every V scale seen is below 2^(vref - 126)
-#pragma unroll
-    for (uint32_t e = 0; e < RT; ++e) vref[e] = 14;
 
     uint32_t stage = 0;
 #pragma unroll 1
-    for (; k0 < it.key1; k0 += step, stage ^= 1u) {
-        fetch(k0 + step, stage ^ 1u);   // that stage's step was read before the last __syncwarp
+    for (; k0 < it.key1; k0 += S::kKeys, stage ^= 1u) {
+        fetch(k0 + S::kKeys, stage ^ 1u);   // that stage's step was read before the last __syncwarp
         cp_async_wait<1>();
-        __syncwarp();   // the other lanes' copies
+        __syncwarp();   // the other lanes' copies (and, at first, the query fragments)
         const uint8_t* kc = ring + stage * S::kStage;
         const uint8_t* vc = kc + S::kKeys * HDP;
+        const float* scales = reinterpret_cast<const float*>(vc + S::kKeys * HDP);
         // ── scores ──
         float s[S::kTiles][4];
 #pragma unroll
@@ -331,7 +341,7 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
             const bool in = 64u * j + 16u * c < hd;
 #pragma unroll
             for (uint32_t t = 0; t < S::kTiles; ++t)
-                kr[t] = in ? *reinterpret_cast<const uint4*>(kc + (8u * t + g) * HDP + 16u * ((4u * j + c) ^ (4u * (g & 1u) & (U - 1u))))
+                kr[t] = in ? *reinterpret_cast<const uint4*>(kc + (8u * t + g) * HDP + 16u * ((4u * j + c) ^ ((g & 1u) * k_sw)))
                            : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) {
@@ -354,53 +364,68 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                 }
             }
         }
-        const float sk_now = sk, sv_now = sv;
-        const uint32_t k_now = k0;
-        fetch_scales(k0 + step);
 
         // ── softmax ──
-        float x[RT][2u * S::kTiles], vsc[2u * S::kTiles];
+        float x[RT][2u * S::kTiles], vs[RT][2u * S::kTiles];   // scores, and the V scales as the row sees them
         float mt[RT];
-        int32_t ev[RT];   // the largest exponent of the V scales that the row sees (not of an infinity or NaN)
+        int32_t ev[RT];   // the largest exponent of those scales (not of an infinity or NaN)
+        {
+            const int32_t e = lane < S::kKeys && k0 + lane < it.key1 ? exponent_bits(scales[S::kKeys + lane]) : 0;
+            const int32_t most = static_cast<int32_t>(__reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(e == 255 ? 0 : e)));
 #pragma unroll
-        for (uint32_t e = 0; e < RT; ++e) {
-            mt[e] = -INFINITY;
-            ev[e] = 0;
+            for (uint32_t n = 0; n < RT; ++n) {
+                mt[n] = -INFINITY;
+                ev[n] = most;
+            }
         }
 #pragma unroll
         for (uint32_t t = 0; t < S::kTiles; ++t) {
+            const float2 ks = *reinterpret_cast<const float2*>(scales + 8u * t + 2u * c);
+            const float2 vv = *reinterpret_cast<const float2*>(scales + S::kKeys + 8u * t + 2u * c);
 #pragma unroll
-            for (uint32_t b = 0; b < 2u; ++b) {
-                const uint32_t in = 8u * t + 2u * c + b, key = k_now + in;
-                const float ks = __shfl_sync(0xFFFFFFFFu, sk_now, in);
-                vsc[2u * t + b] = __shfl_sync(0xFFFFFFFFu, sv_now, in);
-                const int32_t eb = exponent_bits(vsc[2u * t + b]);
-#pragma unroll
-                for (uint32_t e = 0; e < RT; ++e) {
-                    const float dot = WIDE ? s[t][2u * e + b] : __fadd_rn(s[t][b], s[t][2u + b]);
-                    const bool on = key < it.key1 && static_cast<int64_t>(key) < static_cast<int64_t>(seen[e]);
-                    const float v = on ? __fmul_rn(dot, __fmul_rn(ks, rf[e])) : -INFINITY;
-                    x[e][2u * t + b] = v;
-                    mt[e] = fmaxf(mt[e], v);
-                    if (on && eb < 255) ev[e] = max(ev[e], eb);
-                }
+            for (uint32_t e = 0; e < RT; ++e) {
+                const float2 dot = WIDE ? make_float2(s[t][2u * e], s[t][2u * e + 1u])
+                                        : f2_add(make_float2(s[t][0], s[t][1]), make_float2(s[t][2], s[t][3]));
+                const float2 v = f2_mul(dot, f2_mul(ks, make_float2(rf[e], rf[e])));
+                x[e][2u * t] = v.x;
+                x[e][2u * t + 1u] = v.y;
+                vs[e][2u * t] = vv.x;
+                vs[e][2u * t + 1u] = vv.y;
             }
         }
-        float alpha[RT], down[RT], m_use[RT], vup[RT];
+        if (k0 + S::kKeys > all_see) {   // the step has keys that some row does not see: weight 0 whatever they hold
+#pragma unroll
+            for (uint32_t e = 0; e < RT; ++e) {
+                ev[e] = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 2u * S::kTiles; ++i) {
+                    const int32_t eb = exponent_bits(vs[e][i]);
+                    if (k0 + 8u * (i >> 1) + 2u * c + (i & 1u) >= seen[e]) {
+                        x[e][i] = -INFINITY;
+                        vs[e][i] = 0.0f;
+                    } else if (eb < 255) {
+                        ev[e] = max(ev[e], eb);
+                    }
+                }
+                ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 1));
+                ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 2));
+            }
+        }
+        float down[RT], m_use[RT], vup[RT];
         bool moved = false;
 #pragma unroll
         for (uint32_t e = 0; e < RT; ++e) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2u * S::kTiles; ++i) mt[e] = fmaxf(mt[e], x[e][i]);
             mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 1));
             mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 2));
-            ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 1));
-            ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 2));
             const float m_new = fmaxf(run_m[e], mt[e]);
-            alpha[e] = m_new == run_m[e] ? 1.0f : ex2(__fsub_rn(run_m[e], m_new));   // 0 at the first keys
+            const float alpha = m_new == run_m[e] ? 1.0f : ex2(__fsub_rn(run_m[e], m_new));   // 0 at the first keys
             run_m[e] = m_new;
             m_use[e] = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight exp(-inf) = 0
-            run_l[e] = __fmul_rn(run_l[e], alpha[e]);
+            run_l[e] = __fmul_rn(run_l[e], alpha);
             const int32_t vnew = max(vref[e], ev[e]);
-            down[e] = __fmul_rn(alpha[e], pow2_bits(127 + vref[e] - vnew));
+            down[e] = __fmul_rn(alpha, pow2_bits(127 + vref[e] - vnew));
             vref[e] = vnew;
             vup[e] = pow2_bits(267 - vnew);   // 2^14 over the unit: weights below 2^14
             moved |= down[e] != 1.0f;
@@ -408,10 +433,12 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
             for (uint32_t i = 0; i < S::kOut; ++i) {
-                o[i][0] = __fmul_rn(o[i][0], down[0]);
-                o[i][1] = __fmul_rn(o[i][1], down[0]);
-                o[i][2] = __fmul_rn(o[i][2], down[RT - 1u]);
-                o[i][3] = __fmul_rn(o[i][3], down[RT - 1u]);
+                const float2 a = f2_mul(make_float2(o[i][0], o[i][1]), make_float2(down[0], down[0]));
+                const float2 b = f2_mul(make_float2(o[i][2], o[i][3]), make_float2(down[RT - 1u], down[RT - 1u]));
+                o[i][0] = a.x;
+                o[i][1] = a.y;
+                o[i][2] = b.x;
+                o[i][3] = b.y;
             }
         }
         uint32_t ph[RT][S::kTiles], pl[RT][S::kTiles];
@@ -419,12 +446,10 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         for (uint32_t t = 0; t < S::kTiles; ++t) {
 #pragma unroll
             for (uint32_t e = 0; e < RT; ++e) {
-                const float p0 = ex2(__fsub_rn(x[e][2u * t], m_use[e])), p1 = ex2(__fsub_rn(x[e][2u * t + 1u], m_use[e]));
-                run_l[e] = __fadd_rn(run_l[e], __fadd_rn(p0, p1));
-                // a key that this row does not see has weight 0 whatever its scale
-                const float w0 = x[e][2u * t] == -INFINITY ? 0.0f : __fmul_rn(p0, __fmul_rn(vsc[2u * t], vup[e]));
-                const float w1 = x[e][2u * t + 1u] == -INFINITY ? 0.0f : __fmul_rn(p1, __fmul_rn(vsc[2u * t + 1u], vup[e]));
-                split_f16(w0, w1, ph[e][t], pl[e][t]);
+                const float2 w = make_float2(ex2(__fsub_rn(x[e][2u * t], m_use[e])), ex2(__fsub_rn(x[e][2u * t + 1u], m_use[e])));
+                run_l[e] = __fadd_rn(run_l[e], __fadd_rn(w.x, w.y));
+                const float2 y = f2_mul(w, f2_mul(make_float2(vs[e][2u * t], vs[e][2u * t + 1u]), make_float2(vup[e], vup[e])));
+                split_f16(y.x, y.y, ph[e][t], pl[e][t]);
             }
         }
         // ── weighted sum of V ──
@@ -433,10 +458,10 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
             uint32_t vw[4][S::kWords];   // this lane's columns of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
             for (uint32_t r = 0; r < 4u; ++r) {
-                const uint32_t k = 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1);
+                const uint32_t k = 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1);   // k & 6 = 2 c
                 const uint8_t* row = vc + k * HDP;
                 if constexpr (HDP == 64u) {
-                    const uint2 w = 8u * g < hd ? *reinterpret_cast<const uint2*>(row + 16u * ((g >> 1) ^ (k & 6u & (U - 1u))) + 8u * (g & 1u))
+                    const uint2 w = 8u * g < hd ? *reinterpret_cast<const uint2*>(row + 16u * ((g >> 1) ^ (2u * c & v_sw)) + 8u * (g & 1u))
                                                 : make_uint2(0u, 0u);
                     vw[r][0] = w.x;
                     vw[r][1] = w.y;
@@ -444,7 +469,7 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
 #pragma unroll
                     for (uint32_t h = 0; h < HDP / 128u; ++h) {
                         const uint4 w = 128u * h + 16u * g < hd
-                                            ? *reinterpret_cast<const uint4*>(row + 16u * ((8u * h + g) ^ (k & 6u)))
+                                            ? *reinterpret_cast<const uint4*>(row + 16u * ((8u * h + g) ^ (2u * c & v_sw)))
                                             : make_uint4(0u, 0u, 0u, 0u);
                         vw[r][4u * h] = w.x;
                         vw[r][4u * h + 1u] = w.y;
@@ -490,85 +515,51 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
     }
     cp_async_wait<0>();
 
-    // ── join the warps ──
+    // ── the record, or with one chunk a row the output itself ──
 #pragma unroll
     for (uint32_t e = 0; e < RT; ++e) {
         run_l[e] = __fadd_rn(run_l[e], __shfl_xor_sync(0xFFFFFFFFu, run_l[e], 1));
         run_l[e] = __fadd_rn(run_l[e], __shfl_xor_sync(0xFFFFFFFFu, run_l[e], 2));
-    }
-    __syncthreads();   // every ring has been read
-    float* jo = reinterpret_cast<float*>(smem + S::kQBytes);   // [warp][row][HDP + 4]: output, max, sum
-    constexpr uint32_t LD = HDP + 4u;
-#pragma unroll
-    for (uint32_t e = 0; e < RT; ++e) {
-        float* row = jo + (warp * R + g + 8u * e) * LD;
-        const float unit = pow2_bits(vref[e] - 13);
+        const uint32_t r = g + 8u * e, row = it.row0 + r, i = row / G, head = it.h * G + (row - i * G);
+        const int32_t t = it.t0 + static_cast<int32_t>(i);
+        float* rec = p.part ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + it.chunk) * (hd + 4u)
+                            : nullptr;
+        float f = pow2_bits(vref[e] - 13);   // to numbers
+        bool live = r < nrows;
+        if (!rec) {   // the row's output, unless its run is padding
+            uint32_t slot, len;
+            for (uint32_t q = 0; q < 8u; ++q) {   // find_run takes the whole warp: one row at a time
+                const int32_t tq = __shfl_sync(0xFFFFFFFFu, t, 4u * q);
+                const bool lq = __shfl_sync(0xFFFFFFFFu, live, 4u * q);
+                bool ok = false;
+                if (lq) {
+                    const int32_t b = find_run(p.runs, tq);
+                    ok = b >= 0 && run_ok(p, static_cast<uint32_t>(b), &slot, &len);
+                }
+                if (g == q) live = ok;
+            }
+            f = run_l[e] == 0.0f ? 0.0f : __fmul_rn(f, __fdiv_rn(1.0f, run_l[e]));
+        }
+        if (!live) continue;
 #pragma unroll
         for (uint32_t b = 0; b < 2u; ++b) {
             const uint32_t n = 2u * c + b;   // column within an output tile
 #pragma unroll
             for (uint32_t w = 0; w < S::kWords; ++w) {
                 const uint32_t d = HDP == 64u ? 8u * n + 4u * w : 128u * (w >> 2) + 16u * n + 4u * (w & 3u);
+                if (d >= hd) continue;
                 float y[4];
 #pragma unroll
                 for (uint32_t j = 0; j < 4u; ++j) {
                     const float* a = o[4u * w + j];
-                    y[j] = __fmul_rn(WIDE ? a[2u * e + b] : __fadd_rn(a[b], a[2u + b]), unit);
+                    y[j] = __fmul_rn(WIDE ? a[2u * e + b] : __fadd_rn(a[b], a[2u + b]), f);
                 }
-                *reinterpret_cast<float4*>(row + d) = make_float4(y[0], y[1], y[2], y[3]);
+                const float4 v = make_float4(y[0], y[1], y[2], y[3]);
+                if (rec) *reinterpret_cast<float4*>(rec + d) = v;
+                else store4_any(p.out, p.type, static_cast<uint64_t>(t) * p.out_ld + static_cast<uint64_t>(head) * hd + d, v, p.wide);
             }
         }
-        if (c == 0u) {
-            row[HDP] = run_m[e];
-            row[HDP + 1u] = run_l[e];
-        }
-    }
-    __syncthreads();
-    for (uint32_t r = warp; r < nrows; r += kKvaWarps) {
-        const uint32_t row = it.row0 + r, i = row / G, head = it.h * G + (row - i * G);
-        const int32_t t = it.t0 + static_cast<int32_t>(i);
-        float m = -INFINITY, l = 0.0f, f[kKvaWarps];
-#pragma unroll
-        for (uint32_t w = 0; w < kKvaWarps; ++w) m = fmaxf(m, jo[(w * R + r) * LD + HDP]);
-#pragma unroll
-        for (uint32_t w = 0; w < kKvaWarps; ++w) {
-            const float mw = jo[(w * R + r) * LD + HDP];
-            f[w] = mw == -INFINITY ? 0.0f : ex2(__fsub_rn(mw, m));
-            l = fmaf(f[w], jo[(w * R + r) * LD + HDP + 1u], l);
-        }
-        float* rec = p.part ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + it.chunk) *
-                                           (hd + 4u)
-                            : nullptr;
-        bool live = true;
-        if (!rec) {   // the only chunk: this is the row's output, unless its run is padding
-            const int32_t b = find_run(p.runs, t);
-            uint32_t slot, len;
-            live = b >= 0 && run_ok(p, static_cast<uint32_t>(b), &slot, &len);
-        }
-        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-        for (uint32_t d = 4u * lane; d < hd; d += 128u) {
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (uint32_t w = 0; w < kKvaWarps; ++w) {
-                if (f[w] == 0.0f) continue;
-                const float4 a = *reinterpret_cast<const float4*>(jo + (w * R + r) * LD + d);
-                y.x = fmaf(f[w], a.x, y.x);
-                y.y = fmaf(f[w], a.y, y.y);
-                y.z = fmaf(f[w], a.z, y.z);
-                y.w = fmaf(f[w], a.w, y.w);
-            }
-            if (rec) {
-                *reinterpret_cast<float4*>(rec + d) = y;
-            } else if (live) {
-                store4_any(p.out, p.type, static_cast<uint64_t>(t) * p.out_ld + static_cast<uint64_t>(head) * hd + d,
-                           make_float4(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv), __fmul_rn(y.z, inv), __fmul_rn(y.w, inv)),
-                           p.wide);
-            }
-        }
-        if (rec && lane == 0u) {
-            rec[hd] = m;
-            rec[hd + 1u] = l;
-        }
+        if (rec && c == 0u) *reinterpret_cast<float2*>(rec + hd) = make_float2(run_m[e], run_l[e]);
     }
 }
 
@@ -610,7 +601,7 @@ __device__ __forceinline__ bool find_tile(const KvAttnParams& p, uint32_t idx, u
 
 // WIDE: prefix items and own rows in tiles of 16 rows, else own rows in tiles of 8.
 template <uint32_t HDP, bool WIDE>
-__device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem, float* s_rf) {
+__device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem) {
     const uint32_t H = p.kv.kv_heads;
     KvaItem it;
     it.sstride = H;
@@ -631,7 +622,7 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
         it.rows = p.runs.n * p.group;
         it.t0 = 0;
         it.seen0 = INT32_MAX;
-        kva_item<HDP, WIDE>(p, it, kva_smem, s_rf);
+        kva_item<HDP, WIDE>(p, it, kva_smem);
         return;
     }
     idx -= p_items;
@@ -659,15 +650,14 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
     it.t0 = t0;
     it.seen0 = static_cast<int32_t>(len) - static_cast<int32_t>(n) + 1;
     it.chunk = p.p_chunks + s;
-    kva_item<HDP, WIDE>(p, it, kva_smem, s_rf);
+    kva_item<HDP, WIDE>(p, it, kva_smem);
 }
 
 template <uint32_t HDP, bool WIDE>
-__global__ void __launch_bounds__(kKvaThreads, WIDE || HDP == 256u ? 2 : 3) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
+__global__ void __launch_bounds__(32, WIDE || HDP == 256u ? 8 : 11) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
     extern __shared__ __align__(16) uint8_t kva_smem[];
-    __shared__ float s_rf[16];
     pdl_launch_dependents();
-    kva_cta<HDP, WIDE>(p, kva_smem, s_rf);
+    kva_cta<HDP, WIDE>(p, kva_smem);
     // not to end before the prefix's kernel has: the joining kernel waits for this one alone
     if (p.chained && blockIdx.x == 0u) pdl_wait();
 }
@@ -679,13 +669,13 @@ __global__ void __launch_bounds__(kKvaThreads, WIDE || HDP == 256u ? 2 : 3) kv_a
 constexpr uint32_t kJoinFew = 16;
 
 template <uint32_t WPR>
-__global__ void __launch_bounds__(kKvaThreads) kv_attention_join_kernel(const __grid_constant__ KvAttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const __grid_constant__ KvAttnParams p) {
     constexpr uint32_t kMost = WPR == 1u ? kJoinFew : kKvaMaxChunks;
-    __shared__ float s_w[kKvaWarps / WPR][kMost];
-    __shared__ float s_o[WPR == 1u ? 1u : kKvaWarps][kKvaMaxHeadDim];
-    __shared__ float s_l[kKvaWarps];
+    __shared__ float s_w[kJoinWarps / WPR][kMost];
+    __shared__ float s_o[WPR == 1u ? 1u : kJoinWarps][kKvaMaxHeadDim];
+    __shared__ float s_l[kJoinWarps];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = p.kv.hd;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kKvaWarps / WPR) + warp / WPR;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kJoinWarps / WPR) + warp / WPR;
     const uint32_t sub = warp % WPR;
     bool live = row < static_cast<uint64_t>(p.runs.n) * p.heads;
     const uint32_t t = live ? static_cast<uint32_t>(row) / p.heads : 0u, head = static_cast<uint32_t>(row) - t * p.heads;
