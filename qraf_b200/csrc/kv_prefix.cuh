@@ -11,13 +11,15 @@
 // activations are exact in one part; for bf16 the weights take one part too: their
 // rounding, 2^-12 of themselves, is an eighth of the output's own.
 //
-// Two softmax warpgroups take the tiles in turn, each with accumulators S and O of
-// its own, so that the tensor cores work on one while the other's S becomes P (in
-// place: a thread owns a row, so it overwrites only what it has read).  The maximum
-// that weights refer to moves only when a row exceeds it by 2^4 (then the O row is
-// scaled in TMEM); weights stay below 2^15.  Eight warps turn the codes into the
-// MMA's shared-memory layout (K as it lies, V transposed, both K-major with the
-// 128-byte swizzle), with the next tile's loads in flight.
+// Two softmax warpgroups take the tiles in turn.  S becomes P in place (a thread owns
+// a row, so it overwrites only what it has read) in one of three TMEM buffers, so
+// that the scores of the tile after next are there when a warpgroup is done.  The
+// maximum that a row's weights refer to passes from tile to tile through shared
+// memory; it moves only when a tile exceeds it by 2^8 (then the O row is scaled in
+// TMEM, after the PV before), so weights stay below 2^15 and O has one accumulator.
+// Eight warps turn the codes into the MMA's shared-memory layout (K as it lies, V
+// transposed, both K-major with the 128-byte swizzle), the next tiles' codes in flight
+// (cp.async) behind them.
 //
 // The (128 rows, KV head) units times their key tiles are dealt out evenly, one
 // contiguous range a CTA and one CTA an SM; each stretch of one unit leaves a
@@ -37,8 +39,11 @@ namespace qraf_dev {
 
 constexpr uint32_t kPreThreads = 544;   // two softmax warpgroups, eight transform warps, one MMA warp
 constexpr uint32_t kPreWarpXf = 8, kPreWarpMma = 16, kPreXfThreads = 256;
-constexpr float kPreLag = 4.0f;         // log2 of how far a row may exceed the maximum it refers to
-constexpr int32_t kPreUp = 11;          // weights of p = 1 are below 2^11
+// log2 of how far a row may exceed the maximum it refers to.  With 4 the first half dozen
+// tiles still had a row to scale in nearly every warp, each waiting for the PV before; 8
+// makes that rare, and still leaves a weight's lower part 2^-31 of the largest.
+constexpr float kPreLag = 8.0f;
+constexpr int32_t kPreUp = 7;           // weights of p = 1 are below 2^7
 
 // Parts of the queries (16-bit ones are exact in one) and of the weights.
 template <typename Q>
@@ -52,16 +57,16 @@ struct PreShape {
     static constexpr uint32_t kQPart = kPreRows * HDP * 2u;            // one part of Q
     static constexpr uint32_t kKTile = kPreKeys * HDP * 2u;            // one K or V tile in fp16
     static constexpr uint32_t kRaw = kPreKeys * HDP;                   // one K or V tile in codes
-    static constexpr uint32_t kStages = 2;                             // of each in flight
-    static constexpr uint32_t kQ = 0, kK = kQ + QP * kQPart, kV = kK + kKTile;
-    static constexpr uint32_t kRawK = kV + kKTile, kRawV = kRawK + kStages * kRaw, kEnd = kRawV + kStages * kRaw;
-    static constexpr uint32_t kScales = kEnd;                          // [2][2][128] floats: K and V scales of a slot's tile
-    static constexpr uint32_t kRf = kScales + 2048u;                   // [128] row factors
-    static constexpr uint32_t kMl = kRf + 512u;                        // [2][2][128]: max and sum of each warpgroup's rows
+    static constexpr uint32_t kQ = 0, kK = kQ + QP * kQPart, kV = kK + kKTile;      // one K tile, two V tiles
+    static constexpr uint32_t kRawK = kV + 2u * kKTile, kRawV = kRawK + kRaw, kEnd = kRawV + 2u * kRaw;
+    static constexpr uint32_t kScales = kEnd;                          // [3][2][128] floats: K and V scales of a buffer's tile
+    static constexpr uint32_t kRf = kScales + 3072u;                   // [128] row factors
+    static constexpr uint32_t kM = kRf + 512u;                         // [2][128] the maxima referred to, after a tile
+    static constexpr uint32_t kMl = kM + 1024u;                        // [2][2][128]: each warpgroup's sums and their maxima
     static constexpr uint32_t kBars = kMl + 2048u;
-    static constexpr uint32_t kSmem = kBars + 128u + 1024u;            // + alignment of the tiles
+    static constexpr uint32_t kSmem = kBars + 256u + 1024u;            // + alignment of the tiles
     static constexpr uint32_t kJoinLd = HDP + 4u;                      // floats per row where the two outputs meet (over K and V)
-    static_assert(kPreRows * kJoinLd * 4u <= 2u * kKTile + 4u * kRaw, "the joined output must fit over the K and V tiles");
+    static_assert(kPreRows * kJoinLd * 4u <= 3u * kKTile, "the joined output must fit over the K and V tiles");
 };
 
 __device__ __forceinline__ void pre_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -105,19 +110,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
         : "memory");
 }
 
-// One tile's softmax for one row (thread): S at TMEM column s_col becomes P in
-// place, the row's maximum and sum move on, O at o_col is scaled where the maximum
-// moved.  The loops stay rolled: five kinds of code share the instruction caches here,
-// and unrolled (1500 instructions a tile) fetching them took a quarter of the issue
-// slots' waits.  ks, vs: the scales of the tile's keys; MASK: keys from `valid` on are not
-// there; `first`: the warpgroup's first tile of the stretch (O is written anew).
-template <uint32_t HDP, uint32_t PP, bool MASK>
-__device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, const float* ks, const float* vs, uint32_t valid,
-                                            float rf, bool first, float& m, float& l) {
-    float v[32];
+// A row's (thread's) largest scaled score of a tile: S at TMEM column s_col, ks the K
+// scales.  MASK: keys from `valid` on are not there.  The loops here and below stay
+// rolled: five kinds of code share the instruction caches, and unrolled (1500
+// instructions a tile) fetching them took a quarter of the issue slots' waits.
+template <bool MASK>
+__device__ __forceinline__ float pre_max(uint32_t s_col, const float* ks, uint32_t valid) {
     float ymax = -INFINITY;
 #pragma unroll 1
     for (uint32_t c = 0; c < 4u; ++c) {
+        float v[32];
         tmem_ld32(s_col + 32u * c, v);
         tmem_wait_ld();
 #pragma unroll
@@ -134,33 +136,18 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
             ymax = fmaxf(fmaxf(ymax, fmaxf(y.x, y.y)), fmaxf(z.x, z.y));
         }
     }
-    const float mt = __fmul_rn(ymax, rf);
-    float alpha = 1.0f;
-    if (first) {
-        m = mt > -INFINITY ? mt : 0.0f;
-    } else if (mt > __fadd_rn(m, kPreLag)) {
-        alpha = ex2(__fsub_rn(m, mt));
-        m = mt;
-    }
-    if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
-        l = __fmul_rn(l, alpha);
-#pragma unroll 1
-        for (uint32_t c = 0; c < HDP; c += 32u) {
-            tmem_ld32(o_col + c, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (uint32_t j = 0; j < 32u; j += 2u) {
-                const float2 y = f2_mul(make_float2(v[j], v[j + 1u]), make_float2(alpha, alpha));
-                v[j] = y.x;
-                v[j + 1u] = y.y;
-            }
-            tmem_st32(o_col + c, v);
-        }
-    }
+    return ymax;
+}
+
+// The row's weights, relative to the maximum m, in the place of its scores (the hi
+// parts of 32 keys, then their lo parts); returns the sum of exp(s - m).
+template <uint32_t PP, bool MASK>
+__device__ __forceinline__ float pre_weights(uint32_t s_col, const float* ks, const float* vs, uint32_t valid, float rf, float m) {
     const float2 rf2 = make_float2(rf, rf), m2 = make_float2(-m, -m), neg = make_float2(-1.0f, -1.0f);
     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
     for (uint32_t c = 0; c < 4u; ++c) {
+        float v[32];
         tmem_ld32(s_col + 32u * c, v);
         tmem_wait_ld();
         uint32_t hi[16], lo[16];
@@ -189,11 +176,36 @@ __device__ __forceinline__ void pre_softmax(uint32_t s_col, uint32_t o_col, cons
                 }
             }
         }
-        tmem_st16(s_col + 32u * c, hi);   // the chunk's hi parts, then its lo parts
+        tmem_st16(s_col + 32u * c, hi);
         if constexpr (PP == 2u) tmem_st16(s_col + 32u * c + 16u, lo);
     }
-    l = __fadd_rn(l, __fadd_rn(sum.x, sum.y));
     tmem_wait_st();
+    return __fadd_rn(sum.x, sum.y);
+}
+
+// The row's output so far times alpha.
+template <uint32_t HDP>
+__device__ __forceinline__ void pre_scale_row(uint32_t o_col, float alpha) {
+#pragma unroll 1
+    for (uint32_t c = 0; c < HDP; c += 32u) {
+        float v[32];
+        tmem_ld32(o_col + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (uint32_t j = 0; j < 32u; j += 2u) {
+            const float2 y = f2_mul(make_float2(v[j], v[j + 1u]), make_float2(alpha, alpha));
+            v[j] = y.x;
+            v[j + 1u] = y.y;
+        }
+        tmem_st32(o_col + c, v);
+    }
+    tmem_wait_st();
+}
+
+// One row of n floats (a multiple of 4, both ends 16-byte aligned) from shared to
+// global memory, in the executing thread's bulk group.
+__device__ __forceinline__ void bulk_s2g(float* dst, const float* src, uint32_t n) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(4u * n) : "memory");
 }
 
 // Q: the type of q and out.
@@ -208,8 +220,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     float* s_rf = reinterpret_cast<float*>(smem + S::kRf);
     float* s_ml = reinterpret_cast<float*>(smem + S::kMl);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t *k_ready = bars, *v_ready = bars + 2, *s_ready = bars + 4, *p_ready = bars + 6, *pv_done = bars + 8,
-             *q_ready = bars + 10, *drain = bars + 11;
+    float* s_m = reinterpret_cast<float*>(smem + S::kM);
+    // by S buffer (three): the K tile and the scales are there, S is, P is; by tile parity:
+    // the V tile is there, O has it, a warp's rows have their maxima
+    uint64_t *k_ready = bars, *s_ready = bars + 3, *p_ready = bars + 6, *v_ready = bars + 9, *pv_done = bars + 11,
+             *m_ready = bars + 13 /* [2][4] */, *q_ready = bars + 21, *drain = bars + 22;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t hd = p.kv.hd, H = p.kv.kv_heads, G = p.group;
     const uint32_t rows = p.runs.n * G;
@@ -217,12 +232,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
 
     pdl_launch_dependents();
     if (tid == 0) {
-        for (uint32_t i = 0; i < 2u; ++i) {
+        for (uint32_t i = 0; i < 3u; ++i) {
             mbar_init(&k_ready[i], 4);
-            mbar_init(&v_ready[i], 4);
             mbar_init(&s_ready[i], 1);
             mbar_init(&p_ready[i], 4);
+        }
+        for (uint32_t i = 0; i < 2u; ++i) {
+            mbar_init(&v_ready[i], 4);
             mbar_init(&pv_done[i], 1);
+            for (uint32_t j = 0; j < 4u; ++j) mbar_init(&m_ready[4u * i + j], 1);
         }
         mbar_init(q_ready, 8);
         mbar_init(drain, 1);
@@ -237,56 +255,56 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;   // columns: S of slots 0 and 1 [0, 256), O of slots 0 and 1 [256, 512)
+    const uint32_t tmem = s_tmem;   // columns: the S buffers [0, 384), O [384, 384 + HDP)
 
     const uint32_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys;
     const uint32_t w1 = pre_start(p.pre_base, p.pre_extra, blockIdx.x + 1u);
-    uint32_t used[2] = {0u, 0u};   // tiles that each slot has had, over the CTA's stretches
+    uint32_t x0 = 0u;   // tiles of the CTA's stretches before this one: tile t is the CTA's tile x0 + t
     uint32_t q_phase = 0u;
     bool ok = true;
     for (uint32_t w = pre_start(p.pre_base, p.pre_extra, blockIdx.x); w < w1;) {
         const uint32_t unit = w / T, tile0 = w - unit * T, n = min(T - tile0, w1 - w);
         const uint32_t h = unit / p.row_tiles, row0 = (unit - h * p.row_tiles) * kPreRows;
         const uint32_t key0 = tile0 * kPreKeys, key1 = min(p.prefix_len, (tile0 + n) * kPreKeys);
-        float m = -INFINITY, l = 0.0f;
-        const uint32_t slot = warp >> 2;   // of a softmax warp
+        float m = -INFINITY, l = 0.0f;       // of a softmax thread: its sum, and the maximum that it refers to
+        const uint32_t wg = warp >> 2;       // softmax warpgroup: tiles of this parity (of the stretch)
 
         if (warp < kPreWarpXf) {
-            // ── the query rows: two lanes a row, all of a lane's loads in flight ──
+            // ── the query rows: 16 a warp, all of its loads in flight ──
             {
-                constexpr uint32_t C = HDP / 16u;   // 16-byte columns of fp16 (8 elements) a lane
-                const uint32_t r = warp * 16u + (lane & 15u), c0 = (lane >> 4) * C, row = row0 + r;
-                const uint32_t t = row / G;
-                const Q* src = static_cast<const Q*>(p.q) + static_cast<uint64_t>(t) * p.q_ld +
-                               static_cast<uint64_t>(h * G + (row - t * G)) * hd + 8u * c0;
-                float4 x[2u * C];
+                constexpr uint32_t LPR = HDP / 4u, RPA = 32u / LPR, A = 16u / RPA;   // lanes a row, rows an access, accesses
+                const uint32_t ql = lane % LPR, r0 = warp * 16u + lane / LPR;
+                auto src = [&](uint32_t i) {
+                    const uint32_t row = row0 + r0 + i * RPA, t = row / G;
+                    return static_cast<const Q*>(p.q) + static_cast<uint64_t>(t) * p.q_ld +
+                           static_cast<uint64_t>(h * G + (row - t * G)) * hd + 4u * ql;
+                };
+                auto in = [&](uint32_t i) { return row0 + r0 + i * RPA < rows && 4u * ql < hd; };
+                float4 x[A];
+                if (p.q_wide) {
 #pragma unroll
-                for (uint32_t c = 0; c < 2u * C; ++c)
-                    x[c] = row < rows && 8u * c0 + 4u * c < hd && p.q_wide ? load4(src + 4u * c, true) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if (!p.q_wide && row < rows) {
+                    for (uint32_t i = 0; i < A; ++i) x[i] = in(i) ? load4(src(i), true) : make_float4(0.f, 0.f, 0.f, 0.f);
+                } else {
 #pragma unroll
-                    for (uint32_t c = 0; c < 2u * C; ++c)
-                        if (8u * c0 + 4u * c < hd) x[c] = load4(src + 4u * c, false);
+                    for (uint32_t i = 0; i < A; ++i) x[i] = in(i) ? load4(src(i), false) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                float mx = 0.0f;
+                const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
-                for (uint32_t c = 0; c < 2u * C; ++c) mx = absmax4(x[c], mx);
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-                // the largest becomes 2^10 .. 2^11, as in kva_item
-                const int32_t e = max(exponent_bits(mx), 11);
-                const float up = __fmul_rn(pow2_bits(264 - e), p.scale_log2 < 0.0f ? -1.0f : 1.0f);
-                if (lane < 16u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
+                for (uint32_t i = 0; i < A; ++i) {
+                    const uint32_t r = r0 + i * RPA;
+                    float mx = absmax4(x[i], 0.0f);
 #pragma unroll
-                for (uint32_t c = 0; c < C; ++c) {
-                    uint32_t hi[4], lo[4];
-                    split_f16(__fmul_rn(x[2u * c].x, up), __fmul_rn(x[2u * c].y, up), hi[0], lo[0]);
-                    split_f16(__fmul_rn(x[2u * c].z, up), __fmul_rn(x[2u * c].w, up), hi[1], lo[1]);
-                    split_f16(__fmul_rn(x[2u * c + 1u].x, up), __fmul_rn(x[2u * c + 1u].y, up), hi[2], lo[2]);
-                    split_f16(__fmul_rn(x[2u * c + 1u].z, up), __fmul_rn(x[2u * c + 1u].w, up), hi[3], lo[3]);
-                    const uint32_t off = ((c0 + c) >> 3) * (kPreRows * 128u) + tc_sw128_off(r, (c0 + c) & 7u);
-                    *reinterpret_cast<uint4*>(smem + S::kQ + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (QP == 2u)
-                        *reinterpret_cast<uint4*>(smem + S::kQ + S::kQPart + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    for (uint32_t o = LPR / 2u; o > 0u; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+                    // the largest becomes 2^10 .. 2^11, as in kva_item
+                    const int32_t e = max(exponent_bits(mx), 11);
+                    const float up = __fmul_rn(pow2_bits(264 - e), sign);
+                    if (ql == 0u) s_rf[r] = __fmul_rn(pow2_bits(e - 10), fabsf(p.scale_log2));
+                    uint32_t hi[2], lo[2];
+                    split_f16(__fmul_rn(x[i].x, up), __fmul_rn(x[i].y, up), hi[0], lo[0]);
+                    split_f16(__fmul_rn(x[i].z, up), __fmul_rn(x[i].w, up), hi[1], lo[1]);
+                    const uint32_t off = (ql >> 4) * (kPreRows * 128u) + tc_sw128_off(r, (ql & 15u) >> 1) + 8u * (ql & 1u);
+                    *reinterpret_cast<uint2*>(smem + S::kQ + off) = make_uint2(hi[0], hi[1]);
+                    if constexpr (QP == 2u) *reinterpret_cast<uint2*>(smem + S::kQ + S::kQPart + off) = make_uint2(lo[0], lo[1]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -295,27 +313,51 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             asm volatile("bar.sync 2, 256;" ::: "memory");   // the row factors, across warps
 
             // ── softmax ──
-            const uint32_t lane_row = (warp & 3u) * 32u;   // TMEM lanes of this warp
-            const uint32_t s_col = tmem + (lane_row << 16) + slot * 128u, o_col = tmem + (lane_row << 16) + 256u + slot * 128u;
-            const float rf = s_rf[lane_row + lane];
-            const float* ks = s_scales + slot * 256u;
-            for (uint32_t t = slot, j = used[slot]; ok && t < n; t += 2u, ++j) {
-                ok = warp_wait(&k_ready[slot], j & 1u) && warp_wait(&s_ready[slot], j & 1u);
+            const uint32_t lane_row = (warp & 3u) * 32u, r = lane_row + lane;   // TMEM lanes of this warp; this thread's row
+            const uint32_t o_col = tmem + (lane_row << 16) + 384u;
+            const float rf = s_rf[r];
+            for (uint32_t t = wg; ok && t < n; t += 2u) {
+                const uint32_t x = x0 + t, b = x % 3u, ph = x / 3u & 1u;
+                const uint32_t s_col = tmem + (lane_row << 16) + 128u * b;
+                const float* ks = s_scales + b * 256u;
+                ok = warp_wait(&k_ready[b], ph) && warp_wait(&s_ready[b], ph);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t valid = key1 - (key0 + t * kPreKeys);
-                if (valid >= kPreKeys) pre_softmax<HDP, PP, false>(s_col, o_col, ks, ks + 128, kPreKeys, rf, t == slot, m, l);
-                else pre_softmax<HDP, PP, true>(s_col, o_col, ks, ks + 128, valid, rf, t == slot, m, l);
+                const float ymax = valid >= kPreKeys ? pre_max<false>(s_col, ks, kPreKeys) : pre_max<true>(s_col, ks, valid);
+                const float mt = __fmul_rn(ymax, rf);
+                // the maximum that the row refers to from this tile on
+                float m_now = mt > -INFINITY ? mt : 0.0f, alpha = 1.0f;
+                if (t > 0u) {
+                    const uint32_t px = x - 1u;
+                    ok = warp_wait(&m_ready[4u * (px & 1u) + (warp & 3u)], px >> 1 & 1u);
+                    if (!ok) break;
+                    const float before = s_m[(px & 1u) * 128u + r];
+                    if (mt > __fadd_rn(before, kPreLag)) alpha = ex2(__fsub_rn(before, mt));
+                    else m_now = before;
+                }
+                s_m[(x & 1u) * 128u + r] = m_now;
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(&m_ready[4u * (x & 1u) + (warp & 3u)]);
+                if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // O has the tiles before this one, and no other yet
+                    ok = warp_wait(&pv_done[(x - 1u) & 1u], (x - 1u) >> 1 & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pre_scale_row<HDP>(o_col, alpha);
+                }
+                if (m_now != m) l = m == -INFINITY ? 0.0f : __fmul_rn(l, ex2(__fsub_rn(m, m_now)));
+                m = m_now;
+                l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<PP, false>(s_col, ks, ks + 128, kPreKeys, rf, m)
+                                                   : pre_weights<PP, true>(s_col, ks, ks + 128, valid, rf, m));
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0u) mbar_arrive(&p_ready[slot]);
+                if (lane == 0u) mbar_arrive(&p_ready[b]);
             }
         } else if (warp < kPreWarpMma) {
             // ── codes -> fp16 tiles ──
-            // The MMAs run ... PV(t) S(t+2) PV(t+1) S(t+3) ...: V(t) is made while S(t+1)
-            // runs and K(t+2) while PV(t) does, so one fp16 tile of each is enough; two
-            // tiles of codes of each are in flight behind them (cp.async).  Four warps make
-            // K, four V: one chain of waits, loads and stores each.
+            // The MMAs run ... PV(t) S(t+3) PV(t+1) S(t+4) ...: K(t+3) is made while PV(t) runs
+            // and V(t+2) from then on, so K has one fp16 tile and V two, behind one and two
+            // tiles of codes in flight (cp.async).  Four warps make K, four V.
             const uint32_t xw = warp & 3u, xt = tid & 127u;
             const bool for_k = warp < kPreWarpXf + 4u;
             constexpr uint32_t U = HDP / 16u;            // 16-byte units of a row
@@ -347,7 +389,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             const uint32_t v_col = (4u * (xw & 1u) + ko) ^ (4u * (dq & 1u));   // ^ j
             auto fetch_k = [&](uint32_t t) {
                 if (t < n && k_in) {
-                    uint8_t* dst = smem + S::kRawK + (t & 1u) * S::kRaw + k_src;
+                    uint8_t* dst = smem + S::kRawK + k_src;
                     const uint32_t k0 = key0 + t * kPreKeys + k_key;
 #pragma unroll 2
                     for (uint32_t i = 0; i < KL; ++i)
@@ -394,9 +436,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     if (e < 255u) most = max(most, e);
                 }
             }
-            for (uint32_t t = 0; t < 2u; ++t) {   // a group a tile, even past the last
-                if (for_k) fetch_k(t);
-                else fetch_v(t);
+            if (for_k) {   // a group a tile, even past the last
+                fetch_k(0);
+            } else {
+                fetch_v(0);
+                fetch_v(1);
             }
             most = __reduce_max_sync(0xFFFFFFFFu, most);
             if (lane == 0u) s_unit[warp - kPreWarpXf] = most;
@@ -412,15 +456,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 vsc = in ? __ldg(p.pvs + h + static_cast<uint64_t>(key) * H) : 0.0f;
             };
             auto make_k = [&](uint32_t t) {
-                const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
-                cp_async_wait<1>();
-                const uint8_t* raw = smem + S::kRawK + sl * S::kRaw + k_src;
-                if (t > 0u) {   // the K tile is free once the previous tile's S is there
-                    const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
-                    if (!warp_wait(&s_ready[ps], pj & 1u)) return false;
-                }
-                // and the slot's scales once its previous P is written
-                if (j > 0u && !warp_wait(&p_ready[sl], (j - 1u) & 1u)) return false;
+                const uint32_t x = x0 + t, b = x % 3u;
+                cp_async_wait<0>();
+                const uint8_t* raw = smem + S::kRawK + k_src;
+                // the K tile is free once the previous tile's S is there, and the buffer's
+                // scales once its previous P is written
+                if (x > 0u && !warp_wait(&s_ready[(x - 1u) % 3u], (x - 1u) / 3u & 1u)) return false;
+                if (x > 2u && !warp_wait(&p_ready[b], (x / 3u - 1u) & 1u)) return false;
                 uint8_t* dst = smem + S::kK + k_dst;
 #pragma unroll 2
                 for (uint32_t i = 0; i < KL; ++i) {
@@ -433,24 +475,22 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     *reinterpret_cast<uint4*>(row + ((col ^ 1u) << 4)) =
                         make_uint4(codes_f16<0x4140u>(a2), codes_f16<0x4342u>(a2), codes_f16<0x4140u>(a3), codes_f16<0x4342u>(a3));
                 }
-                s_scales[sl * 256u + xt] = ksc;
-                s_scales[sl * 256u + 128u + xt] = __fmul_rn(vsc, up);
+                s_scales[b * 256u + xt] = ksc;
+                s_scales[b * 256u + 128u + xt] = __fmul_rn(vsc, up);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0u) mbar_arrive(&k_ready[sl]);
-                fetch_k(t + 2u);
+                if (lane == 0u) mbar_arrive(&k_ready[b]);
+                fetch_k(t + 1u);
                 fetch_scale(t + 1u);
                 return true;
             };
             auto make_v = [&](uint32_t t, bool fine) {
-                const uint32_t sl = t & 1u;
+                const uint32_t x = x0 + t, sl = x & 1u;
                 cp_async_wait<1>();
                 if (!all_v(fine)) return false;   // the other threads' pieces have come too
-                const uint8_t* raw = smem + S::kRawV + sl * S::kRaw + v_src;
-                if (t > 0u) {   // the V tile is free once the previous tile's O is done
-                    const uint32_t ps = sl ^ 1u, pj = used[ps] + ((t - 1u) >> 1);
-                    fine = warp_wait(&pv_done[ps], pj & 1u);
-                }
+                const uint8_t* raw = smem + S::kRawV + (t & 1u) * S::kRaw + v_src;
+                // the V tile is free once the O of the tile before the previous one is done
+                if (x > 1u) fine = warp_wait(&pv_done[sl], (x / 2u - 1u) & 1u);
 #pragma unroll 1
                 for (uint32_t b = 0; b < VB; ++b) {
                     if (!fine) break;
@@ -459,7 +499,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     uint32_t x[8];
 #pragma unroll
                     for (uint32_t i = 0; i < 8u; ++i) x[i] = in ? *reinterpret_cast<const uint32_t*>(src + i * HDP) ^ 0x80808080u : 0x80808080u;
-                    uint8_t* dst = smem + S::kV + v_dst + b * 4096u;
+                    uint8_t* dst = smem + S::kV + sl * S::kKTile + v_dst + b * 4096u;
                     uint32_t c01[4], c23[4];   // keys 2 i and 2 i + 1, byte-interleaved: dims 0-1 and 2-3
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; ++i) {
@@ -495,28 +535,28 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             const uint32_t idesc_s = (1u << 4) | ((kPreKeys >> 3) << 17) | ((kPreRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | ((HDP >> 3) << 17) | ((kPreRows >> 4) << 24);
             auto scores = [&](uint32_t t) {
-                const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
-                if (!warp_wait(&k_ready[sl], j & 1u)) return false;
+                const uint32_t x = x0 + t, b = x % 3u;
+                if (!warp_wait(&k_ready[b], x / 3u & 1u)) return false;
                 tc_fence_after();
                 if (tc_elect_one()) {
 #pragma unroll 1
                     for (uint32_t part = 0; part < QP; ++part)
 #pragma unroll 4
                         for (uint32_t k = 0; k < HDP / 16u; ++k)
-                            tc_mma_f16(tmem + sl * 128u,
+                            tc_mma_f16(tmem + b * 128u,
                                        tc_smem_desc(base + S::kQ + part * S::kQPart + (k >> 2) * (kPreRows * 128u) + (k & 3u) * 32u),
                                        tc_smem_desc(base + S::kK + (k >> 2) * (kPreKeys * 128u) + (k & 3u) * 32u),
                                        idesc_s, part + k > 0u);
-                    tc_commit(&s_ready[sl]);
+                    tc_commit(&s_ready[b]);
                 }
                 __syncwarp();
                 return true;
             };
             ok = warp_wait(q_ready, q_phase) && scores(0);
-            if (ok && n > 1u) ok = scores(1);
+            for (uint32_t t = 1; ok && t < 3u && t < n; ++t) ok = scores(t);
             for (uint32_t t = 0; ok && t < n; ++t) {
-                const uint32_t sl = t & 1u, j = used[sl] + (t >> 1);
-                ok = warp_wait(&p_ready[sl], j & 1u) && warp_wait(&v_ready[sl], j & 1u);
+                const uint32_t x = x0 + t, b = x % 3u, sl = x & 1u;
+                ok = warp_wait(&p_ready[b], x / 3u & 1u) && warp_wait(&v_ready[sl], x >> 1 & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 if (tc_elect_one()) {
@@ -524,27 +564,25 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     for (uint32_t part = 0; part < PP; ++part)
 #pragma unroll 4
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
-                            pre_mma_ts(tmem + 256u + sl * 128u, tmem + sl * 128u + 32u * (k >> 1) + 16u * part + 8u * (k & 1u),
-                                       tc_smem_desc(base + S::kV + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
-                                       t >= 2u || part + k > 0u);
+                            pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * part + 8u * (k & 1u),
+                                       tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
+                                       t + part + k > 0u);
                     tc_commit(&pv_done[sl]);
                 }
                 __syncwarp();
-                // the next S overwrites this P
-                if (t + 2u < n) ok = warp_wait(&pv_done[sl], j & 1u) && scores(t + 2u);
+                // the next S of this buffer overwrites the P that has just been used
+                if (t + 3u < n) ok = warp_wait(&pv_done[sl], x >> 1 & 1u) && scores(t + 3u);
             }
         }
-        used[0] += (n + 1u) / 2u;
-        used[1] += n / 2u;
+        x0 += n;
         q_phase ^= 1u;
-        // ── the two outputs of a row join in shared memory (over K and V) and leave as one record ──
-        const bool both = n > 1u;
+        // ── the rows leave as records, by way of shared memory (over K and V) ──
         if (warp < kPreWarpXf && ok) {
-            ok = warp_wait(&pv_done[0], (used[0] - 1u) & 1u) && (!both || warp_wait(&pv_done[1], (used[1] - 1u) & 1u));
+            ok = warp_wait(&pv_done[(x0 - 1u) & 1u], (x0 - 1u) >> 1 & 1u);   // the last, and so every one
             tc_fence_after();
             const uint32_t r = (warp & 3u) * 32u + lane;
-            s_ml[slot * 256u + r] = m;   // -inf and 0 where the slot had no tile
-            s_ml[slot * 256u + 128u + r] = l;
+            s_ml[wg * 256u + r] = m;   // -inf and 0 where the warpgroup had no tile
+            s_ml[wg * 256u + 128u + r] = l;
         }
         if (!ok) s_fail = 1u;
         __syncthreads();
@@ -562,62 +600,48 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
             const uint32_t r = (warp & 3u) * 32u + lane;
-            const float m0 = s_ml[r], m1 = s_ml[256u + r], m_all = fmaxf(m0, m1);
-            const float e0 = ex2(__fsub_rn(m0, m_all)), e1 = both ? ex2(__fsub_rn(m1, m_all)) : 0.0f;
             const float unit_f = pow2_bits(static_cast<int32_t>(most) - kPreUp + 1);
-            const float2 f0 = make_float2(__fmul_rn(e0, unit_f), __fmul_rn(e0, unit_f));
-            const float2 f1 = make_float2(__fmul_rn(e1, unit_f), __fmul_rn(e1, unit_f));
-            const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 256u;
+            const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 384u;
             float* dst = jo + r * S::kJoinLd;
 #pragma unroll 1
-            for (uint32_t c = slot * (HDP / 2u); c < (slot + 1u) * (HDP / 2u); c += 32u) {
+            for (uint32_t c = wg * (HDP / 2u); c < (wg + 1u) * (HDP / 2u); c += 32u) {
                 float v[32];
                 tmem_ld32(o_col + c, v);
                 tmem_wait_ld();
 #pragma unroll
-                for (uint32_t k = 0; k < 32u; k += 2u) {
-                    const float2 y = f2_mul(make_float2(v[k], v[k + 1u]), f0);
-                    v[k] = y.x;
-                    v[k + 1u] = y.y;
-                }
-                if (both) {
-                    float z[32];
-                    tmem_ld32(o_col + 128u + c, z);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (uint32_t k = 0; k < 32u; k += 2u) {
-                        const float2 y = f2_fma(make_float2(z[k], z[k + 1u]), f1, make_float2(v[k], v[k + 1u]));
-                        v[k] = y.x;
-                        v[k + 1u] = y.y;
-                    }
-                }
-#pragma unroll
                 for (uint32_t k = 0; k < 32u; k += 4u)
-                    *reinterpret_cast<float4*>(dst + c + k) = make_float4(v[k], v[k + 1u], v[k + 2u], v[k + 3u]);
+                    if (c + k < hd)
+                        *reinterpret_cast<float4*>(dst + c + k) = make_float4(__fmul_rn(v[k], unit_f), __fmul_rn(v[k + 1u], unit_f),
+                                                                              __fmul_rn(v[k + 2u], unit_f), __fmul_rn(v[k + 3u], unit_f));
             }
-            if (slot == 0u) {
-                dst[HDP] = m_all;
-                dst[HDP + 1u] = fmaf(e0, s_ml[128u + r], both ? __fmul_rn(e1, s_ml[256u + 128u + r]) : 0.0f);
+            if (wg == 0u) {
+                const float m_end = s_m[((x0 - 1u) & 1u) * 128u + r];
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 2u; ++i)
+                    if (s_ml[i * 256u + r] > -INFINITY)
+                        sum = fmaf(s_ml[i * 256u + 128u + r], ex2(__fsub_rn(s_ml[i * 256u + r], m_end)), sum);
+                *reinterpret_cast<float4*>(dst + hd) = make_float4(m_end, sum, 0.0f, 0.0f);
             }
             tc_fence_before();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the copies below read what was written here
         }
         __syncthreads();
-        const uint32_t chunk = blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T);
-#pragma unroll 4
-        for (uint32_t r = warp; r < kPreRows; r += kPreThreads / 32u) {
-            const uint32_t row = row0 + r;
+        if (warp < 4u) {   // one bulk copy a row
+            const uint32_t row = row0 + tid;
             if (row < rows) {
+                const uint32_t chunk = blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T);
                 const uint32_t t = row / G, head = h * G + (row - t * G);
-                float* rec = p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + chunk) * (hd + 4u);
-                const float* src = jo + r * S::kJoinLd;
-                if (4u * lane < hd) *reinterpret_cast<float4*>(rec + 4u * lane) = *reinterpret_cast<const float4*>(src + 4u * lane);
-                if (lane == 0u) *reinterpret_cast<float2*>(rec + hd) = *reinterpret_cast<const float2*>(src + HDP);
+                bulk_s2g(p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + chunk) * (hd + 4u),
+                         jo + tid * S::kJoinLd, hd + 4u);
             }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // written: K and V tiles may come, the CTA may end
         }
         w += n;
         if (w < w1) {
             tc_fence_after();
-            __syncthreads();   // the record has been read: K and V tiles may come
+            __syncthreads();   // the records have left: K and V tiles may come
         }
     }
     tc_fence_before();

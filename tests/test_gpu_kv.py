@@ -188,8 +188,8 @@ def attention64(q, cache, slots, lens, runs, prefix=None, prefix_slot=0, prefix_
     is then off by twice that (its own and the maximum's) and 2^-21; the weighted sum and the
     sum of weights lose 2^-23 of sum p |v| at each of their accumulations, two per 16 keys, and
     at each of up to 64 joins.  A weight p vs is held in two fp16 parts, scaled so that the largest
-    vs weighs 2^10 at least where p = 1: the lower part's last bit is 2^-24, so beside its relative
-    error each weight is off by up to 2^-25 2^-10 vs_max, times a code of at most 127, over a sum of
+    vs weighs 2^6 at least where p = 1: the lower part's last bit is 2^-24, so beside its relative
+    error each weight is off by up to 2^-25 2^-6 vs_max, times a code of at most 127, over a sum of
     weights of at least 1.  For bf16 a weight may be held in one part, off by 2^-12 of itself."""
     one_part = 2.0 ** -12 if "bfloat16" in str(q.dtype) and prefix_len else 0.0
     q = q.double().cpu().numpy()
@@ -219,7 +219,7 @@ def attention64(q, cache, slots, lens, runs, prefix=None, prefix_slot=0, prefix_
                     p /= p.sum(1, keepdims=True)
                     out[t] = np.einsum("hk,khd->hd", p, v)
                     size = np.einsum("hk,khd->hd", p, np.abs(v))
-                    floor = len(k) * np.abs(v).max() * 2.0 ** -35   # max |v| is 127 vs_max
+                    floor = len(k) * np.abs(v).max() * 2.0 ** -31   # max |v| is 127 vs_max
                     ds = a * (2 * dim / 16 + 8) * 2.0 ** -23
                     tol[t] = size * (2 * ds[:, None] + one_part + 2.0 ** -21 + (len(k) / 8 + 64) * 2.0 ** -23) + floor
             t += 1
