@@ -95,9 +95,8 @@ int kv_io(const qraf_kv_t* kv, const void* k, const void* v, uint32_t type, uint
     p.wide = wide_rows(k, ld_k, type) && wide_rows(v, ld_v, type);
     const uint32_t hd = kv->head_dim;
     const uint32_t hpw = hd <= 16u ? 8u : hd <= 32u ? 4u : hd <= 64u ? 2u : 1u;
-    const uint64_t tasks = static_cast<uint64_t>(n) * ((kv->kv_heads + hpw - 1u) / hpw);
-    const uint64_t ctas = (tasks + kKvIoThreads / 32u - 1u) / (kKvIoThreads / 32u);
-    const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ctas, 8ull * static_cast<uint64_t>(dev->sm_count)));
+    const uint32_t heads = hpw * (hd > 128u ? kKvIoHeads / 2u : kKvIoHeads);   // of one row a warp
+    const dim3 grid((n + kKvIoThreads / 32u - 1u) / (kKvIoThreads / 32u), (kv->kv_heads + heads - 1u) / heads);
     void (*kernel)(const KvIoParams) = store ? kv_io_pick<true>(type, hd) : kv_io_pick<false>(type, hd);
     (kernel<<<grid, kKvIoThreads, 0, st>>>(p), count_launch());
     QRAF_CUDA_TRY(cudaGetLastError());
@@ -108,7 +107,7 @@ int kv_io(const qraf_kv_t* kv, const void* k, const void* v, uint32_t type, uint
 #define PRE_MIN_ROWS 17
 #endif
 bool prefix_on_tiles(uint64_t rows, uint64_t kv_heads, uint32_t hd, uint64_t prefix_len) {
-    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 128u &&
+    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 1u &&
            (rows / kPreRows + 1u) * kv_heads * (prefix_len / kPreKeys + 1u) < (1ull << 31);   // 32-bit ranges
 }
 

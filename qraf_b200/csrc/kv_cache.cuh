@@ -7,8 +7,7 @@
 // New rows come in runs: rows cu[b] .. cu[b + 1] of the input belong to
 // consecutive cache rows starts[b], starts[b] + 1, ... of slot slots[b], so that
 // one call takes one token of every sequence, a prompt, or drafts of uneven
-// lengths.  Both directions are bound by memory: nothing is read twice, and a
-// warp has two to four 512-byte rows in flight.
+// lengths.  Both directions are bound by memory: nothing is read twice.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -120,11 +119,26 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x, bool wide) {
 __device__ __forceinline__ int8_t kvq_code(float x, float inv) {
     return static_cast<int8_t>(fmaxf(-127.0f, fminf(127.0f, roundf(__fmul_rn(x, inv)))));
 }
+// The same for four values, packed.  Without conversions: with truncating adds
+// (|y| + 0.5) + 2^23 leaves round-half-away(|y|) in the low bits, exactly (a truncated
+// sum does not reach the next integer); the bytes of negative values are negated
+// together.  A NaN (sign clear: the product's) gives 127, as the clamp of kvq_code does.
 __device__ __forceinline__ uint32_t kvq_code4(float4 x, float inv) {
-    return static_cast<uint32_t>(static_cast<uint8_t>(kvq_code(x.x, inv))) |
-           static_cast<uint32_t>(static_cast<uint8_t>(kvq_code(x.y, inv))) << 8 |
-           static_cast<uint32_t>(static_cast<uint8_t>(kvq_code(x.z, inv))) << 16 |
-           static_cast<uint32_t>(static_cast<uint8_t>(kvq_code(x.w, inv))) << 24;
+    const float y[4] = {__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv)};
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        u[i] = __float_as_uint(__fadd_rz(__fadd_rz(fminf(127.0f, fabsf(y[i])), 0.5f), 8388608.0f));
+    const uint32_t v = __byte_perm(__byte_perm(u[0], u[1], 0x0040u), __byte_perm(u[2], u[3], 0x0040u), 0x5410u);
+    // 0xFF where the value is negative (the top bytes' sign bits, replicated)
+    auto sign = [](float a, float b) {
+        uint32_t r;
+        asm("prmt.b32 %0, %1, %2, 0x00fb;" : "=r"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+        return r;
+    };
+    const uint32_t m = __byte_perm(sign(y[0], y[1]), sign(y[2], y[3]), 0x5410u);
+    const uint32_t n = v ^ m;   // per byte n - m, no borrow between bytes: v is at most 127
+    return ((n | 0x80808080u) - (m & 0x7F7F7F7Fu)) ^ ((n ^ ~m) & 0x80808080u);
 }
 __device__ __forceinline__ float4 i8x4_to_f4(uint32_t w) {
     return make_float4(static_cast<float>(static_cast<int8_t>(w)), static_cast<float>(static_cast<int8_t>(w >> 8)),
@@ -148,138 +162,141 @@ struct KvIoParams {
 
 constexpr uint32_t kKvIoThreads = 256;
 
-// Where row t of the runs lives, kept from row to row of one warp.
-struct RunCursor {
-    int32_t b = -1, lo = 0, hi = 0;   // the run that covers [lo, hi), or none there (b = -1)
-    int32_t slot = -1, first = 0;
-    bool bad = false, shared = false;   // shared: a later run writes rows of the same slot
-
-    // The whole warp calls with one t.
-    __device__ __forceinline__ void seek(const KvRuns& r, const KvView& kv, int32_t t, bool stores) {
-        if (t >= lo && t < hi) return;
-        b = find_run(r, t);
-        slot = -1;
-        bad = shared = false;
-        if (b < 0) {
-            lo = t;
-            hi = t + 1;
-            return;
-        }
-        lo = run_begin(r, b);
-        hi = r.cu ? r.cu[b + 1] : lo + 1;
-        if (t >= hi) {   // an unsorted cu
-            lo = t;
-            hi = t + 1;
-            b = -1;
-            return;
-        }
-        first = r.firsts[b];
-        const int32_t s = r.slots[b];
-        if (s == -1) return;   // a padding run
-        // the rows past the slot's end are left out one by one; a run that starts outside is bad
-        bad = s < 0 || static_cast<uint32_t>(s) >= kv.slots || first < 0 || static_cast<uint32_t>(first) >= kv.rows ||
-              static_cast<int64_t>(first) + (hi - lo) > static_cast<int64_t>(kv.rows);
-        if (s < 0 || static_cast<uint32_t>(s) >= kv.slots || first < 0) return;
-        slot = s;
-        if (stores) {
-            bool hit = false;
-            for (uint32_t j = b + 1u + (threadIdx.x & 31u); j < r.count; j += 32u) hit |= r.slots[j] == s;
-            shared = __any_sync(0xFFFFFFFFu, hit);
-        }
+// Cache row of the runs' row t, by the whole warp; *slot its slot.  -1: none (padding,
+// behind the last run, outside the slot, or, for a store, written by a later run too:
+// the last run wins, as if the runs were stored one after another).
+template <bool STORE>
+__device__ __forceinline__ int64_t place_row(const KvRuns& r, const KvView& kv, int32_t t, uint32_t* slot) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const int32_t b = find_run(r, t);
+    if (b < 0) return -1;
+    const int32_t lo = run_begin(r, b), hi = r.cu ? r.cu[b + 1] : lo + 1, s = r.slots[b], first = r.firsts[b];
+    if (s == -1 || t < lo || t >= hi) return -1;   // padding, or an unsorted cu
+    const int64_t at = static_cast<int64_t>(first) + (t - lo);
+    if (s < 0 || static_cast<uint32_t>(s) >= kv.slots || first < 0 || at >= static_cast<int64_t>(kv.rows)) {
+        if (lane == 0u) raise_error(kErrBadLaunch);
+        return -1;
     }
-    // Cache row of row t, or -1: outside the slot, or written by a later run (the
-    // last run wins, as if the runs were stored one after another).
-    __device__ __forceinline__ int64_t row(const KvRuns& r, const KvView& kv, int32_t t) const {
-        if (slot < 0) return -1;
-        const int64_t at = static_cast<int64_t>(first) + (t - lo);
-        if (at >= static_cast<int64_t>(kv.rows)) return -1;
-        if (shared) {
-            bool hit = false;
-            for (uint32_t j = static_cast<uint32_t>(b) + 1u + (threadIdx.x & 31u); j < r.count; j += 32u) {
-                if (r.slots[j] != slot) continue;
-                const int64_t f = r.firsts[j], len = r.cu ? static_cast<int64_t>(r.cu[j + 1]) - r.cu[j] : 1;
-                hit |= f >= 0 && at >= f && at < f + len;
-            }
-            if (__any_sync(0xFFFFFFFFu, hit)) return -1;
+    if constexpr (STORE) {
+        bool hit = false;
+        for (uint32_t j = static_cast<uint32_t>(b) + 1u + lane; j < r.count; j += 32u) {
+            if (r.slots[j] != s) continue;
+            const int64_t f = r.firsts[j], len = r.cu ? static_cast<int64_t>(r.cu[j + 1]) - r.cu[j] : 1;
+            hit |= f >= 0 && at >= f && at < f + len;
         }
-        return at;
+        if (__any_sync(0xFFFFFFFFu, hit)) return -1;
     }
-};
+    *slot = static_cast<uint32_t>(s);
+    return at;
+}
 
-// Warp tasks are (row, group of HPW heads); a group of LPH lanes has one head,
-// QUADS times four elements a lane.  Consecutive tasks go to one warp, so that a
-// warp looks its run up once.
+// A warp has one row's next kKvIoHeads x HPW heads (blockIdx.y: which): a group of
+// LPH lanes has one head, QUADS times four elements a lane.  A store's values are
+// loaded before its row is looked up, so that the two latencies overlap; there is no
+// loop around it: enough warps are resident to keep some 100 KB an SM in flight.
+constexpr uint32_t kKvIoHeads = 4;
+
 template <typename T, bool STORE, uint32_t LPH, uint32_t QUADS>
-__global__ void __launch_bounds__(kKvIoThreads) kv_io_kernel(const KvIoParams p) {
-    constexpr uint32_t HPW = 32u / LPH;
+__global__ void __launch_bounds__(kKvIoThreads) kv_io_kernel(const __grid_constant__ KvIoParams p) {
+    constexpr uint32_t HPW = 32u / LPH, N = QUADS == 1u ? kKvIoHeads : kKvIoHeads / 2u;
     const KvView& kv = p.kv;
-    const uint32_t lane = threadIdx.x & 31u, hd = kv.hd;
-    const uint32_t groups = (kv.kv_heads + HPW - 1u) / HPW;
-    const uint64_t tasks = static_cast<uint64_t>(p.runs.n) * groups;
-    const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kKvIoThreads / 32u);
-    const uint64_t w = static_cast<uint64_t>(blockIdx.x) * (kKvIoThreads / 32u) + (threadIdx.x >> 5);
-    const uint64_t per = (tasks + warps - 1u) / warps;
-    const uint64_t t0 = w * per, t1 = min(tasks, t0 + per);
-    RunCursor cur;
-    for (uint64_t task = t0; task < t1; ++task) {
-        const int32_t t = static_cast<int32_t>(task / groups);
-        const uint32_t g = static_cast<uint32_t>(task - static_cast<uint64_t>(t) * groups);
-        cur.seek(p.runs, kv, t, STORE);
-        if (cur.bad && lane == 0u) raise_error(kErrBadLaunch);
-        const int64_t at = cur.row(p.runs, kv, t);
-        if (at < 0) continue;
-        const uint32_t h = g * HPW + lane / LPH, l = lane % LPH;
-        const bool on = h < kv.kv_heads;
-        const uint64_t idx = (static_cast<uint64_t>(cur.slot) * kv.slot_rows + static_cast<uint64_t>(at)) * kv.kv_heads + h;
-        const uint64_t io_k = static_cast<uint64_t>(t) * p.ld_k + static_cast<uint64_t>(h) * hd;
-        const uint64_t io_v = static_cast<uint64_t>(t) * p.ld_v + static_cast<uint64_t>(h) * hd;
-        if constexpr (STORE) {
-            float4 x[2][QUADS];
-            float m[2] = {0.0f, 0.0f};
+    const uint32_t lane = threadIdx.x & 31u, hd = kv.hd, l = lane % LPH;
+    const uint32_t t = blockIdx.x * (kKvIoThreads / 32u) + (threadIdx.x >> 5);
+    if (t >= p.runs.n) return;
+    const uint32_t h0 = blockIdx.y * (N * HPW) + lane / LPH;   // this lane's first head; HPW apart
+    const uint64_t io_k = static_cast<uint64_t>(t) * p.ld_k, io_v = static_cast<uint64_t>(t) * p.ld_v;
+    uint32_t slot = 0;
+    if constexpr (STORE) {
+        float4 x[2][N][QUADS];
+        auto load = [&](bool wide) {
 #pragma unroll
-            for (uint32_t i = 0; i < QUADS; ++i) {
-                const uint32_t d = 4u * (l + i * LPH);
-                const bool in = on && d < hd;
-                x[0][i] = in ? load4(static_cast<const T*>(p.k_in) + io_k + d, p.wide) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[1][i] = in ? load4(static_cast<const T*>(p.v_in) + io_v + d, p.wide) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            for (uint32_t n = 0; n < N; ++n)
 #pragma unroll
-            for (uint32_t s = 0; s < 2u; ++s) {
-#pragma unroll
-                for (uint32_t i = 0; i < QUADS; ++i) m[s] = absmax4(x[s][i], m[s]);
-#pragma unroll
-                for (uint32_t o = LPH / 2u; o > 0u; o >>= 1) m[s] = fmaxf(m[s], __shfl_xor_sync(0xFFFFFFFFu, m[s], o));
-                const float scale = __fdiv_rn(m[s], 127.0f);
-                const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-                int8_t* codes = (s ? kv.v : kv.k) + idx * hd;
-                if (on) {
-#pragma unroll
-                    for (uint32_t i = 0; i < QUADS; ++i) {
-                        const uint32_t d = 4u * (l + i * LPH);
-                        if (d < hd) *reinterpret_cast<uint32_t*>(codes + d) = kvq_code4(x[s][i], inv);
-                    }
-                    if (l == 0u) (s ? kv.vs : kv.ks)[idx] = scale;
+                for (uint32_t i = 0; i < QUADS; ++i) {
+                    const uint32_t h = h0 + n * HPW, d = 4u * (l + i * LPH);
+                    const bool in = h < kv.kv_heads && d < hd;
+                    const uint64_t at = static_cast<uint64_t>(h) * hd + d;
+                    x[0][n][i] = in ? load4(static_cast<const T*>(p.k_in) + io_k + at, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[1][n][i] = in ? load4(static_cast<const T*>(p.v_in) + io_v + at, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
+        };
+        if (p.wide) load(true);
+        else load(false);
+        const int64_t at = place_row<true>(p.runs, kv, static_cast<int32_t>(t), &slot);
+        if (at < 0) return;
+        const uint64_t idx0 = (static_cast<uint64_t>(slot) * kv.slot_rows + static_cast<uint64_t>(at)) * kv.kv_heads;
+        // the largest of each of the 2 N rows of this lane's group; one lane a row divides
+        float most[2u * N], mine = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < 2u * N; ++k) {
+            float m = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < QUADS; ++i) m = absmax4(x[k & 1u][k >> 1][i], m);
+            if constexpr (LPH == 32u) {
+                m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
+            } else {
+#pragma unroll
+                for (uint32_t o = LPH / 2u; o > 0u; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
             }
-        } else if (on) {
-            const float ks = kv.ks[idx], vs = kv.vs[idx];
-            uint32_t w4[2][QUADS];
+            most[k] = m;
+            if (l == k % LPH) mine = m;
+        }
+        constexpr bool kShare = LPH >= 2u * N;   // lanes enough for one row each
+        const float my_scale = kShare ? __fdiv_rn(mine, 127.0f) : 0.0f;
+        const float my_inv = kShare && my_scale > 0.0f ? __fdiv_rn(1.0f, my_scale) : 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < 2u * N; ++k) {
+            const uint32_t h = h0 + (k >> 1) * HPW;
+            float scale, inv;
+            if constexpr (kShare) {
+                scale = __shfl_sync(0xFFFFFFFFu, my_scale, (lane - l) + k);
+                inv = __shfl_sync(0xFFFFFFFFu, my_inv, (lane - l) + k);
+            } else {
+                scale = __fdiv_rn(most[k], 127.0f);
+                inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+            }
+            if (h >= kv.kv_heads) continue;
+            int8_t* codes = ((k & 1u) ? kv.v : kv.k) + (idx0 + h) * hd;
 #pragma unroll
             for (uint32_t i = 0; i < QUADS; ++i) {
                 const uint32_t d = 4u * (l + i * LPH);
-                w4[0][i] = d < hd ? *reinterpret_cast<const uint32_t*>(kv.k + idx * hd + d) : 0u;
-                w4[1][i] = d < hd ? *reinterpret_cast<const uint32_t*>(kv.v + idx * hd + d) : 0u;
+                if (d < hd) *reinterpret_cast<uint32_t*>(codes + d) = kvq_code4(x[k & 1u][k >> 1][i], inv);
             }
+            if (l == 0u) ((k & 1u) ? kv.vs : kv.ks)[idx0 + h] = scale;
+        }
+    } else {
+        const int64_t at = place_row<false>(p.runs, kv, static_cast<int32_t>(t), &slot);
+        if (at < 0) return;
+        const uint64_t idx0 = (static_cast<uint64_t>(slot) * kv.slot_rows + static_cast<uint64_t>(at)) * kv.kv_heads;
+        uint32_t w[2][N][QUADS];
+        float sc[2][N];
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n) {
+            const uint32_t h = h0 + n * HPW;
+            const bool on = h < kv.kv_heads;
+            sc[0][n] = on ? kv.ks[idx0 + h] : 0.0f;
+            sc[1][n] = on ? kv.vs[idx0 + h] : 0.0f;
 #pragma unroll
             for (uint32_t i = 0; i < QUADS; ++i) {
                 const uint32_t d = 4u * (l + i * LPH);
-                if (d >= hd) continue;
-                const float4 a = i8x4_to_f4(w4[0][i]), b = i8x4_to_f4(w4[1][i]);
-                store4(static_cast<T*>(p.k_out) + io_k + d,
-                       make_float4(__fmul_rn(a.x, ks), __fmul_rn(a.y, ks), __fmul_rn(a.z, ks), __fmul_rn(a.w, ks)), p.wide);
-                store4(static_cast<T*>(p.v_out) + io_v + d,
-                       make_float4(__fmul_rn(b.x, vs), __fmul_rn(b.y, vs), __fmul_rn(b.z, vs), __fmul_rn(b.w, vs)), p.wide);
+                w[0][n][i] = on && d < hd ? *reinterpret_cast<const uint32_t*>(kv.k + (idx0 + h) * hd + d) : 0u;
+                w[1][n][i] = on && d < hd ? *reinterpret_cast<const uint32_t*>(kv.v + (idx0 + h) * hd + d) : 0u;
             }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n) {
+            const uint32_t h = h0 + n * HPW;
+#pragma unroll
+            for (uint32_t s = 0; s < 2u; ++s)
+#pragma unroll
+                for (uint32_t i = 0; i < QUADS; ++i) {
+                    const uint32_t d = 4u * (l + i * LPH);
+                    if (h >= kv.kv_heads || d >= hd) continue;
+                    const float4 c = i8x4_to_f4(w[s][n][i]);
+                    const float f = sc[s][n];
+                    T* dst = static_cast<T*>(s ? p.v_out : p.k_out) + (s ? io_v : io_k) + static_cast<uint64_t>(h) * hd + d;
+                    store4(dst, make_float4(__fmul_rn(c.x, f), __fmul_rn(c.y, f), __fmul_rn(c.z, f), __fmul_rn(c.w, f)), p.wide);
+                }
         }
     }
 }

@@ -110,6 +110,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
         : "memory");
 }
 
+// warp_wait for two barriers at once: with both phases complete, as they mostly are, one
+// vote instead of two.
+__device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+    const bool fa = mbar_try_wait(a, pa), fb = mbar_try_wait(b, pb);
+    if (__all_sync(0xFFFFFFFFu, fa && fb)) return true;
+    return warp_wait(a, pa) && warp_wait(b, pb);
+}
+
 // A row's (thread's) largest scaled score of a tile: S at TMEM column s_col, ks the K
 // scales.  MASK: keys from `valid` on are not there.  The loops here and below stay
 // rolled: five kinds of code share the instruction caches, and unrolled (1500
@@ -320,7 +328,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 const uint32_t x = x0 + t, b = x % 3u, ph = x / 3u & 1u;
                 const uint32_t s_col = tmem + (lane_row << 16) + 128u * b;
                 const float* ks = s_scales + b * 256u;
-                ok = warp_wait(&k_ready[b], ph) && warp_wait(&s_ready[b], ph);
+                ok = warp_wait2(&k_ready[b], ph, &s_ready[b], ph);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t valid = key1 - (key0 + t * kPreKeys);
@@ -534,9 +542,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             const uint32_t base = smem_u32(smem);
             const uint32_t idesc_s = (1u << 4) | ((kPreKeys >> 3) << 17) | ((kPreRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | ((HDP >> 3) << 17) | ((kPreRows >> 4) << 24);
-            auto scores = [&](uint32_t t) {
+            // S of tile t into buffer x % 3, once `other` (with its parity) is complete too
+            auto scores = [&](uint32_t t, uint64_t* other, uint32_t parity) {
                 const uint32_t x = x0 + t, b = x % 3u;
-                if (!warp_wait(&k_ready[b], x / 3u & 1u)) return false;
+                if (!warp_wait2(&k_ready[b], x / 3u & 1u, other, parity)) return false;
                 tc_fence_after();
                 if (tc_elect_one()) {
 #pragma unroll 1
@@ -552,11 +561,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 __syncwarp();
                 return true;
             };
-            ok = warp_wait(q_ready, q_phase) && scores(0);
-            for (uint32_t t = 1; ok && t < 3u && t < n; ++t) ok = scores(t);
+            for (uint32_t t = 0; ok && t < 3u && t < n; ++t) ok = scores(t, q_ready, q_phase);
             for (uint32_t t = 0; ok && t < n; ++t) {
                 const uint32_t x = x0 + t, b = x % 3u, sl = x & 1u;
-                ok = warp_wait(&p_ready[b], x / 3u & 1u) && warp_wait(&v_ready[sl], x >> 1 & 1u);
+                ok = warp_wait2(&p_ready[b], x / 3u & 1u, &v_ready[sl], x >> 1 & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 if (tc_elect_one()) {
@@ -571,7 +579,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 }
                 __syncwarp();
                 // the next S of this buffer overwrites the P that has just been used
-                if (t + 3u < n) ok = warp_wait(&pv_done[sl], x >> 1 & 1u) && scores(t + 3u);
+                if (t + 3u < n) ok = scores(t + 3u, &pv_done[sl], x >> 1 & 1u);
             }
         }
         x0 += n;

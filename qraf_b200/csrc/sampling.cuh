@@ -14,9 +14,15 @@
 
 namespace qraf_dev {
 
-constexpr uint32_t kProbThreads = 512;
+#ifndef PT
+#define PT 512
+#endif
+#ifndef PS
+#define PS 16384
+#endif
+constexpr uint32_t kProbThreads = PT;
 constexpr uint32_t kProbMaxCluster = 8;
-constexpr uint32_t kProbSlice = 16384;       // values of a row that a CTA keeps in shared memory, at most,
+constexpr uint32_t kProbSlice = PS;       // values of a row that a CTA keeps in shared memory, at most,
                                              // while the cluster can grow: three CTAs an SM
 constexpr uint32_t kProbSliceMax = 49152;    // with the largest cluster: one CTA an SM
 
@@ -171,10 +177,10 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 // reading the two rows once.
 __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid_constant__ VerifyParams p) {
     namespace cg = cooperative_groups;
-    __shared__ double s_rest[kVerWarps], s_row[kVerWarps];   // this CTA's parts: sums of max(p - q, 0) and of p
-    __shared__ double s_scan[kVerWarps];
+    __shared__ double s_sum[kVerWarps];   // the weights of this CTA's parts
+    __shared__ double s_scan[kVerWarps], s_from, s_goal;
     __shared__ uint32_t s_fall;
-    __shared__ int32_t s_found, s_last;
+    __shared__ int32_t s_found, s_last, s_pick;
     const cg::cluster_group cl = cg::this_cluster();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cl.block_rank(), blocks = cl.num_blocks();
     const uint32_t seq = blockIdx.x / blocks, K = p.drafts;
@@ -213,98 +219,92 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid
     // ── sums of this warp's part ──
     const uint32_t part = p.slice / kVerWarps;   // a multiple of 4
     const uint32_t a0 = min(p.vocab, rank * p.slice + warp * part), a1 = min(p.vocab, a0 + part);
-    double rest = 0.0, row = 0.0;
     auto weigh = [](float pv, float qv) { return pv > qv ? static_cast<double>(pv) - static_cast<double>(qv) : 0.0; };
-    auto take = [&](float pv, float qv) {
-        rest += weigh(pv, qv);
-        row += pv > 0.0f ? static_cast<double>(pv) : 0.0;
-    };
+    auto own = [](float pv) { return pv > 0.0f ? static_cast<double>(pv) : 0.0; };
     const bool wide = ((reinterpret_cast<uintptr_t>(pr) | reinterpret_cast<uintptr_t>(qr)) & 15u) == 0u;
-    uint32_t i = a0;
-    if (wide) {
-        const uint32_t quads = (a1 - a0) / 4u;
-        if (qr) {
+    auto sum_part = [&](bool use_rest) {
+        double sum = 0.0;
+        uint32_t i = a0;
+        if (wide) {
+            const uint32_t quads = (a1 - a0) / 4u;
+            const float4* x4 = reinterpret_cast<const float4*>(pr + a0);
+            const float4* y4 = reinterpret_cast<const float4*>(qr + a0);
+            if (use_rest) {
 #pragma unroll 4
-            for (uint32_t j = lane; j < quads; j += 32u) {
-                const float4 x = __ldg(reinterpret_cast<const float4*>(pr + a0) + j);
-                const float4 y = __ldg(reinterpret_cast<const float4*>(qr + a0) + j);
-                take(x.x, y.x);
-                take(x.y, y.y);
-                take(x.z, y.z);
-                take(x.w, y.w);
-            }
-        } else {
+                for (uint32_t j = lane; j < quads; j += 32u) {
+                    const float4 x = __ldg(x4 + j), y = __ldg(y4 + j);
+                    sum += (weigh(x.x, y.x) + weigh(x.y, y.y)) + (weigh(x.z, y.z) + weigh(x.w, y.w));
+                }
+            } else {
 #pragma unroll 4
-            for (uint32_t j = lane; j < quads; j += 32u) {
-                const float4 x = __ldg(reinterpret_cast<const float4*>(pr + a0) + j);
-                take(x.x, 0.0f);
-                take(x.y, 0.0f);
-                take(x.z, 0.0f);
-                take(x.w, 0.0f);
+                for (uint32_t j = lane; j < quads; j += 32u) {
+                    const float4 x = __ldg(x4 + j);
+                    sum += (own(x.x) + own(x.y)) + (own(x.z) + own(x.w));
+                }
             }
+            i = a0 + 4u * quads;
         }
-        i = a0 + 4u * quads;
-    }
 #pragma unroll 4
-    for (uint32_t j = i + lane; j < a1; j += 32u) take(__ldg(pr + j), qr ? __ldg(qr + j) : 0.0f);
-    rest = warp_sum_f64(rest);
-    row = warp_sum_f64(row);
-    if (lane == 0u) {
-        s_rest[warp] = rest;
-        s_row[warp] = row;
-    }
-    cl.sync();
+        for (uint32_t j = i + lane; j < a1; j += 32u) sum += use_rest ? weigh(__ldg(pr + j), __ldg(qr + j)) : own(__ldg(pr + j));
+        sum = warp_sum_f64(sum);
+        if (lane == 0u) s_sum[warp] = sum;
+    };
 
-    // ── which part holds the crossing: every warp of every CTA finds the same ──
+    // ── which part holds the crossing: the first warp of every CTA finds the same ──
     const uint32_t parts = blocks * kVerWarps;   // at most 128: four a lane
     constexpr uint32_t PPL = kVerMaxCluster * kVerWarps / 32u;
-    double mine[PPL], total = 0.0;
-    bool use_rest = true;
-    for (uint32_t pass = 0; pass < 2u; ++pass) {
-        total = 0.0;
+    bool use_rest = !all;
+    for (;;) {
+        sum_part(use_rest);
+        cl.sync();
+        if (warp == 0u) {
+            double mine[PPL], lane_sum = 0.0;
 #pragma unroll
-        for (uint32_t k = 0; k < PPL; ++k) {
-            const uint32_t j = lane * PPL + k;
-            mine[k] = j < parts ? cl.map_shared_rank(use_rest ? s_rest : s_row, j / kVerWarps)[j % kVerWarps] : 0.0;
-            total += mine[k];
-        }
-        total = warp_sum_f64(total);
-        if (total != 0.0) break;
-        use_rest = false;   // p <= q everywhere: draw from p
-    }
-    if (all) use_rest = true;   // q is zero there, so the rest is the row
-    cl.sync();   // the other CTAs' sums have been read: a CTA may leave
-    double before = 0.0;
+            for (uint32_t k = 0; k < PPL; ++k) {
+                const uint32_t j = lane * PPL + k;
+                mine[k] = j < parts ? cl.map_shared_rank(s_sum, j / kVerWarps)[j % kVerWarps] : 0.0;
+                lane_sum += mine[k];
+            }
+            double run = lane_sum;   // inclusive scan of the lanes' sums
 #pragma unroll
-    for (uint32_t k = 0; k < PPL; ++k) before += mine[k];
-    double run = before;   // inclusive scan of the lanes' sums
+            for (uint32_t o = 1u; o < 32u; o <<= 1) {
+                const double y = __shfl_up_sync(0xFFFFFFFFu, run, o);
+                if (lane >= o) run += y;
+            }
+            double acc = __shfl_up_sync(0xFFFFFFFFu, run, 1);
+            if (lane == 0u) acc = 0.0;
+            const double goal = static_cast<double>(p.u_last[seq]) * __shfl_sync(0xFFFFFFFFu, run, 31);
+            // the first part whose running sum exceeds the goal; without one (u_last of 1 or
+            // more), the last part with any weight
+            int32_t hit = -1, tail = -1;
+            double hit_start = 0.0, tail_start = 0.0;
 #pragma unroll
-    for (uint32_t o = 1u; o < 32u; o <<= 1) {
-        const double y = __shfl_up_sync(0xFFFFFFFFu, run, o);
-        if (lane >= o) run += y;
-    }
-    double start = __shfl_up_sync(0xFFFFFFFFu, run, 1);
-    if (lane == 0u) start = 0.0;
-    const double goal = static_cast<double>(p.u_last[seq]) * total;
-    // the first part whose running sum exceeds the goal; without one (u_last of 1 or
-    // more), the last part with any weight
-    int32_t hit = -1, tail = -1;
-    double hit_start = 0.0, tail_start = 0.0, acc = start;
-#pragma unroll
-    for (uint32_t k = 0; k < PPL; ++k) {
-        const int32_t j = static_cast<int32_t>(lane * PPL + k);
-        if (mine[k] > 0.0) {
-            tail = j;
-            tail_start = acc;
-            if (hit < 0 && acc + mine[k] > goal) {
-                hit = j;
-                hit_start = acc;
+            for (uint32_t k = 0; k < PPL; ++k) {
+                if (mine[k] > 0.0) {
+                    tail = static_cast<int32_t>(lane * PPL + k);
+                    tail_start = acc;
+                    if (hit < 0 && acc + mine[k] > goal) {
+                        hit = tail;
+                        hit_start = acc;
+                    }
+                }
+                acc += mine[k];
+            }
+            const uint32_t hits = __ballot_sync(0xFFFFFFFFu, hit >= 0), tails = __ballot_sync(0xFFFFFFFFu, tail >= 0);
+            const int src = hits ? __ffs(static_cast<int>(hits)) - 1 : tails ? 31 - __clz(static_cast<int>(tails)) : 0;
+            const int32_t pick = __shfl_sync(0xFFFFFFFFu, hits ? hit : tail, src);
+            const double from = __shfl_sync(0xFFFFFFFFu, hits ? hit_start : tail_start, src);
+            if (lane == 0u) {
+                s_pick = pick;   // -1: no weight at all
+                s_from = from;
+                s_goal = goal;
             }
         }
-        acc += mine[k];
+        cl.sync();   // the sums have been read, the answer is there
+        if (s_pick >= 0 || !use_rest) break;
+        use_rest = false;   // p <= q everywhere: draw from p
     }
-    const uint32_t hits = __ballot_sync(0xFFFFFFFFu, hit >= 0), tails = __ballot_sync(0xFFFFFFFFu, tail >= 0);
-    if (tails == 0u) {   // no weight at all: nothing can be drawn
+    if (s_pick < 0) {   // nothing can be drawn
         if (rank == 0u && tid == 0u) {
             raise_error(kErrBadLaunch);
             for (uint32_t k = 0; k <= K; ++k)
@@ -314,17 +314,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid
         }
         return;
     }
-    int32_t pick;
-    double from;
-    if (hits) {
-        const int src = __ffs(static_cast<int>(hits)) - 1;
-        pick = __shfl_sync(0xFFFFFFFFu, hit, src);
-        from = __shfl_sync(0xFFFFFFFFu, hit_start, src);
-    } else {
-        const int src = 31 - __clz(static_cast<int>(tails));
-        pick = __shfl_sync(0xFFFFFFFFu, tail, src);
-        from = __shfl_sync(0xFFFFFFFFu, tail_start, src);
-    }
+    const int32_t pick = s_pick;
+    const double from = s_from, goal = s_goal;
     if (static_cast<uint32_t>(pick) / kVerWarps != rank) return;
 
     // ── the token within the part, by this CTA: a stretch of it per thread ──
@@ -333,8 +324,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid
     const uint32_t c0 = min(b1, b0 + tid * per), c1 = min(b1, c0 + per);
     auto weight = [&](uint32_t j) {
         const float pv = __ldg(pr + j);
-        if (use_rest && qr) return weigh(pv, __ldg(qr + j));
-        return pv > 0.0f ? static_cast<double>(pv) : 0.0;
+        return use_rest ? weigh(pv, __ldg(qr + j)) : own(pv);
     };
     double sum = 0.0;
     for (uint32_t j = c0; j < c1; ++j) sum += weight(j);
