@@ -14,15 +14,9 @@
 
 namespace qraf_dev {
 
-#ifndef PT
-#define PT 512
-#endif
-#ifndef PS
-#define PS 16384
-#endif
-constexpr uint32_t kProbThreads = PT;
+constexpr uint32_t kProbThreads = 512;
 constexpr uint32_t kProbMaxCluster = 8;
-constexpr uint32_t kProbSlice = PS;       // values of a row that a CTA keeps in shared memory, at most,
+constexpr uint32_t kProbSlice = 16384;       // values of a row that a CTA keeps in shared memory, at most,
                                              // while the cluster can grow: three CTAs an SM
 constexpr uint32_t kProbSliceMax = 49152;    // with the largest cluster: one CTA an SM
 
@@ -41,12 +35,9 @@ __device__ __forceinline__ float ex2_probs(float x) {   // 2^x, within 2 ulp; 0 
     return y;
 }
 
-// Max or sum of v over the cluster's threads.  s_red: kProbThreads / 32 + 1 floats,
-// not reused before the cluster's next barrier.
+// Max or sum of v over the CTA's threads, to all of them.  s_red: one float a warp.
 template <bool MAX>
-__device__ __forceinline__ float cluster_reduce(float v, float* s_red) {
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cl = cg::this_cluster();
+__device__ __forceinline__ float block_reduce(float v, float* s_red) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -55,19 +46,10 @@ __device__ __forceinline__ float cluster_reduce(float v, float* s_red) {
     }
     if (lane == 0u) s_red[warp] = v;
     __syncthreads();
-    if (warp == 0u) {
-        v = lane < kProbThreads / 32u ? s_red[lane] : (MAX ? -INFINITY : 0.0f);
+    v = s_red[lane % (kProbThreads / 32u)];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-            v = MAX ? fmaxf(v, y) : __fadd_rn(v, y);
-        }
-        if (lane == 0u) s_red[kProbThreads / 32u] = v;
-    }
-    cl.sync();
-    v = MAX ? -INFINITY : 0.0f;
-    for (uint32_t r = 0; r < cl.num_blocks(); ++r) {
-        const float y = *cl.map_shared_rank(s_red + kProbThreads / 32u, r);
+    for (uint32_t o = kProbThreads / 64u; o > 0u; o >>= 1) {
+        const float y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
         v = MAX ? fmaxf(v, y) : __fadd_rn(v, y);
     }
     return v;
@@ -75,14 +57,16 @@ __device__ __forceinline__ float cluster_reduce(float v, float* s_red) {
 
 // out = exp((x - max) / T) / sum over each row; a row of nothing but -inf gives
 // zeros.  A cluster has a row and each of its CTAs a slice that stays in shared
-// memory, so the row is read once and written once: bound by memory.
+// memory, so the row is read once and written once.  A CTA takes its slice's own
+// maximum and sum, and the cluster exchanges both at once: out = e 2^(own - all) / l.
 __global__ void __launch_bounds__(kProbThreads) token_probs_kernel(const __grid_constant__ ProbParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) float prob_smem[];
-    __shared__ float s_max[kProbThreads / 32u + 1u], s_sum[kProbThreads / 32u + 1u];
+    __shared__ float s_max[kProbThreads / 32u], s_sum[kProbThreads / 32u];
+    __shared__ float2 s_ml;
     const cg::cluster_group cl = cg::this_cluster();
-    const uint32_t tid = threadIdx.x, rank = cl.block_rank();
-    const uint64_t row = blockIdx.x / cl.num_blocks();
+    const uint32_t tid = threadIdx.x, rank = cl.block_rank(), blocks = cl.num_blocks();
+    const uint64_t row = blockIdx.x / blocks;
     const uint32_t i0 = min(p.vocab, rank * p.slice), n = min(p.vocab, i0 + p.slice) - i0;
     const float* x = p.x + row * p.x_ld + i0;
     float* out = p.out + row * p.out_ld + i0;
@@ -97,49 +81,64 @@ __global__ void __launch_bounds__(kProbThreads) token_probs_kernel(const __grid_
         const uint32_t rest = hx + 4u * qx;
         if (rest + tid < n) f1(rest + tid);
     };
+    float* keep = prob_smem + 4u - hx;   // value i of the slice, its quads aligned
     each(
         [&](uint32_t i) {
             const float v = x[i];
             m = fmaxf(m, v);
-            if (p.cached) prob_smem[i + 4u - hx] = v;
+            if (p.cached) keep[i] = v;
         },
         [&](uint32_t i) {
             const float4 v = *reinterpret_cast<const float4*>(x + i);
             m = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-            if (p.cached) *reinterpret_cast<float4*>(prob_smem + i + 4u - hx) = v;
+            if (p.cached) *reinterpret_cast<float4*>(keep + i) = v;
         });
-    m = cluster_reduce<true>(m, s_max);
+    m = block_reduce<true>(m, s_max);
     const float mu = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
     auto e = [&](float v) { return ex2_probs(__fmul_rn(__fsub_rn(v, mu), p.scale)); };
     each(
         [&](uint32_t i) {
-            const float v = e(p.cached ? prob_smem[i + 4u - hx] : x[i]);
+            const float v = e(p.cached ? keep[i] : x[i]);
             l = __fadd_rn(l, v);
-            if (p.cached) prob_smem[i + 4u - hx] = v;
+            if (p.cached) keep[i] = v;
         },
         [&](uint32_t i) {
-            float4 v = *reinterpret_cast<const float4*>(p.cached ? prob_smem + i + 4u - hx : x + i);
+            float4 v = *reinterpret_cast<const float4*>(p.cached ? keep + i : x + i);
             v = make_float4(e(v.x), e(v.y), e(v.z), e(v.w));
             l = __fadd_rn(l, __fadd_rn(__fadd_rn(v.x, v.y), __fadd_rn(v.z, v.w)));
-            if (p.cached) *reinterpret_cast<float4*>(prob_smem + i + 4u - hx) = v;
+            if (p.cached) *reinterpret_cast<float4*>(keep + i) = v;
         });
-    l = cluster_reduce<false>(l, s_sum);
-    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    l = block_reduce<false>(l, s_sum);
+    float f;   // what this slice's values are multiplied by
+    if (blocks > 1u) {
+        if (tid == 0u) s_ml = make_float2(m, l);
+        cl.sync();
+        float m_all = -INFINITY, l_all = 0.0f;
+        for (uint32_t r = 0; r < blocks; ++r) m_all = fmaxf(m_all, cl.map_shared_rank(&s_ml, r)->x);
+        for (uint32_t r = 0; r < blocks; ++r) {
+            const float2 o = *cl.map_shared_rank(&s_ml, r);
+            if (o.x > -INFINITY || isnan(o.y)) l_all = fmaf(o.y, ex2_probs(__fmul_rn(__fsub_rn(o.x, m_all), p.scale)), l_all);
+        }
+        cl.barrier_arrive();   // no CTA leaves while another reads its pair
+        f = l_all == 0.0f ? 0.0f : __fdiv_rn(m > -INFINITY ? ex2_probs(__fmul_rn(__fsub_rn(m, m_all), p.scale)) : 0.0f, l_all);
+        if (isnan(l_all)) f = l_all;
+    } else {
+        f = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    }
     const bool wide = ((reinterpret_cast<uintptr_t>(out + hx)) & 15u) == 0u;
     each(
-        [&](uint32_t i) { out[i] = __fmul_rn(p.cached ? prob_smem[i + 4u - hx] : e(x[i]), inv); },
+        [&](uint32_t i) { out[i] = __fmul_rn(p.cached ? keep[i] : e(x[i]), f); },
         [&](uint32_t i) {
-            float4 v = *reinterpret_cast<const float4*>(p.cached ? prob_smem + i + 4u - hx : x + i);
+            float4 v = *reinterpret_cast<const float4*>(p.cached ? keep + i : x + i);
             if (!p.cached) v = make_float4(e(v.x), e(v.y), e(v.z), e(v.w));
-            store4(out + i, make_float4(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv), __fmul_rn(v.z, inv), __fmul_rn(v.w, inv)),
-                   wide);
+            store4(out + i, make_float4(__fmul_rn(v.x, f), __fmul_rn(v.y, f), __fmul_rn(v.z, f), __fmul_rn(v.w, f)), wide);
         });
-    cl.sync();   // no CTA leaves while another reads its sums
+    if (blocks > 1u) cl.barrier_wait();
 }
 
 // ── verification of drafts ───────────────────────────────────────────────────
-constexpr uint32_t kVerThreads = 512;
+constexpr uint32_t kVerThreads = 256;   // by registers four CTAs an SM: 64 sequences are one round of clusters
 constexpr uint32_t kVerWarps = kVerThreads / 32u;
 constexpr uint32_t kVerMaxCluster = 8;
 constexpr uint32_t kVerMaxDrafts = 256;
@@ -175,7 +174,7 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 // the slice), the sums meet in distributed shared memory, and the CTA whose part
 // holds the crossing reads that part again (from L2) to find the token.  Bound by
 // reading the two rows once.
-__global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(kVerThreads, 4) verify_drafts_kernel(const __grid_constant__ VerifyParams p) {
     namespace cg = cooperative_groups;
     __shared__ double s_sum[kVerWarps];   // the weights of this CTA's parts
     __shared__ double s_scan[kVerWarps], s_from, s_goal;
@@ -251,8 +250,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const __grid
     };
 
     // ── which part holds the crossing: the first warp of every CTA finds the same ──
-    const uint32_t parts = blocks * kVerWarps;   // at most 128: four a lane
-    constexpr uint32_t PPL = kVerMaxCluster * kVerWarps / 32u;
+    const uint32_t parts = blocks * kVerWarps;
+    constexpr uint32_t PPL = kVerMaxCluster * kVerWarps / 32u;   // parts a lane, at most
     bool use_rest = !all;
     for (;;) {
         sum_part(use_rest);
