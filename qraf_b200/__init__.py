@@ -621,9 +621,9 @@ def _allocating_on(stream, device):
 def _empty(shape, dtype, like, stream):
     """A tensor on `like`'s device for a call on `stream`."""
     if stream is None:
-        return _torch().empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     with _allocating_on(stream, like.device):
-        return _torch().empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _stream_on(stream, index: int):

@@ -134,6 +134,12 @@ int ensure_device(int* dev_out, DeviceInfo** info_out) {
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 16>, lim));
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 32>, lim));
         QRAF_CUDA_TRY(allow_smem(qmm_tc_kernel<kDtypeQ4, 64>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<64, false>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<64, true>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<128, false>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<128, true>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<256, false>, lim));
+        QRAF_CUDA_TRY(allow_smem(kv_attention_cluster_kernel<256, true>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<64, false>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<64, true>, lim));
         QRAF_CUDA_TRY(allow_smem(kv_attention_kernel<128, false>, lim));

@@ -103,17 +103,21 @@ int kv_io(const qraf_kv_t* kv, const void* k, const void* v, uint32_t type, uint
     return QRAF_OK;
 }
 
-#ifndef PRE_MIN_ROWS
-#define PRE_MIN_ROWS 17
-#endif
-bool prefix_on_tiles(uint64_t rows, uint64_t kv_heads, uint32_t hd, uint64_t prefix_len) {
-    return hd <= 128u && rows >= PRE_MIN_ROWS && prefix_len >= 1u &&
-           (rows / kPreRows + 1u) * kv_heads * (prefix_len / kPreKeys + 1u) < (1ull << 31);   // 32-bit ranges
+// Whether the prefix goes to kv_prefix_kernel's tiles of 128 rows x 128 keys, or to
+// kv_attention_kernel's of 16 rows.  Measured on a B200 (us a call, tiles / by 16; heads of
+// 128, 64 own rows): 2 KV heads, 8 rows, 8192 keys 19 / 25; 64 rows, 32768 keys 36 / 49; 8 KV
+// heads, 64 rows, 8192 keys 35 / 40; but 8 KV heads, 32 rows, 8192 keys 34 / 27, where most of
+// a tile's rows are empty and there are many tiles.
+bool prefix_on_tiles(uint64_t rows, uint64_t kv_heads, uint32_t hd, uint64_t prefix_len, int sm_count) {
+    const uint64_t tiles = (rows + kPreRows - 1u) / kPreRows * kv_heads * ((prefix_len + kPreKeys - 1u) / kPreKeys);
+    return hd <= 128u && prefix_len >= kPreKeys && tiles < (1ull << 31) &&
+           (rows >= 48u || tiles <= 3ull * static_cast<uint64_t>(sm_count));
 }
 
 struct KvaPlan {
     uint32_t row_tiles = 0, p_chunks = 0, p_chunk = 0, own_tiles = 0, splits = 0, own_wide = 0, pre_ctas = 0;
     uint32_t pre_base = 0, pre_extra = 0;
+    uint32_t cluster = 0;   // CTAs of a cluster: kv_attention_cluster_kernel has the call
     uint64_t items = 0, part_bytes = 0;
 };
 
@@ -125,7 +129,31 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
     const uint64_t G = heads / kv_heads, rows = static_cast<uint64_t>(n) * G;
     if (rows > 0x7FFFFFFFull / 16u || static_cast<uint64_t>(n) * heads > 0x7FFFFFFFull)
         return fail(QRAF_ERR_UNSUPPORTED, "%u new rows of %u heads are too many for one call", n, heads);
-    const bool tiles = prefix_len && prefix_on_tiles(rows, kv_heads, hd, prefix_len);
+    {   // kv_attention_cluster_kernel
+        const bool wide = ragged ? rows > 8ull * std::min(count, n) : G > 8u;
+        const uint64_t R = wide ? 16u : 8u, keys = hd > 128u ? 16u : 32u;
+        const uint64_t tiles = ragged ? (rows + static_cast<uint64_t>(std::min(count, n)) * (R - 1u)) / R
+                                      : static_cast<uint64_t>(count) * ((G + R - 1u) / R);
+        const uint64_t equal = ragged ? std::max<uint64_t>({1, rows / R, std::min(count, n)}) : tiles;   // for runs of equal lengths
+        const uint64_t steps = (prefix_len + keys - 1u) / keys + (max_len + keys - 1u) / keys;
+        const uint64_t groups = equal * kv_heads, room = 2ull * static_cast<uint64_t>(sm_count);   // CTAs that run at once
+        uint32_t cl = 1;
+        while (cl < 8u && steps > 4u * cl && 2u * cl * groups <= room) cl *= 2;   // a step a warp
+        // One launch where every cluster runs at once, unless a prefix makes the warps' shares
+        // long: it is read for every tile of rows here.  Measured on a B200 (us a call, cluster /
+        // the other kernels; 8 query heads a KV head of 128): 2 KV heads, 4 sequences, 512 own rows
+        // 8 / 12; 8 KV heads, 16 sequences, 2048 own rows 23 / 32; 2 KV heads, 64 sequences, 64 own
+        // rows behind 512 12 / 19, behind 2048 24 / 24; 16 behind 8192 25 / 22.
+        const uint64_t a_warp = (steps + 4u * cl - 1u) / (4u * cl);
+        if (groups * cl <= room && (!prefix_len || a_warp <= 8u)) {
+            pl->own_wide = wide;
+            pl->own_tiles = static_cast<uint32_t>(tiles);
+            pl->cluster = cl;
+            pl->items = tiles * kv_heads * cl;
+            return QRAF_OK;
+        }
+    }
+    const bool tiles = prefix_len && prefix_on_tiles(rows, kv_heads, hd, prefix_len, sm_count);
     // rows by 16: wherever the prefix is among the kernel's items (it is read once for every
     // tile of rows), or where a sequence's own rows do not fit 8
     pl->own_wide = (prefix_len && !tiles) || (ragged ? rows > 8ull * std::min(count, n) : G > 8u);
@@ -197,6 +225,27 @@ cudaError_t launch_kv(K kernel, uint64_t grid, uint32_t threads, uint32_t smem, 
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 1 : 0;
     return counted(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <uint32_t HDP, bool WIDE>
+cudaError_t launch_cluster(const KvAttnParams& p, uint64_t items, uint32_t cl, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items));
+    cfg.blockDim = dim3(32u * kKvaClusterWarps);
+    cfg.dynamicSmemBytes = kKvaClusterWarps * KvaShape<HDP, WIDE>::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cl;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return counted(cudaLaunchKernelEx(&cfg, kv_attention_cluster_kernel<HDP, WIDE>, p));
+}
+template <uint32_t HDP>
+cudaError_t launch_cluster(const KvAttnParams& p, uint64_t items, uint32_t cl, cudaStream_t st) {
+    return p.own_wide ? launch_cluster<HDP, true>(p, items, cl, st) : launch_cluster<HDP, false>(p, items, cl, st);
 }
 
 template <uint32_t HDP>
@@ -363,6 +412,12 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     p.chained = pl.pre_ctas ? 1u : 0u;
     p.part = pl.part_bytes ? static_cast<float*>(workspace_dev) : nullptr;
     const uint32_t hd = kv->head_dim;
+    if (pl.cluster) {
+        QRAF_CUDA_TRY(hd <= 64u ? launch_cluster<64>(p, pl.items, pl.cluster, st)
+                                : hd <= 128u ? launch_cluster<128>(p, pl.items, pl.cluster, st)
+                                             : launch_cluster<256>(p, pl.items, pl.cluster, st));
+        return QRAF_OK;
+    }
     if (p.pre_ctas) QRAF_CUDA_TRY(hd <= 64u ? launch_prefix<64>(p, st) : launch_prefix<128>(p, st));
     if (pl.items)
         QRAF_CUDA_TRY(hd <= 64u ? launch_kva<64>(p, pl.items, st)

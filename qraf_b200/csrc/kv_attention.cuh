@@ -22,9 +22,11 @@
 // warp has an item and is a CTA of its own: it takes steps of 32 keys, keeps
 // maximum, sum and output in registers and leaves them as the chunk's record; a
 // second kernel joins the chunks of a row, in their order, so results do not
-// depend on timing.  A call with one chunk a row writes its output at once.
+// depend on timing.  A call with one chunk a row writes its output at once, and a
+// small call joins its chunks within a thread-block cluster (one launch).
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -142,19 +144,25 @@ __device__ __forceinline__ float pow2_bits(int32_t biased) {   // 2^(biased - 12
 }
 __device__ __forceinline__ int32_t exponent_bits(float x) { return static_cast<int32_t>(__float_as_uint(x) >> 23) & 0xFF; }
 
-// What one CTA works on.
-struct KvaItem {
-    const int8_t* k;      // key 0 of this KV head
+// A span of keys of one KV head.
+struct KvaKeys {
+    const int8_t* k;      // key 0
     const int8_t* v;
     const float* ks;
     const float* vs;
+    uint32_t key0, key1;
+    int32_t seen0;        // keys that row 0's token sees (grows by one a token); INT32_MAX: all of the span
+};
+
+// What one warp works on.
+struct KvaItem {
+    KvaKeys a, b;         // one span or two
+    uint32_t spans;
     uint64_t stride;      // elements from key to key
     uint32_t sstride;     // scales from key to key
-    uint32_t key0, key1;  // the chunk
     uint32_t row0, rows;  // rows [row0, rows) of the group; row r is token t0 + r / group, head h * group + r % group
     int32_t t0;
     uint32_t h;
-    int32_t seen0;        // keys that row 0's token sees (grows by one a token); INT_MAX: all of the chunk
     uint32_t chunk;       // index of the chunk in the row's partials
 };
 
@@ -196,43 +204,45 @@ struct KvaShape {
 // that its score accumulators belong to, and pairs their bytes.  The codes come to
 // shared memory by cp.async, one step ahead; the rows' 16-byte units are exchanged
 // so that both reads meet no bank twice.
-template <uint32_t HDP, bool WIDE>
+//
+// SHARED: the record goes to the start of the warp's ring ([row][head_dim + 4]).
+template <uint32_t HDP, bool WIDE, bool SHARED>
 __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& it, uint8_t* smem) {
     using S = KvaShape<HDP, WIDE>;
     constexpr uint32_t R = S::kRows, RT = WIDE ? 2u : 1u;   // RT: score rows of a thread
     constexpr uint32_t U = HDP / 16u;                       // 16-byte units of a row
-    const uint32_t lane = threadIdx.x, g = lane >> 2, c = lane & 3u;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, c = lane & 3u;
     const uint32_t hd = p.kv.hd, G = p.group;
     const uint32_t nrows = min(R, it.rows - it.row0);
 
     // ── the first step's codes and scales ──
     uint8_t* ring = smem + S::kQBytes;
-    const uint32_t last = it.key1 - 1u;
+    KvaKeys span = it.a;
     constexpr uint32_t KPA = 32u / U;   // keys per copy
     const uint32_t cu = lane % U, ck = lane / U;
     const uint32_t k_at = ck * HDP, k_sw = 4u & (U - 1u), v_sw = 6u & (U - 1u);
     auto fetch = [&](uint32_t k0, uint32_t stage) {   // the step from key k0, a group even past the end
-        if (k0 < it.key1) {
+        if (k0 < span.key1) {
+            const uint32_t last = span.key1 - 1u;
             uint8_t* dst = ring + stage * S::kStage;
             if (16u * cu < hd) {
 #pragma unroll
                 for (uint32_t i = 0; i < S::kKeys / KPA; ++i) {
                     const uint32_t k = ck + i * KPA;
                     const uint64_t off = static_cast<uint64_t>(min(k0 + k, last)) * it.stride + 16u * cu;
-                    cp_async16(dst + k_at + i * KPA * HDP + 16u * (cu ^ ((k & 1u) * k_sw)), it.k + off);
-                    cp_async16(dst + S::kKeys * HDP + k_at + i * KPA * HDP + 16u * (cu ^ (k & v_sw)), it.v + off);
+                    cp_async16(dst + k_at + i * KPA * HDP + 16u * (cu ^ ((k & 1u) * k_sw)), span.k + off);
+                    cp_async16(dst + S::kKeys * HDP + k_at + i * KPA * HDP + 16u * (cu ^ (k & v_sw)), span.v + off);
                 }
             }
             if (lane < S::kKeys) {
                 const uint64_t off = static_cast<uint64_t>(min(k0 + lane, last)) * it.sstride;
-                cp_async4(dst + 2u * S::kKeys * HDP + 4u * lane, it.ks + off);
-                cp_async4(dst + 2u * S::kKeys * HDP + 4u * (S::kKeys + lane), it.vs + off);
+                cp_async4(dst + 2u * S::kKeys * HDP + 4u * lane, span.ks + off);
+                cp_async4(dst + 2u * S::kKeys * HDP + 4u * (S::kKeys + lane), span.vs + off);
             }
         }
         cp_async_commit();
     };
-    uint32_t k0 = it.key0;
-    fetch(k0, 0);
+    if (it.spans) fetch(span.key0, 0);
 
     // ── the query rows: powers of two, then the fragments in shared memory ──
     float rf[RT];
@@ -299,17 +309,6 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         }
     }
 
-    uint32_t seen[RT];   // keys below this one are visible to the row
-#pragma unroll
-    for (uint32_t e = 0; e < RT; ++e) {
-        const uint32_t r = g + 8u * e, row = it.row0 + r;
-        seen[e] = it.key1;
-        if (it.seen0 != INT32_MAX && r < nrows) {
-            const int32_t n = it.seen0 + static_cast<int32_t>(row / G);
-            seen[e] = min(it.key1, static_cast<uint32_t>(max(n, 0)));
-        }
-    }   // rows past the tile's last are zeros that see every key; they are not written
-    const uint32_t all_see = __reduce_min_sync(0xFFFFFFFFu, RT == 2u ? min(seen[0], seen[RT - 1u]) : seen[0]);
     float o[S::kOut][4];
 #pragma unroll
     for (uint32_t i = 0; i < S::kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -322,198 +321,217 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         vref[e] = 14;
     }
 
-    uint32_t stage = 0;
 #pragma unroll 1
-    for (; k0 < it.key1; k0 += S::kKeys, stage ^= 1u) {
-        fetch(k0 + S::kKeys, stage ^ 1u);   // that stage's step was read before the last __syncwarp
-        cp_async_wait<1>();
-        __syncwarp();   // the other lanes' copies (and, at first, the query fragments)
-        const uint8_t* kc = ring + stage * S::kStage;
-        const uint8_t* vc = kc + S::kKeys * HDP;
-        const float* scales = reinterpret_cast<const float*>(vc + S::kKeys * HDP);
-        // ── scores ──
-        float s[S::kTiles][4];
-#pragma unroll
-        for (uint32_t t = 0; t < S::kTiles; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < HDP / 64u; ++j) {
-            uint4 kr[S::kTiles];
-            const bool in = 64u * j + 16u * c < hd;
-#pragma unroll
-            for (uint32_t t = 0; t < S::kTiles; ++t)
-                kr[t] = in ? *reinterpret_cast<const uint4*>(kc + (8u * t + g) * HDP + 16u * ((4u * j + c) ^ ((g & 1u) * k_sw)))
-                           : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                const uint4 qa = reinterpret_cast<const uint4*>(smem)[(4u * j + i) * 32u + lane];
-                const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
-                uint32_t al[4];
-                if constexpr (WIDE) {
-                    const uint4 ql = reinterpret_cast<const uint4*>(smem)[(S::kSteps + 4u * j + i) * 32u + lane];
-                    al[0] = ql.x;
-                    al[1] = ql.y;
-                    al[2] = ql.z;
-                    al[3] = ql.w;
-                }
-#pragma unroll
-                for (uint32_t t = 0; t < S::kTiles; ++t) {
-                    const uint32_t w = (i == 0u ? kr[t].x : i == 1u ? kr[t].y : i == 2u ? kr[t].z : kr[t].w) ^ 0x80808080u;
-                    const uint32_t b0 = codes_f16<0x4140u>(w), b1 = codes_f16<0x4342u>(w);
-                    mma_f16(s[t], a, b0, b1);
-                    if constexpr (WIDE) mma_f16(s[t], al, b0, b1);
-                }
-            }
+    for (uint32_t n_span = 0; n_span < it.spans; ++n_span) {
+        if (n_span) {
+            span = it.b;
+            fetch(span.key0, 0);
         }
-
-        // ── softmax ──
-        float x[RT][2u * S::kTiles], vs[RT][2u * S::kTiles];   // scores, and the V scales as the row sees them
-        float mt[RT];
-        int32_t ev[RT];   // the largest exponent of those scales (not of an infinity or NaN)
-        {
-            const int32_t e = lane < S::kKeys && k0 + lane < it.key1 ? exponent_bits(scales[S::kKeys + lane]) : 0;
-            const int32_t most = static_cast<int32_t>(__reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(e == 255 ? 0 : e)));
-#pragma unroll
-            for (uint32_t n = 0; n < RT; ++n) {
-                mt[n] = -INFINITY;
-                ev[n] = most;
-            }
-        }
-#pragma unroll
-        for (uint32_t t = 0; t < S::kTiles; ++t) {
-            const float2 ks = *reinterpret_cast<const float2*>(scales + 8u * t + 2u * c);
-            const float2 vv = *reinterpret_cast<const float2*>(scales + S::kKeys + 8u * t + 2u * c);
-#pragma unroll
-            for (uint32_t e = 0; e < RT; ++e) {
-                const float2 dot = WIDE ? make_float2(s[t][2u * e], s[t][2u * e + 1u])
-                                        : f2_add(make_float2(s[t][0], s[t][1]), make_float2(s[t][2], s[t][3]));
-                const float2 v = f2_mul(dot, f2_mul(ks, make_float2(rf[e], rf[e])));
-                x[e][2u * t] = v.x;
-                x[e][2u * t + 1u] = v.y;
-                vs[e][2u * t] = vv.x;
-                vs[e][2u * t + 1u] = vv.y;
-            }
-        }
-        if (k0 + S::kKeys > all_see) {   // the step has keys that some row does not see: weight 0 whatever they hold
-#pragma unroll
-            for (uint32_t e = 0; e < RT; ++e) {
-                ev[e] = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < 2u * S::kTiles; ++i) {
-                    const int32_t eb = exponent_bits(vs[e][i]);
-                    if (k0 + 8u * (i >> 1) + 2u * c + (i & 1u) >= seen[e]) {
-                        x[e][i] = -INFINITY;
-                        vs[e][i] = 0.0f;
-                    } else if (eb < 255) {
-                        ev[e] = max(ev[e], eb);
-                    }
-                }
-                ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 1));
-                ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 2));
-            }
-        }
-        float down[RT], m_use[RT], vup[RT];
-        bool moved = false;
+        uint32_t seen[RT];   // keys below this one are visible to the row
 #pragma unroll
         for (uint32_t e = 0; e < RT; ++e) {
-#pragma unroll
-            for (uint32_t i = 0; i < 2u * S::kTiles; ++i) mt[e] = fmaxf(mt[e], x[e][i]);
-            mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 1));
-            mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 2));
-            const float m_new = fmaxf(run_m[e], mt[e]);
-            const float alpha = m_new == run_m[e] ? 1.0f : ex2(__fsub_rn(run_m[e], m_new));   // 0 at the first keys
-            run_m[e] = m_new;
-            m_use[e] = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight exp(-inf) = 0
-            run_l[e] = __fmul_rn(run_l[e], alpha);
-            const int32_t vnew = max(vref[e], ev[e]);
-            down[e] = __fmul_rn(alpha, pow2_bits(127 + vref[e] - vnew));
-            vref[e] = vnew;
-            vup[e] = pow2_bits(267 - vnew);   // 2^14 over the unit: weights below 2^14
-            moved |= down[e] != 1.0f;
-        }
-        if (__any_sync(0xFFFFFFFFu, moved)) {
-#pragma unroll
-            for (uint32_t i = 0; i < S::kOut; ++i) {
-                const float2 a = f2_mul(make_float2(o[i][0], o[i][1]), make_float2(down[0], down[0]));
-                const float2 b = f2_mul(make_float2(o[i][2], o[i][3]), make_float2(down[RT - 1u], down[RT - 1u]));
-                o[i][0] = a.x;
-                o[i][1] = a.y;
-                o[i][2] = b.x;
-                o[i][3] = b.y;
+            const uint32_t r = g + 8u * e, row = it.row0 + r;
+            seen[e] = span.key1;
+            if (span.seen0 != INT32_MAX && r < nrows) {
+                const int32_t n = span.seen0 + static_cast<int32_t>(row / G);
+                seen[e] = min(span.key1, static_cast<uint32_t>(max(n, 0)));
             }
-        }
-        uint32_t ph[RT][S::kTiles], pl[RT][S::kTiles];
+        }   // rows past the tile's last are zeros that see every key; they are not written
+        const uint32_t all_see = __reduce_min_sync(0xFFFFFFFFu, RT == 2u ? min(seen[0], seen[RT - 1u]) : seen[0]);
+        uint32_t stage = 0;
+#pragma unroll 1
+        for (uint32_t k0 = span.key0; k0 < span.key1; k0 += S::kKeys, stage ^= 1u) {
+            fetch(k0 + S::kKeys, stage ^ 1u);   // that stage's step was read before the last __syncwarp
+            cp_async_wait<1>();
+            __syncwarp();   // the other lanes' copies (and, at first, the query fragments)
+            const uint8_t* kc = ring + stage * S::kStage;
+            const uint8_t* vc = kc + S::kKeys * HDP;
+            const float* scales = reinterpret_cast<const float*>(vc + S::kKeys * HDP);
+            // ── scores ──
+            float s[S::kTiles][4];
 #pragma unroll
-        for (uint32_t t = 0; t < S::kTiles; ++t) {
+            for (uint32_t t = 0; t < S::kTiles; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-            for (uint32_t e = 0; e < RT; ++e) {
-                const float2 w = make_float2(ex2(__fsub_rn(x[e][2u * t], m_use[e])), ex2(__fsub_rn(x[e][2u * t + 1u], m_use[e])));
-                run_l[e] = __fadd_rn(run_l[e], __fadd_rn(w.x, w.y));
-                const float2 y = f2_mul(w, f2_mul(make_float2(vs[e][2u * t], vs[e][2u * t + 1u]), make_float2(vup[e], vup[e])));
-                split_f16(y.x, y.y, ph[e][t], pl[e][t]);
-            }
-        }
-        // ── weighted sum of V ──
+            for (uint32_t j = 0; j < HDP / 64u; ++j) {
+                uint4 kr[S::kTiles];
+                const bool in = 64u * j + 16u * c < hd;
 #pragma unroll
-        for (uint32_t u = 0; u < S::kKeys / 16u; ++u) {
-            uint32_t vw[4][S::kWords];   // this lane's columns of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+                for (uint32_t t = 0; t < S::kTiles; ++t)
+                    kr[t] = in ? *reinterpret_cast<const uint4*>(kc + (8u * t + g) * HDP + 16u * ((4u * j + c) ^ ((g & 1u) * k_sw)))
+                               : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-            for (uint32_t r = 0; r < 4u; ++r) {
-                const uint32_t k = 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1);   // k & 6 = 2 c
-                const uint8_t* row = vc + k * HDP;
-                if constexpr (HDP == 64u) {
-                    const uint2 w = 8u * g < hd ? *reinterpret_cast<const uint2*>(row + 16u * ((g >> 1) ^ (2u * c & v_sw)) + 8u * (g & 1u))
-                                                : make_uint2(0u, 0u);
-                    vw[r][0] = w.x;
-                    vw[r][1] = w.y;
-                } else {
+                for (uint32_t i = 0; i < 4u; ++i) {
+                    const uint4 qa = reinterpret_cast<const uint4*>(smem)[(4u * j + i) * 32u + lane];
+                    const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
+                    uint32_t al[4];
+                    if constexpr (WIDE) {
+                        const uint4 ql = reinterpret_cast<const uint4*>(smem)[(S::kSteps + 4u * j + i) * 32u + lane];
+                        al[0] = ql.x;
+                        al[1] = ql.y;
+                        al[2] = ql.z;
+                        al[3] = ql.w;
+                    }
 #pragma unroll
-                    for (uint32_t h = 0; h < HDP / 128u; ++h) {
-                        const uint4 w = 128u * h + 16u * g < hd
-                                            ? *reinterpret_cast<const uint4*>(row + 16u * ((8u * h + g) ^ (2u * c & v_sw)))
-                                            : make_uint4(0u, 0u, 0u, 0u);
-                        vw[r][4u * h] = w.x;
-                        vw[r][4u * h + 1u] = w.y;
-                        vw[r][4u * h + 2u] = w.z;
-                        vw[r][4u * h + 3u] = w.w;
+                    for (uint32_t t = 0; t < S::kTiles; ++t) {
+                        const uint32_t w = (i == 0u ? kr[t].x : i == 1u ? kr[t].y : i == 2u ? kr[t].z : kr[t].w) ^ 0x80808080u;
+                        const uint32_t b0 = codes_f16<0x4140u>(w), b1 = codes_f16<0x4342u>(w);
+                        mma_f16(s[t], a, b0, b1);
+                        if constexpr (WIDE) mma_f16(s[t], al, b0, b1);
                     }
                 }
             }
-            uint32_t a[4], al[4];
-            if constexpr (WIDE) {
-                a[0] = ph[0][2u * u];
-                a[1] = ph[1][2u * u];
-                a[2] = ph[0][2u * u + 1u];
-                a[3] = ph[1][2u * u + 1u];
-                al[0] = pl[0][2u * u];
-                al[1] = pl[1][2u * u];
-                al[2] = pl[0][2u * u + 1u];
-                al[3] = pl[1][2u * u + 1u];
-            } else {
-                a[0] = ph[0][2u * u];
-                a[1] = pl[0][2u * u];
-                a[2] = ph[0][2u * u + 1u];
-                a[3] = pl[0][2u * u + 1u];
-            }
+
+            // ── softmax ──
+            float x[RT][2u * S::kTiles], vs[RT][2u * S::kTiles];   // scores, and the V scales as the row sees them
+            float mt[RT];
+            int32_t ev[RT];   // the largest exponent of those scales (not of an infinity or NaN)
+            {
+                const int32_t e = lane < S::kKeys && k0 + lane < span.key1 ? exponent_bits(scales[S::kKeys + lane]) : 0;
+                const int32_t most = static_cast<int32_t>(__reduce_max_sync(0xFFFFFFFFu, static_cast<uint32_t>(e == 255 ? 0 : e)));
 #pragma unroll
-            for (uint32_t w = 0; w < S::kWords; ++w) {
-                const uint32_t v0 = vw[0][w] ^ 0x80808080u, v1 = vw[1][w] ^ 0x80808080u;
-                const uint32_t v2 = vw[2][w] ^ 0x80808080u, v3 = vw[3][w] ^ 0x80808080u;
-                const uint32_t a01 = __byte_perm(v0, v1, 0x5140u), a23 = __byte_perm(v0, v1, 0x7362u);
-                const uint32_t b01 = __byte_perm(v2, v3, 0x5140u), b23 = __byte_perm(v2, v3, 0x7362u);
-                const uint32_t b[4][2] = {{codes_f16<0x4140u>(a01), codes_f16<0x4140u>(b01)},
-                                          {codes_f16<0x4342u>(a01), codes_f16<0x4342u>(b01)},
-                                          {codes_f16<0x4140u>(a23), codes_f16<0x4140u>(b23)},
-                                          {codes_f16<0x4342u>(a23), codes_f16<0x4342u>(b23)}};
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) {
-                    mma_f16(o[4u * w + j], a, b[j][0], b[j][1]);
-                    if constexpr (WIDE) mma_f16(o[4u * w + j], al, b[j][0], b[j][1]);
+                for (uint32_t n = 0; n < RT; ++n) {
+                    mt[n] = -INFINITY;
+                    ev[n] = most;
                 }
             }
+#pragma unroll
+            for (uint32_t t = 0; t < S::kTiles; ++t) {
+                const float2 ks = *reinterpret_cast<const float2*>(scales + 8u * t + 2u * c);
+                const float2 vv = *reinterpret_cast<const float2*>(scales + S::kKeys + 8u * t + 2u * c);
+#pragma unroll
+                for (uint32_t e = 0; e < RT; ++e) {
+                    const float2 dot = WIDE ? make_float2(s[t][2u * e], s[t][2u * e + 1u])
+                                            : f2_add(make_float2(s[t][0], s[t][1]), make_float2(s[t][2], s[t][3]));
+                    const float2 v = f2_mul(dot, f2_mul(ks, make_float2(rf[e], rf[e])));
+                    x[e][2u * t] = v.x;
+                    x[e][2u * t + 1u] = v.y;
+                    vs[e][2u * t] = vv.x;
+                    vs[e][2u * t + 1u] = vv.y;
+                }
+            }
+            if (k0 + S::kKeys > all_see) {   // the step has keys that some row does not see: weight 0 whatever they hold
+#pragma unroll
+                for (uint32_t e = 0; e < RT; ++e) {
+                    ev[e] = 0;
+#pragma unroll
+                    for (uint32_t i = 0; i < 2u * S::kTiles; ++i) {
+                        const int32_t eb = exponent_bits(vs[e][i]);
+                        if (k0 + 8u * (i >> 1) + 2u * c + (i & 1u) >= seen[e]) {
+                            x[e][i] = -INFINITY;
+                            vs[e][i] = 0.0f;
+                        } else if (eb < 255) {
+                            ev[e] = max(ev[e], eb);
+                        }
+                    }
+                    ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 1));
+                    ev[e] = max(ev[e], __shfl_xor_sync(0xFFFFFFFFu, ev[e], 2));
+                }
+            }
+            float down[RT], m_use[RT], vup[RT];
+            bool moved = false;
+#pragma unroll
+            for (uint32_t e = 0; e < RT; ++e) {
+#pragma unroll
+                for (uint32_t i = 0; i < 2u * S::kTiles; ++i) mt[e] = fmaxf(mt[e], x[e][i]);
+                mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 1));
+                mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xFFFFFFFFu, mt[e], 2));
+                const float m_new = fmaxf(run_m[e], mt[e]);
+                const float alpha = m_new == run_m[e] ? 1.0f : ex2(__fsub_rn(run_m[e], m_new));   // 0 at the first keys
+                run_m[e] = m_new;
+                m_use[e] = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight exp(-inf) = 0
+                run_l[e] = __fmul_rn(run_l[e], alpha);
+                const int32_t vnew = max(vref[e], ev[e]);
+                down[e] = __fmul_rn(alpha, pow2_bits(127 + vref[e] - vnew));
+                vref[e] = vnew;
+                vup[e] = pow2_bits(267 - vnew);   // 2^14 over the unit: weights below 2^14
+                moved |= down[e] != 1.0f;
+            }
+            if (__any_sync(0xFFFFFFFFu, moved)) {
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOut; ++i) {
+                    const float2 a = f2_mul(make_float2(o[i][0], o[i][1]), make_float2(down[0], down[0]));
+                    const float2 b = f2_mul(make_float2(o[i][2], o[i][3]), make_float2(down[RT - 1u], down[RT - 1u]));
+                    o[i][0] = a.x;
+                    o[i][1] = a.y;
+                    o[i][2] = b.x;
+                    o[i][3] = b.y;
+                }
+            }
+            uint32_t ph[RT][S::kTiles], pl[RT][S::kTiles];
+#pragma unroll
+            for (uint32_t t = 0; t < S::kTiles; ++t) {
+#pragma unroll
+                for (uint32_t e = 0; e < RT; ++e) {
+                    const float2 w = make_float2(ex2(__fsub_rn(x[e][2u * t], m_use[e])), ex2(__fsub_rn(x[e][2u * t + 1u], m_use[e])));
+                    run_l[e] = __fadd_rn(run_l[e], __fadd_rn(w.x, w.y));
+                    const float2 y = f2_mul(w, f2_mul(make_float2(vs[e][2u * t], vs[e][2u * t + 1u]), make_float2(vup[e], vup[e])));
+                    split_f16(y.x, y.y, ph[e][t], pl[e][t]);
+                }
+            }
+            // ── weighted sum of V ──
+#pragma unroll
+            for (uint32_t u = 0; u < S::kKeys / 16u; ++u) {
+                uint32_t vw[4][S::kWords];   // this lane's columns of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+#pragma unroll
+                for (uint32_t r = 0; r < 4u; ++r) {
+                    const uint32_t k = 16u * u + 2u * c + (r & 1u) + 8u * (r >> 1);   // k & 6 = 2 c
+                    const uint8_t* row = vc + k * HDP;
+                    if constexpr (HDP == 64u) {
+                        const uint2 w = 8u * g < hd ? *reinterpret_cast<const uint2*>(row + 16u * ((g >> 1) ^ (2u * c & v_sw)) + 8u * (g & 1u))
+                                                    : make_uint2(0u, 0u);
+                        vw[r][0] = w.x;
+                        vw[r][1] = w.y;
+                    } else {
+#pragma unroll
+                        for (uint32_t h = 0; h < HDP / 128u; ++h) {
+                            const uint4 w = 128u * h + 16u * g < hd
+                                                ? *reinterpret_cast<const uint4*>(row + 16u * ((8u * h + g) ^ (2u * c & v_sw)))
+                                                : make_uint4(0u, 0u, 0u, 0u);
+                            vw[r][4u * h] = w.x;
+                            vw[r][4u * h + 1u] = w.y;
+                            vw[r][4u * h + 2u] = w.z;
+                            vw[r][4u * h + 3u] = w.w;
+                        }
+                    }
+                }
+                uint32_t a[4], al[4];
+                if constexpr (WIDE) {
+                    a[0] = ph[0][2u * u];
+                    a[1] = ph[1][2u * u];
+                    a[2] = ph[0][2u * u + 1u];
+                    a[3] = ph[1][2u * u + 1u];
+                    al[0] = pl[0][2u * u];
+                    al[1] = pl[1][2u * u];
+                    al[2] = pl[0][2u * u + 1u];
+                    al[3] = pl[1][2u * u + 1u];
+                } else {
+                    a[0] = ph[0][2u * u];
+                    a[1] = pl[0][2u * u];
+                    a[2] = ph[0][2u * u + 1u];
+                    a[3] = pl[0][2u * u + 1u];
+                }
+#pragma unroll
+                for (uint32_t w = 0; w < S::kWords; ++w) {
+                    const uint32_t v0 = vw[0][w] ^ 0x80808080u, v1 = vw[1][w] ^ 0x80808080u;
+                    const uint32_t v2 = vw[2][w] ^ 0x80808080u, v3 = vw[3][w] ^ 0x80808080u;
+                    const uint32_t a01 = __byte_perm(v0, v1, 0x5140u), a23 = __byte_perm(v0, v1, 0x7362u);
+                    const uint32_t b01 = __byte_perm(v2, v3, 0x5140u), b23 = __byte_perm(v2, v3, 0x7362u);
+                    const uint32_t b[4][2] = {{codes_f16<0x4140u>(a01), codes_f16<0x4140u>(b01)},
+                                              {codes_f16<0x4342u>(a01), codes_f16<0x4342u>(b01)},
+                                              {codes_f16<0x4140u>(a23), codes_f16<0x4140u>(b23)},
+                                              {codes_f16<0x4342u>(a23), codes_f16<0x4342u>(b23)}};
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) {
+                        mma_f16(o[4u * w + j], a, b[j][0], b[j][1]);
+                        if constexpr (WIDE) mma_f16(o[4u * w + j], al, b[j][0], b[j][1]);
+                    }
+                }
+            }
+            __syncwarp();   // the stage has been read
         }
-        __syncwarp();   // the stage has been read
+        cp_async_wait<0>();
     }
-    cp_async_wait<0>();
+    __syncwarp();
 
     // ── the record, or with one chunk a row the output itself ──
 #pragma unroll
@@ -522,7 +540,8 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         run_l[e] = __fadd_rn(run_l[e], __shfl_xor_sync(0xFFFFFFFFu, run_l[e], 2));
         const uint32_t r = g + 8u * e, row = it.row0 + r, i = row / G, head = it.h * G + (row - i * G);
         const int32_t t = it.t0 + static_cast<int32_t>(i);
-        float* rec = p.part ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + it.chunk) * (hd + 4u)
+        float* rec = SHARED ? reinterpret_cast<float*>(ring) + r * (hd + 4u)
+                     : p.part ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + it.chunk) * (hd + 4u)
                             : nullptr;
         float f = pow2_bits(vref[e] - 13);   // to numbers
         bool live = r < nrows;
@@ -599,6 +618,42 @@ __device__ __forceinline__ bool find_tile(const KvAttnParams& p, uint32_t idx, u
     return false;
 }
 
+// The keys of a KV head: of the prefix, and of a run's slot.
+__device__ __forceinline__ KvaKeys prefix_keys(const KvAttnParams& p, uint32_t h) {
+    KvaKeys k;
+    k.k = p.pk + static_cast<uint64_t>(h) * p.kv.hd;
+    k.v = p.pv + static_cast<uint64_t>(h) * p.kv.hd;
+    k.ks = p.pks + h;
+    k.vs = p.pvs + h;
+    k.seen0 = INT32_MAX;
+    return k;
+}
+__device__ __forceinline__ KvaKeys slot_keys(const KvAttnParams& p, uint32_t h, uint32_t slot, uint32_t len, uint32_t n) {
+    const uint64_t base = static_cast<uint64_t>(slot) * p.kv.slot_rows * p.kv.kv_heads + h;
+    KvaKeys k;
+    k.k = p.kv.k + base * p.kv.hd;
+    k.v = p.kv.v + base * p.kv.hd;
+    k.ks = p.kv.ks + base;
+    k.vs = p.kv.vs + base;
+    k.seen0 = static_cast<int32_t>(len) - static_cast<int32_t>(n) + 1;
+    return k;
+}
+
+// Own-row tile `idx` of R rows into the item; false where there is none, or its run
+// is padding or out of range.
+__device__ __forceinline__ bool own_item(const KvAttnParams& p, uint32_t idx, uint32_t R, KvaItem& it, uint32_t* slot,
+                                         uint32_t* len, uint32_t* n) {
+    uint32_t b, tile;
+    if (!find_tile(p, idx, R, &b, &tile) || !run_ok(p, b, slot, len)) return false;
+    const int32_t t0 = max(run_begin(p.runs, b), 0);
+    const int32_t t1 = p.runs.cu ? min(p.runs.cu[b + 1u], static_cast<int32_t>(p.runs.n)) : t0 + 1;
+    *n = static_cast<uint32_t>(t1 - t0);
+    it.row0 = tile * R;
+    it.rows = *n * p.group;
+    it.t0 = t0;
+    return true;
+}
+
 // WIDE: prefix items and own rows in tiles of 16 rows, else own rows in tiles of 8.
 template <uint32_t HDP, bool WIDE>
 __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem) {
@@ -606,51 +661,33 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
     KvaItem it;
     it.sstride = H;
     it.stride = static_cast<uint64_t>(H) * p.kv.hd;
+    it.spans = 1u;
     uint32_t idx = blockIdx.x;
     const uint32_t p_items = !WIDE || p.pre_ctas ? 0u : p.row_tiles * H * p.p_chunks;
     if (WIDE && idx < p_items) {
         const uint32_t q = idx / p.row_tiles, rt = idx - q * p.row_tiles;
         it.chunk = q / H;
         it.h = q - it.chunk * H;
-        it.key0 = it.chunk * p.p_chunk;
-        it.key1 = min(p.prefix_len, it.key0 + p.p_chunk);
-        it.k = p.pk + static_cast<uint64_t>(it.h) * p.kv.hd;
-        it.v = p.pv + static_cast<uint64_t>(it.h) * p.kv.hd;
-        it.ks = p.pks + it.h;
-        it.vs = p.pvs + it.h;
+        it.a = prefix_keys(p, it.h);
+        it.a.key0 = it.chunk * p.p_chunk;
+        it.a.key1 = min(p.prefix_len, it.a.key0 + p.p_chunk);
         it.row0 = rt * 16u;
         it.rows = p.runs.n * p.group;
         it.t0 = 0;
-        it.seen0 = INT32_MAX;
-        kva_item<HDP, WIDE>(p, it, kva_smem);
-        return;
+    } else {
+        idx -= p_items;
+        const uint32_t q = idx / p.splits, s = idx - q * p.splits, tile_idx = q / H;
+        it.h = q - tile_idx * H;
+        uint32_t slot, len, n, count;
+        if (!own_item(p, tile_idx, WIDE ? 16u : 8u, it, &slot, &len, &n)) return;
+        const uint32_t chunk = own_chunk(len, p.splits, &count);
+        if (s >= max(count, p.part ? 0u : 1u)) return;   // with one chunk a row, an empty slot's rows still get their zeros
+        it.a = slot_keys(p, it.h, slot, len, n);
+        it.a.key0 = s * chunk;
+        it.a.key1 = min(len, it.a.key0 + chunk);
+        it.chunk = p.p_chunks + s;
     }
-    idx -= p_items;
-    constexpr uint32_t R = WIDE ? 16u : 8u;
-    const uint32_t q = idx / p.splits, s = idx - q * p.splits;
-    const uint32_t tile_idx = q / H;
-    it.h = q - tile_idx * H;
-    uint32_t b, tile, slot, len;
-    if (!find_tile(p, tile_idx, R, &b, &tile) || !run_ok(p, b, &slot, &len)) return;
-    const int32_t t0 = max(run_begin(p.runs, b), 0);
-    const int32_t t1 = p.runs.cu ? min(p.runs.cu[b + 1u], static_cast<int32_t>(p.runs.n)) : t0 + 1;
-    const uint32_t n = static_cast<uint32_t>(t1 - t0);
-    uint32_t count;
-    const uint32_t chunk = own_chunk(len, p.splits, &count);
-    if (s >= max(count, p.part ? 0u : 1u)) return;   // with one chunk a row, an empty slot's rows still get their zeros
-    it.key0 = s * chunk;
-    it.key1 = min(len, it.key0 + chunk);
-    const uint64_t base = static_cast<uint64_t>(slot) * p.kv.slot_rows * H + it.h;
-    it.k = p.kv.k + base * p.kv.hd;
-    it.v = p.kv.v + base * p.kv.hd;
-    it.ks = p.kv.ks + base;
-    it.vs = p.kv.vs + base;
-    it.row0 = tile * R;
-    it.rows = n * p.group;
-    it.t0 = t0;
-    it.seen0 = static_cast<int32_t>(len) - static_cast<int32_t>(n) + 1;
-    it.chunk = p.p_chunks + s;
-    kva_item<HDP, WIDE>(p, it, kva_smem);
+    kva_item<HDP, WIDE, false>(p, it, kva_smem);
 }
 
 template <uint32_t HDP, bool WIDE>
@@ -660,6 +697,84 @@ __global__ void __launch_bounds__(32, WIDE || HDP == 256u ? 8 : 11) kv_attention
     kva_cta<HDP, WIDE>(p, kva_smem);
     // not to end before the prefix's kernel has: the joining kernel waits for this one alone
     if (p.chained && blockIdx.x == 0u) pdl_wait();
+}
+
+// Small calls, where latency counts: one launch, no workspace.  A cluster has a row
+// tile of one sequence and one KV head; its up to 32 warps take the steps of prefix
+// and own rows in equal shares, and join their records through distributed shared
+// memory.  The prefix is read once for every tile here, from L2.
+constexpr uint32_t kKvaClusterWarps = 4;   // a CTA
+
+template <uint32_t HDP, bool WIDE>
+__global__ void __launch_bounds__(32 * kKvaClusterWarps) kv_attention_cluster_kernel(const __grid_constant__ KvAttnParams p) {
+    namespace cg = cooperative_groups;
+    using S = KvaShape<HDP, WIDE>;
+    extern __shared__ __align__(16) uint8_t kva_smem[];
+    const cg::cluster_group cl = cg::this_cluster();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, H = p.kv.kv_heads, hd = p.kv.hd;
+    const uint32_t ctas = cl.num_blocks(), rank = cl.block_rank(), W = ctas * kKvaClusterWarps, me = rank * kKvaClusterWarps + warp;
+    const uint32_t idx = blockIdx.x / ctas, tile_idx = idx / H;
+    KvaItem it;
+    it.sstride = H;
+    it.stride = static_cast<uint64_t>(H) * hd;
+    it.chunk = 0u;
+    it.h = idx - tile_idx * H;
+    uint32_t slot, len, n;
+    if (!own_item(p, tile_idx, S::kRows, it, &slot, &len, &n)) return;   // the whole cluster
+    const uint32_t pre = (p.prefix_len + S::kKeys - 1u) / S::kKeys, own = (len + S::kKeys - 1u) / S::kKeys;
+    const uint32_t s0 = (pre + own) * me / W, s1 = (pre + own) * (me + 1u) / W;   // steps of this warp
+    it.spans = 0u;
+    if (s0 < min(s1, pre)) {
+        it.a = prefix_keys(p, it.h);
+        it.a.key0 = s0 * S::kKeys;
+        it.a.key1 = min(p.prefix_len, min(s1, pre) * S::kKeys);
+        it.spans = 1u;
+    }
+    if (s1 > max(s0, pre)) {
+        KvaKeys k = slot_keys(p, it.h, slot, len, n);
+        k.key0 = (max(s0, pre) - pre) * S::kKeys;
+        k.key1 = min(len, (s1 - pre) * S::kKeys);
+        if (it.spans) it.b = k;
+        else it.a = k;
+        ++it.spans;
+    }
+    kva_item<HDP, WIDE, true>(p, it, kva_smem + warp * S::kSmem);
+    cl.sync();
+    const uint32_t ld = hd + 4u, nrows = min(S::kRows, it.rows - it.row0);
+    auto record = [&](uint32_t w, uint32_t r) {   // row r of warp w of the cluster
+        return reinterpret_cast<const float*>(cl.map_shared_rank(kva_smem, w / kKvaClusterWarps) +
+                                              (w % kKvaClusterWarps) * S::kSmem + S::kQBytes) + r * ld;
+    };
+    for (uint32_t r = rank + ctas * warp; r < nrows; r += W) {
+        const float2 ml = lane < W ? *reinterpret_cast<const float2*>(record(lane, r) + hd) : make_float2(-INFINITY, 0.0f);
+        float m = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        const float w = ml.x == -INFINITY ? 0.0f : ex2(__fsub_rn(ml.x, m));
+        const float l = warp_sum(__fmul_rn(w, ml.y));
+        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        const uint32_t row = it.row0 + r, i = row / p.group, head = it.h * p.group + (row - i * p.group);
+        const uint64_t out = static_cast<uint64_t>(it.t0 + static_cast<int32_t>(i)) * p.out_ld + static_cast<uint64_t>(head) * hd;
+#pragma unroll 1
+        for (uint32_t d0 = 0; d0 < hd; d0 += 128u) {
+            const uint32_t d = d0 + 4u * lane;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (uint32_t c = 0; c < W; ++c) {
+                const float f = __shfl_sync(0xFFFFFFFFu, w, c);
+                const float4 a = d < hd ? *reinterpret_cast<const float4*>(record(c, r) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f == 0.0f) continue;
+                y.x = fmaf(f, a.x, y.x);
+                y.y = fmaf(f, a.y, y.y);
+                y.z = fmaf(f, a.z, y.z);
+                y.w = fmaf(f, a.w, y.w);
+            }
+            if (d < hd)
+                store4_any(p.out, p.type, out + d,
+                           make_float4(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv), __fmul_rn(y.z, inv), __fmul_rn(y.w, inv)), p.wide);
+        }
+    }
+    cl.sync();   // no CTA leaves while another reads its records
 }
 
 // out = sum_c w_c o_c / sum_c w_c l_c with w_c = 2^(m_c - max m) over a row's chunks,

@@ -273,19 +273,91 @@ def test_drafted_runs_are_causal(cuda, dtype, heads, kv_heads, dim, prefix_len):
     assert qb.device_status() == qb.OK
 
 
-@pytest.mark.parametrize("seqs,heads,kv_heads,dim,prefix_len", [(33, 8, 1, 128, 1000), (40, 32, 4, 64, 2049),
-                                                                (70, 16, 2, 128, 4111), (17, 24, 3, 96, 700)])
-def test_many_sequences_behind_one_prefix(cuda, seqs, heads, kv_heads, dim, prefix_len):
-    """Enough rows for whole tiles of them, lengths that end inside tiles of keys."""
-    rng = _gen(seqs)
-    lens = [int(v) for v in rng.integers(0, 65, seqs)]
+def _big(cuda, dtype, seqs, heads, kv_heads, dim, prefix_len, own, run, seed):
+    """A batch with ragged lengths and runs, its arguments and its exact answer."""
+    rng = _gen(seed)
+    runs = [int(v) for v in rng.integers(1, run + 1, seqs)]
+    lens = [int(v) for v in rng.integers(0, own + 1, seqs)]
     slots = [int(v) for v in rng.permutation(seqs)]
-    cache, prefix = _filled(rng, seqs, 64, kv_heads, dim, cuda), _filled(rng, 1, prefix_len, kv_heads, dim, cuda)
-    q = _tensor(rng.standard_normal((seqs, heads, dim)) * 2, cuda)
-    got = qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_len=prefix_len)
-    check(got, *attention64(q, cache, slots, lens, [1] * seqs, prefix, 0, prefix_len))
-    again = qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_len=prefix_len)
-    assert got.cpu().numpy().tobytes() == again.cpu().numpy().tobytes()   # no order of arrival in the results
+    cache = _filled(rng, seqs, own, kv_heads, dim, cuda)
+    prefix = _filled(rng, 1, prefix_len, kv_heads, dim, cuda) if prefix_len else None
+    q = _tensor(rng.standard_normal((sum(runs), heads, dim)) * 2, cuda, dtype)
+    args = (q, cache, _i32(slots, cuda), _i32(lens, cuda), _cu(runs, cuda))
+    return args, dict(prefix=prefix, prefix_len=prefix_len), attention64(q, cache, slots, lens, runs, prefix, 0, prefix_len)
+
+
+# one launch: clusters; two: own rows (and a prefix, 16 rows at a time) and the join; three: the
+# prefix on tiles of 128 rows, own rows, the join
+@pytest.mark.parametrize("launches,dtype,seqs,heads,kv_heads,dim,prefix_len,own,run", [
+    (1, "float32", 33, 8, 1, 128, 500, 64, 1), (1, "bfloat16", 3, 16, 2, 64, 3000, 40, 2), (1, "float32", 9, 4, 4, 256, 0, 777, 3),
+    (1, "float16", 20, 6, 2, 96, 33, 90, 1),
+    (2, "float32", 200, 16, 2, 64, 0, 300, 1), (2, "float32", 80, 10, 5, 128, 0, 333, 2), (2, "bfloat16", 300, 4, 2, 32, 0, 65, 1),
+    (2, "float32", 200, 16, 2, 256, 700, 50, 1), (2, "float16", 2, 32, 8, 128, 9000, 40, 3),
+    (3, "float32", 70, 16, 2, 128, 4111, 64, 1), (3, "float32", 64, 32, 4, 64, 2049, 100, 1), (3, "float16", 100, 24, 3, 96, 700, 64, 1),
+    (3, "bfloat16", 90, 16, 4, 80, 1500, 130, 2), (3, "float32", 40, 28, 4, 112, 1023, 70, 3), (3, "bfloat16", 8, 64, 8, 128, 20000, 33, 1),
+    (3, "float16", 150, 8, 2, 16, 1900, 20, 1)])
+def test_every_plan(cuda, launches, dtype, seqs, heads, kv_heads, dim, prefix_len, own, run):
+    """Each way a call is carried out (told by its launches), at head sizes that fill no tile and
+    lengths that end inside one; the same call again gives the same bits."""
+    import torch
+
+    args, kw, (want, tol) = _big(cuda, dtype, seqs, heads, kv_heads, dim, prefix_len, own, run, seqs + dim)
+    before = qb.launch_count()
+    got = qb.kv_attention(*args, **kw)
+    assert qb.launch_count() - before == launches
+    check(got, want, tol, dtype)
+    again = qb.kv_attention(*args, **kw)
+    assert torch.equal(got, again)   # no order of arrival in the results
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_prefix_that_keeps_raising_the_maximum(cuda, dtype):
+    """Keys sorted by their scores, so that every tile of the prefix moves the rows' maxima (the
+    outputs so far are scaled), and sorted the other way; a negative and a zero scale."""
+    import torch
+
+    rng = _gen(21)
+    seqs, heads, kv_heads, dim, n = 70, 16, 2, 128, 2000
+    cache, prefix = _filled(rng, seqs, 16, kv_heads, dim, cuda), _filled(rng, 1, n, kv_heads, dim, cuda)
+    base = rng.standard_normal((1, 1, dim))
+    q = _tensor(base + 0.1 * rng.standard_normal((seqs, heads, dim)), cuda, dtype)
+    s = torch.einsum("d,nhd->nh", torch.from_numpy(base[0, 0]).to(cuda).float(), prefix.k[0].float() * prefix.k_scale[0].unsqueeze(-1))
+    slots, lens = list(range(seqs)), [int(v) for v in rng.integers(0, 17, seqs)]
+    for order in (False, True):
+        at = s[:, 0].argsort(descending=order)
+        for t in (prefix.k, prefix.k_scale, prefix.v, prefix.v_scale):
+            t[0] = t[0][at]
+        s = s[at]
+        for scale in (1.0, -0.5, 0.0):
+            got = qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_len=n, scale=scale)
+            check(got, *attention64(q, cache, slots, lens, [1] * seqs, prefix, 0, n, scale), dtype)
+    assert qb.device_status() == qb.OK
+
+
+def test_a_batch_whose_other_rows_are_wild(cuda):
+    """Queries of NaN, infinities and 1e30 in some sequences (a padded batch's leftovers) do not
+    reach the others' outputs, with the prefix on tiles of 128 rows; V scales over forty binary
+    orders keep the bound."""
+    import torch
+
+    rng = _gen(22)
+    seqs, heads, kv_heads, dim, n = 70, 16, 2, 128, 1500
+    cache, prefix = _filled(rng, seqs, 16, kv_heads, dim, cuda), _filled(rng, 1, n, kv_heads, dim, cuda)
+    prefix.v_scale.mul_(torch.exp2(torch.from_numpy(rng.integers(-20, 21, (1, n, kv_heads)).astype(np.float32)).to(cuda)))
+    q = _tensor(rng.standard_normal((seqs, heads, dim)), cuda)
+    slots, lens = list(range(seqs)), [9] * seqs
+    want, tol = attention64(q, cache, slots, lens, [1] * seqs, prefix, 0, n)
+    q[3] = float("nan")
+    q[17, 5] = float("inf")
+    q[40] = 1e30
+    slots[3] = -1
+    out = torch.full_like(q, 7.0)
+    qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_len=n, out=out)
+    assert (out[3] == 7.0).all()
+    keep = [i for i in range(seqs) if i not in (3, 17, 40)]
+    check(out[keep], want[keep], tol[keep])
+    assert qb.device_status() == qb.OK
 
 
 def test_extreme_magnitudes(cuda):
@@ -354,7 +426,25 @@ def test_padded_batch_and_bad_lengths(cuda):
             rows_of = [0, 3, 4]
             check(out[rows_of], want[rows_of], tol[rows_of])
             assert (out[[1, 2, 5]] == 7.0).all()
-    # one chunk a row: the output is written by the first kernel
+    # the same with the prefix on tiles, and with one chunk a row (the first kernel writes the output)
+    seqs = 160
+    wide, far = _filled(rng, seqs, 40, 2, 64, cuda), _filled(rng, 1, 900, 2, 64, cuda)
+    qq = _tensor(rng.standard_normal((seqs + 4, 8, 64)), cuda)
+    slots, lens = list(range(seqs)), [int(v) for v in rng.integers(0, 41, seqs)]
+    slots[5], slots[77], lens[100] = -1, seqs, 41
+    for pre, launches in ((900, 3), (0, 1)):
+        out = torch.full((seqs + 4, 8, 64), 7.0, device=cuda)
+        n0 = qb.launch_count()
+        qb.kv_attention(qq, wide, _i32(slots, cuda), _i32(lens, cuda), _i32(list(range(seqs + 1)), cuda),
+                        prefix=far if pre else None, prefix_len=pre, max_len=40, out=out)
+        assert qb.launch_count() - n0 == launches or not pre
+        assert qb.device_status() == qb.ERR_INVALID
+        left = [5, 77, 100] + list(range(seqs, seqs + 4))
+        keep = [i for i in range(seqs) if i not in left]
+        want, tol = attention64(qq[:seqs], wide, [s if i not in left else -1 for i, s in enumerate(slots)],
+                                [min(v, 40) for v in lens], [1] * seqs, far, 0, pre)
+        check(out[keep], want[keep], tol[keep])
+        assert (out[left] == 7.0).all()
     out = torch.full((2, 4, 64), 7.0, device=cuda)
     qb.kv_attention(q[:2], cache, _i32([1, -1], cuda), _i32([60, 60], cuda), max_len=64, out=out)
     want, tol = attention64(q[:2], cache, [1, -1], [60, 0], [1, 1])
@@ -498,9 +588,13 @@ def test_refusals_on_the_device(cuda):
     lib, d = qb.lib, cache.desc
     import ctypes as C
 
-    rc = lib.qraf_cuda_kv_attention(C.byref(d), C.byref(d), 0, 8, q.data_ptr(), q.data_ptr(), 0, 256, 256, 1, 4,
-                                    one.data_ptr(), one.data_ptr(), None, 1, 8, 1.0, None, 0, None)
-    assert rc == qb.ERR_INVALID and "workspace" in qb.last_error()
+    long, ints, many = qb.KvCache(1, 4096, 8, 64), _i32([0] * 64, cuda), torch.zeros(64, 64, 64, device=cuda)
+    size = C.c_uint64()
+    assert lib.qraf_cuda_kv_attention_workspace(C.byref(long.desc), 0, 64, 64, 64, 0, 4096, C.byref(size)) == qb.OK
+    for given, at in ((size.value - 1, many.data_ptr()), (size.value, many.data_ptr() + 4), (size.value, None)):
+        rc = lib.qraf_cuda_kv_attention(C.byref(long.desc), None, 0, 0, many.data_ptr(), many.data_ptr(), 0, 4096, 4096, 64, 64,
+                                        ints.data_ptr(), ints.data_ptr(), None, 64, 4096, 1.0, at, given, None)
+        assert rc == qb.ERR_INVALID and "workspace" in qb.last_error()
     with pytest.raises(ValueError, match="float64"):
         qb.kv_store(cache, torch.zeros(1, 2, 64, device=cuda).double(), torch.zeros(1, 2, 64, device=cuda).double(), one, one)
     with pytest.raises(ValueError, match="int32"):
