@@ -451,6 +451,30 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
 int qraf_cuda_kv_attention_workspace(const qraf_kv_t* kv, uint32_t prefix_len, uint32_t n, uint32_t heads, uint32_t count,
                                      int ragged, uint32_t max_len, uint64_t* bytes);
 
+/* ── the decoder's int8 cache, a shared prefix, steps over runs ──────────── */
+/* Layer `layer` of a decoder's int8 cache (QRAF_DECODER_KV_INT8) as a descriptor for
+ * the operators above, valid until qraf_cuda_decoder_close. */
+int qraf_cuda_decoder_kv(qraf_decoder_t d, uint32_t layer, qraf_kv_t* out);
+/* From now on every sequence's first `length` positions are those of slot `slot`
+ * (a prompt that steps have already put there), shared: qraf_cuda_decoder_step_runs
+ * reads them once for the whole batch, takes tokens at positions >= length, and
+ * keeps position p of a sequence in row p - length of its slot.  length 0: none.
+ * Needs the int8 cache; qraf_cuda_decoder_step knows nothing of it.  Not for use
+ * while a step runs; a captured step keeps what was set at its capture. */
+int qraf_cuda_decoder_share_prefix(qraf_decoder_t d, uint32_t slot, uint32_t length);
+/* One step over runs of tokens (prompts, drafts to be verified, single tokens; int8
+ * cache): run b puts tokens_dev[cu_dev[b]] .. at positions starts_dev[b], + 1, ... of
+ * slot slots_dev[b] (runs as above, of distinct slots; n tokens and `count` runs, each
+ * at most max_slots), stores their K and V, attends causally (each token sees the
+ * prefix, its slot's rows and its run's tokens up to itself) and leaves every token's
+ * logits in logits_dev[n][vocab].  Rows behind the last run are not cached, and what
+ * their logits hold is unspecified.  A run whose slot or positions are out of range
+ * raises the device status.  The first call of a shape allocates; make one before
+ * capturing. */
+int qraf_cuda_decoder_step_runs(qraf_decoder_t d, uint32_t n, const int32_t* tokens_dev, const int32_t* slots_dev,
+                                const int32_t* starts_dev, const int32_t* cu_dev, uint32_t count, float* logits_dev, int mode,
+                                void* stream);
+
 /* ── from logits to accepted tokens ─────────────────────────────────────── */
 /* probs[r] = softmax(logits[r] / temperature) for rows of `vocab` values, rows
  * logits_ld and probs_ld apart (the temperature step of Sampler::sample,

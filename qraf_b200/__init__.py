@@ -134,6 +134,9 @@ def _load() -> C.CDLL:
         "qraf_cuda_kv_attention": (i32, [KV, KV, u32, u32, vp, vp, u32, u64, u64, u32, u32, vp, vp, vp, u32, u32,
                                          C.c_float, vp, u64, vp]),
         "qraf_cuda_kv_attention_workspace": (i32, [KV, u32, u32, u32, u32, i32, u32, C.POINTER(u64)]),
+        "qraf_cuda_decoder_kv": (i32, [vp, u32, KV]),
+        "qraf_cuda_decoder_share_prefix": (i32, [vp, u32, u32]),
+        "qraf_cuda_decoder_step_runs": (i32, [vp, u32, vp, vp, vp, vp, u32, vp, i32, vp]),
         "qraf_cuda_token_probs": (i32, [vp, u64, vp, u64, u32, u32, C.c_float, vp]),
         "qraf_cuda_verify_drafts": (i32, [vp, u64, u64, vp, u64, u64, vp, vp, vp, vp, u32, u32, u32, vp, vp, vp]),
         "qraf_fill_normal": (None, [u32, C.c_float, C.c_float, f32p, u64]),
@@ -361,6 +364,36 @@ class Decoder:
                                                 C.c_void_p(positions.data_ptr()), C.c_void_p(slots.data_ptr()),
                                                 C.c_void_p(logits.data_ptr()), mode, _stream(stream)))
         return logits
+
+    def step_runs(self, tokens, slots, starts, cu=None, mode: int = MODE_AUTO, logits=None, stream=None):
+        """One step over runs of tokens, e.g. prompts or drafts to be verified
+        (qraf_cuda_decoder_step_runs; a decoder opened with kv_int8): tokens cu[b] .. cu[b + 1] go to
+        positions starts[b] .. of slot slots[b] (without cu, one token each); at most max_slots
+        tokens.  tokens, slots, starts, cu: contiguous CUDA int32 tensors.  Returns logits [n, vocab]."""
+        n, index = tokens.numel(), tokens.get_device()
+        if index < 0:
+            raise ValueError("tokens must be a CUDA tensor")
+        slots_p, starts_p, cu_p, count = _runs_of(slots, starts, cu, n, index, "starts")
+        tokens_p = _ints(tokens, index, "tokens")
+        if logits is None:
+            logits = _empty((n, self.vocab), _torch().float32, tokens, stream)
+        elif logits.dtype != _torch().float32 or logits.get_device() != index or tuple(logits.shape) != (n, self.vocab) or \
+                not logits.is_contiguous():
+            raise ValueError(f"logits must be a contiguous float32 tensor [{n}, {self.vocab}] on cuda:{index}")
+        check(_get_lib().qraf_cuda_decoder_step_runs(self._h, n, tokens_p, slots_p, starts_p, cu_p, count, logits.data_ptr(),
+                                                     mode, _stream_on(stream, index)))
+        return logits
+
+    def share_prefix(self, slot: int, length: int) -> None:
+        """Share the first `length` positions of `slot` among all sequences of the steps over runs
+        (qraf_cuda_decoder_share_prefix); 0: no longer."""
+        check(_get_lib().qraf_cuda_decoder_share_prefix(self._h, slot, length))
+
+    def layer_cache(self, layer: int) -> "KvCache":
+        """One layer of the int8 cache for kv_store, kv_load and kv_attention; it keeps the decoder."""
+        d = qraf_kv_t()
+        check(_get_lib().qraf_cuda_decoder_kv(self._h, layer, C.byref(d)))
+        return KvCache._of_desc(d, self)
 
     def kv_read(self, slot: int, layer: int, pos: int, kv_heads: int, head_dim: int):
         """One cache row: (k, v) float32 [kv_heads * head_dim], or with the int8 cache
@@ -680,9 +713,32 @@ class KvCache:
         d = qraf_kv_t()
         check(_get_lib().qraf_cuda_kv_wrap(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots,
                                            rows, apart.pop() if apart else rows, heads, dim, C.byref(d)))
-        self.desc, self.k, self.v, self.k_scale, self.v_scale = d, k, v, k_scale, v_scale
-        self.device, self._index, self._ref = k.device, k.device.index, C.byref(d)
-        self.slots, self.rows, self.kv_heads, self.head_dim = slots, rows, heads, dim
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._describe(d)
+
+    @classmethod
+    def _of_desc(cls, d: qraf_kv_t, keepalive) -> "KvCache":
+        """A cache in the library's memory: its tensors are views of that."""
+        torch = _torch()
+        self = cls.__new__(cls)
+        self._keep = keepalive
+        for name, typestr, size in (("k", "|i1", 1), ("v", "|i1", 1), ("k_scale", "<f4", 4), ("v_scale", "<f4", 4)):
+            shape = (d.slots, d.rows, d.kv_heads) + ((d.head_dim,) if size == 1 else ())
+            width = d.head_dim if size == 1 else 1   # elements of a (row, head)
+            strides = (d.slot_rows * d.kv_heads * width * size, d.kv_heads * width * size, width * size) + ((1,) if size == 1 else ())
+
+            class _Holder:
+                __cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (getattr(d, name), False), "version": 3,
+                                            "strides": strides}
+
+            setattr(self, name, torch.as_tensor(_Holder(), device=f"cuda:{d.device}"))
+        self._describe(d)
+        return self
+
+    def _describe(self, d: qraf_kv_t) -> None:
+        self.desc, self._ref = d, C.byref(d)
+        self.device, self._index = self.k.device, d.device
+        self.slots, self.rows, self.kv_heads, self.head_dim = d.slots, d.rows, d.kv_heads, d.head_dim
         self._workspace = {}
 
 

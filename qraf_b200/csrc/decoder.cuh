@@ -529,6 +529,85 @@ __global__ void __launch_bounds__(kAttnThreads) dec_attention_kernel(const AttnP
     }
 }
 
+// ── steps over runs of tokens (qraf_cuda_decoder_step_runs) ─────────────────────
+struct RopeStoreParams {
+    float* q;                // [n][heads * hd]: rotated in place
+    const float* k;          // [n][kv_dim], before RoPE
+    const float* v;
+    const float2* rope;      // [max_seq][hd / 2]
+    KvView kv;               // one layer of the int8 cache
+    KvRuns runs;             // firsts = position of each run's first token
+    uint32_t heads, max_seq, prefix_len, prefix_slot;
+};
+
+// Row of the slot that holds a run's position, and whether the run may be carried out:
+// behind a shared prefix a slot's rows begin where the prefix ends, and the prefix's own
+// slot takes no tokens.
+__device__ __forceinline__ bool run_row(int32_t slot, int32_t pos, uint32_t prefix_len, uint32_t prefix_slot, uint32_t slots,
+                                        uint32_t max_seq, uint32_t* row) {
+    const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < slots && pos >= static_cast<int32_t>(prefix_len) &&
+                    static_cast<uint32_t>(pos) < max_seq && !(prefix_len && static_cast<uint32_t>(slot) == prefix_slot);
+    *row = ok ? static_cast<uint32_t>(pos) - prefix_len : 0u;
+    return ok;
+}
+
+// Rows that each run's slot holds after the step (-1: the run is refused), for
+// kv_attention; raises the status for runs out of range.
+__global__ void __launch_bounds__(256) dec_run_lens_kernel(KvRuns runs, uint32_t prefix_len, uint32_t prefix_slot,
+                                                           uint32_t slots, uint32_t max_seq, int32_t* __restrict__ lens) {
+    const uint32_t b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b >= runs.count) return;
+    const int32_t n = runs.cu ? runs.cu[b + 1u] - runs.cu[b] : 1, slot = runs.slots[b], pos = runs.firsts[b];
+    uint32_t row;
+    const bool ok = run_row(slot, pos, prefix_len, prefix_slot, slots, max_seq, &row) && n >= 0 &&
+                    static_cast<uint32_t>(n) <= max_seq - static_cast<uint32_t>(pos);
+    if (!ok && slot != -1) raise_error(kErrBadLaunch);
+    lens[b] = ok ? static_cast<int32_t>(row) + n : -1;
+}
+
+// One token a CTA: q and k rotated, k and v quantised into the cache
+// (QuantizedKVCache::store, as dec_attention_kernel does for a step's single tokens).
+__global__ void __launch_bounds__(256) dec_rope_store_kernel(const RopeStoreParams a) {
+    const uint32_t t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = a.kv.hd, half = hd / 2u;
+    const int32_t b = find_run(a.runs, static_cast<int32_t>(t));
+    if (b < 0) return;
+    const int32_t first = run_begin(a.runs, b), pos = a.runs.firsts[b] + (static_cast<int32_t>(t) - first), slot = a.runs.slots[b];
+    uint32_t row;
+    if (a.runs.firsts[b] < 0 || !run_row(slot, pos, a.prefix_len, a.prefix_slot, a.kv.slots, a.max_seq, &row)) return;
+    const float2* cs = a.rope + static_cast<size_t>(pos) * half;
+    const uint32_t kv_heads = a.kv.kv_heads;
+    for (uint32_t u = warp; u < a.heads + 2u * kv_heads; u += 8u) {
+        if (u < a.heads) {
+            float2* q = reinterpret_cast<float2*>(a.q + (static_cast<size_t>(t) * a.heads + u) * hd);
+            for (uint32_t i = lane; i < half; i += 32u) q[i] = rope_pair(q[i].x, q[i].y, cs[i]);
+            continue;
+        }
+        const bool is_k = u < a.heads + kv_heads;
+        const uint32_t h = u - a.heads - (is_k ? 0u : kv_heads);
+        const float2* src = reinterpret_cast<const float2*>((is_k ? a.k : a.v) + (static_cast<size_t>(t) * kv_heads + h) * hd);
+        float2 x[kAttnMaxHeadDim / 64u];
+        float m = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < kAttnMaxHeadDim / 64u; ++j) {
+            const uint32_t i = lane + 32u * j;
+            x[j] = make_float2(0.0f, 0.0f);
+            if (i < half) x[j] = is_k ? rope_pair(src[i].x, src[i].y, cs[i]) : src[i];
+            m = fmaxf(fmaxf(m, fabsf(x[j].x)), fabsf(x[j].y));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        const float scale = __fdiv_rn(m, 127.0f), inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+        const uint64_t idx = (static_cast<uint64_t>(slot) * a.kv.slot_rows + row) * kv_heads + h;
+        char2* codes = reinterpret_cast<char2*>((is_k ? a.kv.k : a.kv.v) + idx * hd);
+#pragma unroll
+        for (uint32_t j = 0; j < kAttnMaxHeadDim / 64u; ++j) {
+            const uint32_t i = lane + 32u * j;
+            if (i < half) codes[i] = make_char2(kvq_code(x[j].x, inv), kvq_code(x[j].y, inv));
+        }
+        if (lane == 0u) (is_k ? a.kv.ks : a.kv.vs)[idx] = scale;
+    }
+}
+
 // logits[m][r] = dot(W[r], x[m]) for an F32 LM head (a tied embedding,
 // dispatch_matvec_opt at transformer.cpp:607-609): one warp per (row, vector),
 // lane stripes then a warp sum.
@@ -584,6 +663,12 @@ struct qraf_decoder {
     // the tensor-core route (TC, or AUTO from three slots): every projection one
     // launch pair with its fusions; needs Q/K/V and gate/up back to back in memory
     bool tc_route = false;
+    // steps over runs: a prefix that every sequence shares, the runs' lengths, kv_attention's workspace
+    uint32_t prefix_slot = 0, prefix_len = 0;
+    int32_t* lens = nullptr;             // [max_slots]
+    uint8_t* runs_ws = nullptr;
+    size_t runs_ws_bytes = 0;
+    std::vector<uint8_t*> runs_ws_old;   // captured steps may hold these
 };
 
 namespace {
@@ -609,6 +694,9 @@ int qraf_cuda_decoder_close(qraf_decoder_t d) {
     for (void* p : {static_cast<void*>(d->kq), static_cast<void*>(d->vq), static_cast<void*>(d->ksc),
                     static_cast<void*>(d->vsc)})
         if (p) cudaFree(p);
+    if (d->lens) cudaFree(d->lens);
+    if (d->runs_ws) cudaFree(d->runs_ws);
+    for (uint8_t* p : d->runs_ws_old) cudaFree(p);
     for (void* p : {static_cast<void*>(d->kc), static_cast<void*>(d->vc), static_cast<void*>(d->rope),
                     static_cast<void*>(d->part), static_cast<void*>(d->counter), static_cast<void*>(d->work)})
         if (p) cudaFree(p);
@@ -867,8 +955,8 @@ namespace {
 // and up; down: silu(gate) * up formed by the prep, the residual in the store;
 // the LM head: the final RMSNorm in the prep.  The arithmetic is that of the
 // separate passes (tests/test_gpu_decoder.py compares with the reference).
-int tc_step(qraf_decoder* d, uint32_t M, const DeviceInfo* dev, AttnParams ap, cudaLaunchConfig_t cfg,
-            float* logits_dev, cudaStream_t st) {
+template <typename Attention>
+int tc_step(qraf_decoder* d, uint32_t M, const DeviceInfo* dev, Attention&& attention, float* logits_dev, cudaStream_t st) {
     const uint32_t q_dim = d->heads * d->hd, kv_dim = d->kv_heads * d->hd;
     int rc = QRAF_OK;
     for (uint32_t l = 0; l < d->layers; ++l) {
@@ -886,8 +974,8 @@ int tc_step(qraf_decoder* d, uint32_t M, const DeviceInfo* dev, AttnParams ap, c
         for (int i = 0; i <= kMaxSeg; ++i) qkv.seg_row0[i] = row0[i];
         rc = matmul_tc(ly.qkv_all, d->x, nullptr, M, true, st, *dev, nullptr, 0, &qkv);
         if (rc) return rc;
-        ap.layer = l;
-        QRAF_CUDA_TRY(counted(cudaLaunchKernelEx(&cfg, d->attn_kernel, ap)));
+        rc = attention(l);
+        if (rc) return rc;
         TcFusion res;
         res.accumulate = true;
         rc = matmul_tc(ly.o, d->att, d->x, M, true, st, *dev, nullptr, 0, &res);
@@ -915,6 +1003,49 @@ int tc_step(qraf_decoder* d, uint32_t M, const DeviceInfo* dev, AttnParams ap, c
         return matmul_tc(d->lm_head, d->x, logits_dev, M, true, st, *dev, nullptr, 0, &head);
     }
     (rmsnorm_kernel<<<M, 256, 0, st>>>(d->x, d->out_norm, d->eps, d->hidden, d->xn, 0), count_launch());
+    QRAF_CUDA_TRY(cudaGetLastError());
+    const size_t warps = static_cast<size_t>(d->vocab) * M;
+    (dec_f32_matvec_kernel<<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, st>>>(
+         static_cast<const float*>(d->lm_head.data), d->xn, d->vocab, d->hidden, M, logits_dev),
+     count_launch());
+    QRAF_CUDA_TRY(cudaGetLastError());
+    return QRAF_OK;
+}
+
+// One step of M rows: the embedding, per layer the projections around attention(layer),
+// the LM head.
+template <typename Attention>
+int run_step(qraf_decoder* d, uint32_t M, const int32_t* tokens_dev, int base_mode, const DeviceInfo* dev, cudaStream_t st,
+             float* logits_dev, Attention&& attention) {
+    const int pmode = base_mode | QRAF_MODE_FLAG_OVERLAP;
+    int rc = QRAF_OK;
+    (dec_embed_kernel<<<M, 256, 0, st>>>(d->emb, tokens_dev, d->vocab, d->hidden, d->x), count_launch());
+    QRAF_CUDA_TRY(cudaGetLastError());
+    const bool tc = d->tc_route && M >= 2 &&
+                    (base_mode == QRAF_MODE_TC || (base_mode == QRAF_MODE_AUTO && M >= kAutoTcMinVectors));
+    if (tc) return tc_step(d, M, dev, attention, logits_dev, st);
+    for (uint32_t l = 0; l < d->layers; ++l) {
+        const DecLayer& ly = d->L[l];
+        float* qkv_out[3] = {d->q, d->k, d->v};
+        const float* biases[3] = {ly.bias[0], ly.bias[1], ly.bias[2]};
+        const bool any_bias = biases[0] || biases[1] || biases[2];
+        rc = multi_impl(ly.qkv, 3, d->x, ly.attn_norm, d->eps, any_bias ? biases : nullptr, qkv_out, M, pmode, st);
+        if (rc) return rc;
+        rc = attention(l);
+        if (rc) return rc;
+        rc = matvec_impl(&ly.o, d->att, d->x, M, pmode, st, true);
+        if (rc) return rc;
+        rc = swiglu_impl(&ly.gate, &ly.up, d->x, ly.ffn_norm, d->eps, d->h, M, pmode, st);
+        if (rc) return rc;
+        rc = matvec_impl(&ly.down, d->h, d->x, M, pmode, st, true);
+        if (rc) return rc;
+    }
+    if (!d->tied) {
+        float* outs[1] = {logits_dev};
+        return multi_impl(&d->lm_head, 1, d->x, d->out_norm, d->eps, nullptr, outs, M, pmode, st);
+    }
+    (rmsnorm_kernel<<<M, 256, 0, st>>>(d->x, d->out_norm, d->eps, d->hidden, d->xn, base_mode == QRAF_MODE_EXACT),
+     count_launch());
     QRAF_CUDA_TRY(cudaGetLastError());
     const size_t warps = static_cast<size_t>(d->vocab) * M;
     (dec_f32_matvec_kernel<<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, st>>>(
@@ -966,7 +1097,6 @@ int qraf_cuda_decoder_step(qraf_decoder_t d, uint32_t M, const int32_t* tokens_d
     if (base_mode != QRAF_MODE_EXACT && base_mode != QRAF_MODE_FAST && base_mode != QRAF_MODE_TC &&
         base_mode != QRAF_MODE_AUTO)
         return fail(QRAF_ERR_INVALID, "unknown mode %d", mode);
-    const int pmode = base_mode | QRAF_MODE_FLAG_OVERLAP;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     DeviceInfo* dev = nullptr;
     int cur = 0;
@@ -1010,40 +1140,121 @@ int qraf_cuda_decoder_step(qraf_decoder_t d, uint32_t M, const int32_t* tokens_d
     cfg.attrs = attr;
     cfg.numAttrs = 1;
 
-    (dec_embed_kernel<<<M, 256, 0, st>>>(d->emb, tokens_dev, d->vocab, d->hidden, d->x), count_launch());
-    QRAF_CUDA_TRY(cudaGetLastError());
-    const bool tc = d->tc_route && M >= 2 &&
-                    (base_mode == QRAF_MODE_TC || (base_mode == QRAF_MODE_AUTO && M >= kAutoTcMinVectors));
-    if (tc) return tc_step(d, M, dev, ap, cfg, logits_dev, st);
-    for (uint32_t l = 0; l < d->layers; ++l) {
-        const DecLayer& ly = d->L[l];
-        float* qkv_out[3] = {d->q, d->k, d->v};
-        const float* biases[3] = {ly.bias[0], ly.bias[1], ly.bias[2]};
-        const bool any_bias = biases[0] || biases[1] || biases[2];
-        rc = multi_impl(ly.qkv, 3, d->x, ly.attn_norm, d->eps, any_bias ? biases : nullptr, qkv_out, M, pmode, st);
-        if (rc) return rc;
+    return run_step(d, M, tokens_dev, base_mode, dev, st, logits_dev, [&](uint32_t l) -> int {
         ap.layer = l;
         QRAF_CUDA_TRY(counted(cudaLaunchKernelEx(&cfg, d->attn_kernel, ap)));
-        rc = matvec_impl(&ly.o, d->att, d->x, M, pmode, st, true);
-        if (rc) return rc;
-        rc = swiglu_impl(&ly.gate, &ly.up, d->x, ly.ffn_norm, d->eps, d->h, M, pmode, st);
-        if (rc) return rc;
-        rc = matvec_impl(&ly.down, d->h, d->x, M, pmode, st, true);
-        if (rc) return rc;
-    }
-    if (!d->tied) {
-        float* outs[1] = {logits_dev};
-        return multi_impl(&d->lm_head, 1, d->x, d->out_norm, d->eps, nullptr, outs, M, pmode, st);
-    }
-    (rmsnorm_kernel<<<M, 256, 0, st>>>(d->x, d->out_norm, d->eps, d->hidden, d->xn, base_mode == QRAF_MODE_EXACT),
-     count_launch());
-    QRAF_CUDA_TRY(cudaGetLastError());
-    const size_t warps = static_cast<size_t>(d->vocab) * M;
-    (dec_f32_matvec_kernel<<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, st>>>(
-         static_cast<const float*>(d->lm_head.data), d->xn, d->vocab, d->hidden, M, logits_dev),
-     count_launch());
-    QRAF_CUDA_TRY(cudaGetLastError());
+        return QRAF_OK;
+    });
+}
+
+int qraf_cuda_decoder_kv(qraf_decoder_t d, uint32_t layer, qraf_kv_t* out) {
+    if (!out) return fail(QRAF_ERR_INVALID, "out is NULL");
+    std::memset(out, 0, sizeof(*out));
+    if (!d) return fail(QRAF_ERR_INVALID, "decoder is NULL");
+    if (!d->kv8) return fail(QRAF_ERR_UNSUPPORTED, "the decoder's cache is not int8 (QRAF_DECODER_KV_INT8)");
+    if (layer >= d->layers) return fail(QRAF_ERR_INVALID, "layer %u out of range", layer);
+    const size_t row = static_cast<size_t>(layer) * d->max_seq * d->kv_heads;
+    out->k = d->kq + row * d->hd;
+    out->v = d->vq + row * d->hd;
+    out->k_scale = d->ksc + row;
+    out->v_scale = d->vsc + row;
+    out->slot_rows = static_cast<uint64_t>(d->layers) * d->max_seq;
+    out->slots = d->max_slots;
+    out->rows = d->max_seq;
+    out->kv_heads = d->kv_heads;
+    out->head_dim = d->hd;
+    out->device = d->device;
     return QRAF_OK;
+}
+
+int qraf_cuda_decoder_share_prefix(qraf_decoder_t d, uint32_t slot, uint32_t length) {
+    if (!d) return fail(QRAF_ERR_INVALID, "decoder is NULL");
+    if (!d->kv8) return fail(QRAF_ERR_UNSUPPORTED, "a shared prefix needs the int8 cache (QRAF_DECODER_KV_INT8)");
+    if (slot >= d->max_slots || length > d->max_seq)
+        return fail(QRAF_ERR_INVALID, "slot %u or length %u out of range", slot, length);
+    d->prefix_slot = slot;
+    d->prefix_len = length;
+    return QRAF_OK;
+}
+
+int qraf_cuda_decoder_step_runs(qraf_decoder_t d, uint32_t n, const int32_t* tokens_dev, const int32_t* slots_dev,
+                                const int32_t* starts_dev, const int32_t* cu_dev, uint32_t count, float* logits_dev, int mode,
+                                void* stream) {
+    if (!d) return fail(QRAF_ERR_INVALID, "decoder is NULL");
+    if (!d->kv8) return fail(QRAF_ERR_UNSUPPORTED, "steps over runs need the int8 cache (QRAF_DECODER_KV_INT8)");
+    if (n == 0 || count == 0) return QRAF_OK;
+    if (n > d->max_slots || count > d->max_slots)
+        return fail(QRAF_ERR_INVALID, "%u tokens in %u runs exceed max_slots = %u", n, count, d->max_slots);
+    if (!tokens_dev || !logits_dev) return fail(QRAF_ERR_INVALID, "a pointer is NULL");
+    int rc = check_runs(slots_dev, starts_dev, count, n, cu_dev);
+    if (rc) return rc;
+    const int base_mode = mode & 0xFF;
+    if (base_mode != QRAF_MODE_EXACT && base_mode != QRAF_MODE_FAST && base_mode != QRAF_MODE_TC &&
+        base_mode != QRAF_MODE_AUTO)
+        return fail(QRAF_ERR_INVALID, "unknown mode %d", mode);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    DeviceInfo* dev = nullptr;
+    int cur = 0;
+    rc = ensure_device(&cur, &dev);
+    if (rc) return rc;
+    if (cur != d->device)
+        return fail(QRAF_ERR_INVALID, "the decoder lives on device %d, the current device is %d", d->device, cur);
+    const uint32_t max_len = d->max_seq - d->prefix_len;
+    KvaPlan pl;
+    rc = plan_kva(n, d->heads, d->kv_heads, d->hd, d->prefix_len, count, cu_dev != nullptr, max_len, dev->sm_count, &pl);
+    if (rc) return rc;
+    if (!d->lens || d->runs_ws_bytes < pl.part_bytes) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        QRAF_CUDA_TRY(cudaStreamIsCapturing(st, &cs));
+        if (cs != cudaStreamCaptureStatusNone)
+            return fail(QRAF_ERR_UNSUPPORTED, "a step over runs needs %llu bytes of workspace (the decoder has %zu); make a first "
+                                              "call of this shape before capturing it",
+                        static_cast<unsigned long long>(pl.part_bytes), d->runs_ws_bytes);
+        if (!d->lens && cudaMalloc(&d->lens, d->max_slots * sizeof(int32_t)) != cudaSuccess) {
+            cudaGetLastError();
+            d->lens = nullptr;
+            return fail(QRAF_ERR_NOMEM, "the runs' lengths could not be allocated");
+        }
+        if (d->runs_ws_bytes < pl.part_bytes) {
+            const size_t want = std::max<size_t>(pl.part_bytes, 2 * d->runs_ws_bytes);
+            uint8_t* fresh = nullptr;
+            if (cudaMalloc(&fresh, want) != cudaSuccess) {
+                cudaGetLastError();
+                return fail(QRAF_ERR_NOMEM, "a step over runs: workspace of %zu bytes could not be allocated", want);
+            }
+            if (d->runs_ws) d->runs_ws_old.push_back(d->runs_ws);
+            d->runs_ws = fresh;
+            d->runs_ws_bytes = want;
+        }
+    }
+    const KvRuns runs = {slots_dev, starts_dev, cu_dev, count, n};
+    (dec_run_lens_kernel<<<(count + 255u) / 256u, 256, 0, st>>>(runs, d->prefix_len, d->prefix_slot, d->max_slots, d->max_seq,
+                                                               d->lens),
+     count_launch());
+    QRAF_CUDA_TRY(cudaGetLastError());
+    const float scale = 1.0f / std::sqrt(static_cast<float>(d->hd));   // attention.cpp:118, IEEE on the host as there
+    return run_step(d, n, tokens_dev, base_mode, dev, st, logits_dev, [&](uint32_t l) -> int {
+        qraf_kv_t kv;
+        int r = qraf_cuda_decoder_kv(d, l, &kv);
+        if (r) return r;
+        RopeStoreParams a{};
+        a.q = d->q;
+        a.k = d->k;
+        a.v = d->v;
+        a.rope = d->rope;
+        a.kv = view_of(kv);
+        a.runs = runs;
+        a.heads = d->heads;
+        a.max_seq = d->max_seq;
+        a.prefix_len = d->prefix_len;
+        a.prefix_slot = d->prefix_slot;
+        (dec_rope_store_kernel<<<n, 256, 0, st>>>(a), count_launch());
+        QRAF_CUDA_TRY(cudaGetLastError());
+        const uint64_t q_dim = static_cast<uint64_t>(d->heads) * d->hd;
+        return qraf_cuda_kv_attention(&kv, d->prefix_len ? &kv : nullptr, d->prefix_slot, d->prefix_len, d->q, d->att,
+                                      QRAF_TYPE_F32, q_dim, q_dim, n, d->heads, slots_dev, d->lens, cu_dev, count, max_len, scale,
+                                      d->runs_ws, d->runs_ws_bytes, st);
+    });
 }
 
 }  // extern "C"

@@ -191,39 +191,39 @@ def attention64(q, cache, slots, lens, runs, prefix=None, prefix_slot=0, prefix_
     vs weighs 2^6 at least where p = 1: the lower part's last bit is 2^-24, so beside its relative
     error each weight is off by up to 2^-25 2^-6 vs_max, times a code of at most 127, over a sum of
     weights of at least 1.  For bf16 a weight may be held in one part, off by 2^-12 of itself."""
-    one_part = 2.0 ** -12 if "bfloat16" in str(q.dtype) and prefix_len else 0.0
-    q = q.double().cpu().numpy()
+    import torch
+
+    one_part = 2.0 ** -12 if q.dtype == torch.bfloat16 and prefix_len else 0.0
+    q = q.double()
     n, heads, dim = q.shape
     group = heads // cache.kv_heads
     scale = dim ** -0.5 if scale is None else scale
-    out, tol = np.zeros(q.shape), np.zeros(q.shape)
-    val = {}
-    for name in "kv":
-        val[name] = getattr(cache, name).double().cpu().numpy() * getattr(cache, name + "_scale").double().cpu().numpy()[..., None]
-        if prefix_len:
-            val["p" + name] = (getattr(prefix, name)[prefix_slot, :prefix_len].double().cpu().numpy() *
-                               getattr(prefix, name + "_scale")[prefix_slot, :prefix_len].double().cpu().numpy()[..., None])
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+
+    def values(c, name, slot, rows):
+        return getattr(c, name)[slot, :rows].double() * getattr(c, name + "_scale")[slot, :rows].double().unsqueeze(-1)
+
+    if prefix_len:
+        far = values(prefix, "k", prefix_slot, prefix_len), values(prefix, "v", prefix_slot, prefix_len)
     t = 0
     for slot, length, m in zip(slots, lens, runs):
         for i in range(m):
-            if slot >= 0:
-                seen = max(0, length - m + 1 + i)
-                k, v = val["k"][slot, :seen], val["v"][slot, :seen]
+            seen = max(0, length - m + 1 + i)
+            if slot >= 0 and prefix_len + seen:
+                k, v = values(cache, "k", slot, seen), values(cache, "v", slot, seen)
                 if prefix_len:
-                    k, v = np.concatenate([val["pk"], k]), np.concatenate([val["pv"], v])
-                if len(k):
-                    k, v = np.repeat(k, group, 1), np.repeat(v, group, 1)
-                    s = np.einsum("hd,khd->hk", q[t], k) * scale
-                    a = (np.einsum("hd,khd->hk", np.abs(q[t]), np.abs(k)) * abs(scale)).max(1)
-                    p = np.exp(s - s.max(1, keepdims=True))
-                    p /= p.sum(1, keepdims=True)
-                    out[t] = np.einsum("hk,khd->hd", p, v)
-                    size = np.einsum("hk,khd->hd", p, np.abs(v))
-                    floor = len(k) * np.abs(v).max() * 2.0 ** -31   # max |v| is 127 vs_max
-                    ds = a * (2 * dim / 16 + 8) * 2.0 ** -23
-                    tol[t] = size * (2 * ds[:, None] + one_part + 2.0 ** -21 + (len(k) / 8 + 64) * 2.0 ** -23) + floor
+                    k, v = torch.cat([far[0], k]), torch.cat([far[1], v])
+                k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+                s = torch.einsum("hd,khd->hk", q[t], k) * scale
+                a = (torch.einsum("hd,khd->hk", q[t].abs(), k.abs()) * abs(scale)).amax(1)
+                p = torch.softmax(s, 1)
+                out[t] = torch.einsum("hk,khd->hd", p, v)
+                size = torch.einsum("hk,khd->hd", p, v.abs())
+                floor = len(k) * v.abs().max() * 2.0 ** -31   # max |v| is 127 vs_max
+                ds = a * (2 * dim / 16 + 8) * 2.0 ** -23
+                tol[t] = size * (2 * ds.unsqueeze(1) + one_part + 2.0 ** -21 + (len(k) / 8 + 64) * 2.0 ** -23) + floor
             t += 1
-    return out, tol
+    return out.cpu().numpy(), tol.cpu().numpy()
 
 
 def check(got, want, tol, dtype="float32"):
