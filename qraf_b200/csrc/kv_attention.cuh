@@ -74,6 +74,7 @@ struct KvAttnParams {
     uint32_t p_chunks, p_chunk;   // its chunks (pre_ctas: records of a row at most) and keys in one
     uint32_t pre_ctas;       // CTAs of kv_prefix_kernel, which has the prefix then; 0: kv_attention_kernel has it
     uint32_t pre_base, pre_extra;   // its ranges
+    uint32_t pre_term, pre_terms;   // tiles in one sum, and the records of a row that a CTA may leave: one per sum
     uint32_t chained;        // kv_attention_kernel was launched as kv_prefix_kernel's dependent
     uint32_t own_tiles, splits;              // own rows: row tiles over all runs (at most), chunks of each (at most)
     uint32_t own_wide;       // the kernel with tiles of 16 rows, else 8
@@ -801,12 +802,22 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const _
         live = b >= 0 && run_ok(p, static_cast<uint32_t>(b), &slot, &len);
         if (live && p.splits) own_chunk(len, p.splits, &own);
     }
-    uint32_t pre = p.p_chunks;
+    uint32_t pre = p.p_chunks, tile0 = 0, T = 0, c0 = 0;
     if (p.pre_ctas) {   // the CTAs whose ranges meet this row's unit
-        const uint32_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys, h = head / p.group;
-        const uint32_t unit = h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows;
-        pre = pre_owner(p.pre_base, p.pre_extra, unit * T + T - 1u) - pre_owner(p.pre_base, p.pre_extra, unit * T) + 1u;
+        T = (p.prefix_len + kPreKeys - 1u) / kPreKeys;
+        const uint32_t h = head / p.group;
+        tile0 = (h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows) * T;
+        c0 = pre_owner(p.pre_base, p.pre_extra, tile0);
+        pre = (pre_owner(p.pre_base, p.pre_extra, tile0 + T - 1u) - c0 + 1u) * p.pre_terms;
     }
+    // whether record i of the prefix was left: a CTA leaves one per pre_term tiles of its stretch
+    auto left = [&](uint32_t i) {
+        if (!p.pre_ctas || i >= pre) return true;
+        const uint32_t c = c0 + i / p.pre_terms;
+        const uint32_t a = max(tile0, pre_start(p.pre_base, p.pre_extra, c));
+        const uint32_t b = min(tile0 + T, pre_start(p.pre_base, p.pre_extra, c + 1u));
+        return i % p.pre_terms * p.pre_term < b - a;
+    };
     const uint32_t chunks = live ? pre + own : 0u;
     auto at = [&](uint32_t i) { return i < pre ? i : p.p_chunks + (i - pre); };   // record of chunk i
     const uint64_t ld = hd + 4u;
@@ -814,15 +825,16 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const _
     float* w = s_w[warp / WPR];
     pdl_wait();
     float m = -INFINITY;
-    for (uint32_t i = lane; i < chunks; i += 32u) m = fmaxf(m, __ldcg(rec + at(i) * ld + hd));
+    for (uint32_t i = lane; i < chunks; i += 32u)
+        if (left(i)) m = fmaxf(m, __ldcg(rec + at(i) * ld + hd));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     float l = 0.0f;
     for (uint32_t i = sub + WPR * lane; i < chunks; i += 32u * WPR) {
-        const float mi = __ldcg(rec + at(i) * ld + hd);
+        const float mi = left(i) ? __ldcg(rec + at(i) * ld + hd) : -INFINITY;
         const float wi = mi == -INFINITY ? 0.0f : ex2(__fsub_rn(mi, m));
         w[i] = wi;
-        l = fmaf(wi, __ldcg(rec + at(i) * ld + hd + 1u), l);
+        if (wi != 0.0f) l = fmaf(wi, __ldcg(rec + at(i) * ld + hd + 1u), l);
     }
     l = warp_sum(l);
     __syncwarp();

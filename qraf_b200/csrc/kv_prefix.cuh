@@ -51,6 +51,14 @@ constexpr uint32_t pre_q_parts() { return sizeof(Q) == 4u ? 2u : 1u; }
 template <typename Q>
 constexpr uint32_t pre_p_parts() { return std::is_same<Q, __nv_bfloat16>::value ? 1u : 2u; }
 
+// The tensor cores' fp32 accumulator truncates: every accumulation may lose a last bit, and
+// always toward zero.  So the lower parts' products go first (into small sums); O is
+// lengthened by what it loses on the average (measured on a B200: 1.0e-7 of itself a tile and
+// part, 8 accumulations; without this 16 tiles came out 3e-6 short); and O starts anew every
+// p.pre_term tiles (32 where that keeps a row's records below 256), its sum so far leaving as
+// a record.
+constexpr float kPreLoss = 1.0e-7f;
+
 template <uint32_t HDP, uint32_t QP>
 struct PreShape {
     static constexpr uint32_t kAtoms = HDP / 64u;                      // 64-element (128-byte) column blocks of Q and K
@@ -191,6 +199,25 @@ __device__ __forceinline__ float pre_weights(uint32_t s_col, const float* ks, co
     return __fadd_rn(sum.x, sum.y);
 }
 
+// The row's output so far, in numbers, to its record (with the maximum that it refers to and
+// no sum of weights: that is in the stretch's last record).
+template <uint32_t HDP>
+__device__ __forceinline__ void pre_flush_row(uint32_t o_col, float* rec, uint32_t hd, float unit, float m) {
+#pragma unroll 1
+    for (uint32_t c = 0; c < HDP; c += 32u) {
+        float v[32];
+        tmem_ld32(o_col + c, v);
+        tmem_wait_ld();
+        if (!rec) continue;
+#pragma unroll
+        for (uint32_t j = 0; j < 32u; j += 4u)
+            if (c + j < hd)
+                *reinterpret_cast<float4*>(rec + c + j) =
+                    make_float4(__fmul_rn(v[j], unit), __fmul_rn(v[j + 1u], unit), __fmul_rn(v[j + 2u], unit), __fmul_rn(v[j + 3u], unit));
+    }
+    if (rec) *reinterpret_cast<float2*>(rec + hd) = make_float2(m, 0.0f);
+}
+
 // The row's output so far times alpha.
 template <uint32_t HDP>
 __device__ __forceinline__ void pre_scale_row(uint32_t o_col, float alpha) {
@@ -276,6 +303,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         const uint32_t key0 = tile0 * kPreKeys, key1 = min(p.prefix_len, (tile0 + n) * kPreKeys);
         float m = -INFINITY, l = 0.0f;       // of a softmax thread: its sum, and the maximum that it refers to
         const uint32_t wg = warp >> 2;       // softmax warpgroup: tiles of this parity (of the stretch)
+        const uint32_t first_rec = (blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T)) * p.pre_terms;
+        auto record = [&](uint32_t r, uint32_t term) -> float* {   // of the tile's row r; nullptr past the last row
+            const uint32_t row = row0 + r, t = row / G, head = h * G + (row - t * G);
+            return row < rows ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + first_rec + term) * (hd + 4u)
+                              : nullptr;
+        };
+        auto unit_factor = [&](uint32_t tiles) {   // the sum of that many tiles to numbers
+            uint32_t most = 14u;
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
+            return __fmul_rn(pow2_bits(static_cast<int32_t>(most) - kPreUp + 1),
+                             fmaf(static_cast<float>(tiles * PP), kPreLoss, 1.0f));
+        };
 
         if (warp < kPreWarpXf) {
             // ── the query rows: 16 a warp, all of its loads in flight ──
@@ -341,13 +381,22 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     ok = warp_wait(&m_ready[4u * (px & 1u) + (warp & 3u)], px >> 1 & 1u);
                     if (!ok) break;
                     const float before = s_m[(px & 1u) * 128u + r];
-                    if (mt > __fadd_rn(before, kPreLag)) alpha = ex2(__fsub_rn(before, mt));
-                    else m_now = before;
+                    if (t % p.pre_term == 0u) {   // a term of the sum is full: O starts anew, with this tile's maximum
+                        ok = warp_wait(&pv_done[px & 1u], px >> 1 & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        pre_flush_row<HDP>(o_col, record(r, t / p.pre_term - 1u), hd, unit_factor(p.pre_term), before);
+                        tc_fence_before();
+                    } else if (mt > __fadd_rn(before, kPreLag)) {
+                        alpha = ex2(__fsub_rn(before, mt));
+                    } else {
+                        m_now = before;
+                    }
                 }
                 s_m[(x & 1u) * 128u + r] = m_now;
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&m_ready[4u * (x & 1u) + (warp & 3u)]);
-                if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // O has the tiles before this one, and no other yet
+                if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // O has the term's tiles before this one, and no other yet
                     ok = warp_wait(&pv_done[(x - 1u) & 1u], (x - 1u) >> 1 & 1u);
                     if (!ok) break;
                     tc_fence_after();
@@ -553,7 +602,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
 #pragma unroll 4
                         for (uint32_t k = 0; k < HDP / 16u; ++k)
                             tc_mma_f16(tmem + b * 128u,
-                                       tc_smem_desc(base + S::kQ + part * S::kQPart + (k >> 2) * (kPreRows * 128u) + (k & 3u) * 32u),
+                                       tc_smem_desc(base + S::kQ + (QP - 1u - part) * S::kQPart + (k >> 2) * (kPreRows * 128u) + (k & 3u) * 32u),
                                        tc_smem_desc(base + S::kK + (k >> 2) * (kPreKeys * 128u) + (k & 3u) * 32u),
                                        idesc_s, part + k > 0u);
                     tc_commit(&s_ready[b]);
@@ -572,9 +621,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     for (uint32_t part = 0; part < PP; ++part)
 #pragma unroll 4
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
-                            pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * part + 8u * (k & 1u),
+                            pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * (PP - 1u - part) + 8u * (k & 1u),
                                        tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
-                                       t + part + k > 0u);
+                                       t % p.pre_term + part + k > 0u);
                     tc_commit(&pv_done[sl]);
                 }
                 __syncwarp();
@@ -604,11 +653,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         }
         float* jo = reinterpret_cast<float*>(smem + S::kK);   // [128][HDP + 4]
         if (warp < kPreWarpXf) {   // each warpgroup has half of the columns
-            uint32_t most = 14u;
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
             const uint32_t r = (warp & 3u) * 32u + lane;
-            const float unit_f = pow2_bits(static_cast<int32_t>(most) - kPreUp + 1);
+            const float unit_f = unit_factor((n - 1u) % p.pre_term + 1u);
             const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 384u;
             float* dst = jo + r * S::kJoinLd;
 #pragma unroll 1
@@ -636,13 +682,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         }
         __syncthreads();
         if (warp < 4u) {   // one bulk copy a row
-            const uint32_t row = row0 + tid;
-            if (row < rows) {
-                const uint32_t chunk = blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T);
-                const uint32_t t = row / G, head = h * G + (row - t * G);
-                bulk_s2g(p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + chunk) * (hd + 4u),
-                         jo + tid * S::kJoinLd, hd + 4u);
-            }
+            if (float* rec = record(tid, (n - 1u) / p.pre_term)) bulk_s2g(rec, jo + tid * S::kJoinLd, hd + 4u);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // written: K and V tiles may come, the CTA may end
         }

@@ -295,7 +295,9 @@ def _big(cuda, dtype, seqs, heads, kv_heads, dim, prefix_len, own, run, seed):
     (2, "float32", 200, 16, 2, 256, 700, 50, 1), (2, "float16", 2, 32, 8, 128, 9000, 40, 3),
     (3, "float32", 70, 16, 2, 128, 4111, 64, 1), (3, "float32", 64, 32, 4, 64, 2049, 100, 1), (3, "float16", 100, 24, 3, 96, 700, 64, 1),
     (3, "bfloat16", 90, 16, 4, 80, 1500, 130, 2), (3, "float32", 40, 28, 4, 112, 1023, 70, 3), (3, "bfloat16", 8, 64, 8, 128, 20000, 33, 1),
-    (3, "float16", 150, 8, 2, 16, 1900, 20, 1)])
+    (3, "float16", 150, 8, 2, 16, 1900, 20, 1),
+    # one unit whose tiles are one or two for each CTA, and one with more tiles a CTA than one sum takes
+    (3, "float32", 8, 8, 1, 128, 36993, 30, 1), (3, "float32", 7, 8, 1, 16, 640001, 20, 1), (3, "bfloat16", 7, 8, 1, 32, 630000, 20, 1)])
 def test_every_plan(cuda, launches, dtype, seqs, heads, kv_heads, dim, prefix_len, own, run):
     """Each way a call is carried out (told by its launches), at head sizes that fill no tile and
     lengths that end inside one; the same call again gives the same bits."""
