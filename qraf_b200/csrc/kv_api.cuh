@@ -436,7 +436,7 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     const uint64_t out_rows = static_cast<uint64_t>(n) * heads;
     const bool few = pl.p_chunks + pl.splits <= kJoinFew;
     QRAF_CUDA_TRY(few ? launch_kv(kv_attention_join_kernel<1>, (out_rows + kJoinWarps - 1) / kJoinWarps, kJoinThreads, 0, true, p, st)
-                      : launch_kv(kv_attention_join_kernel<4>, out_rows, kJoinThreads, 0, true, p, st));
+                      : launch_kv(kv_attention_join_kernel<8>, out_rows, kJoinThreads, 0, true, p, st));
     return QRAF_OK;
 }
 

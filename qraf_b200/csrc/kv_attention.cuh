@@ -35,7 +35,7 @@
 namespace qraf_dev {
 
 constexpr uint32_t kKvaStages = 2;          // steps of codes that a warp has in shared memory
-constexpr uint32_t kJoinThreads = 128, kJoinWarps = kJoinThreads / 32u;
+constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32u;
 constexpr uint32_t kKvaMinChunk = 64;       // keys per chunk, at least: two steps
 constexpr uint32_t kKvaMaxHeadDim = 256;
 constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own rows together
@@ -780,16 +780,16 @@ __global__ void __launch_bounds__(32 * kKvaClusterWarps) kv_attention_cluster_ke
 
 // out = sum_c w_c o_c / sum_c w_c l_c with w_c = 2^(m_c - max m) over a row's chunks,
 // in chunk order.  WPR warps a row: one where a row has up to 16 chunks (then a CTA
-// joins four rows), else four, each with every fourth chunk.  The runs are looked up
-// before the dependency wait: nothing that they say is written by the kernels before.
+// joins eight rows), else eight, each with every eighth chunk; eight records are in
+// flight at a time.  The runs are looked up before the dependency wait: nothing that
+// they say is written by the kernels before.
 constexpr uint32_t kJoinFew = 16;
 
 template <uint32_t WPR>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const __grid_constant__ KvAttnParams p) {
-    constexpr uint32_t kMost = WPR == 1u ? kJoinFew : kKvaMaxChunks;
-    __shared__ float s_w[kJoinWarps / WPR][kMost];
+    constexpr uint32_t kMine = WPR == 1u ? 1u : kKvaMaxChunks / (32u * WPR);   // records a lane has the weights of
+    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
     __shared__ float s_o[WPR == 1u ? 1u : kJoinWarps][kKvaMaxHeadDim];
-    __shared__ float s_l[kJoinWarps];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = p.kv.hd;
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kJoinWarps / WPR) + warp / WPR;
     const uint32_t sub = warp % WPR;
@@ -822,38 +822,58 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const _
     auto at = [&](uint32_t i) { return i < pre ? i : p.p_chunks + (i - pre); };   // record of chunk i
     const uint64_t ld = hd + 4u;
     const float* rec = p.part + row * (p.p_chunks + p.splits) * ld;
-    float* w = s_w[warp / WPR];
+    // this warp's records are sub, sub + WPR, ...; lane i of it has the weights of its (i + 32 k)th
     pdl_wait();
+    float2 ml[kMine];
     float m = -INFINITY;
-    for (uint32_t i = lane; i < chunks; i += 32u)
-        if (left(i)) m = fmaxf(m, __ldcg(rec + at(i) * ld + hd));
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        const uint32_t i = sub + WPR * (lane + 32u * k);
+        ml[k] = i < chunks && left(i) ? __ldcg(reinterpret_cast<const float2*>(rec + at(i) * ld + hd)) : make_float2(-INFINITY, 0.0f);
+        m = fmaxf(m, ml[k].x);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    float l = 0.0f;
-    for (uint32_t i = sub + WPR * lane; i < chunks; i += 32u * WPR) {
-        const float mi = left(i) ? __ldcg(rec + at(i) * ld + hd) : -INFINITY;
-        const float wi = mi == -INFINITY ? 0.0f : ex2(__fsub_rn(mi, m));
-        w[i] = wi;
-        if (wi != 0.0f) l = fmaf(wi, __ldcg(rec + at(i) * ld + hd + 1u), l);
-    }
-    l = warp_sum(l);
-    __syncwarp();
-    float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-    for (uint32_t i = sub; i < chunks; i += WPR) {
-        const float wi = w[i];
+    if constexpr (WPR > 1u) {
+        if (lane == 0u) s_m[warp] = m;
+        __syncthreads();
 #pragma unroll
-        for (uint32_t j = 0; j < 2u; ++j) {
-            const uint32_t d = 4u * lane + 128u * j;
-            if (d >= hd) continue;
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(rec + at(i) * ld + d));
-            if (wi == 0.0f) continue;
-            y[j].x = fmaf(wi, a.x, y[j].x);
-            y[j].y = fmaf(wi, a.y, y[j].y);
-            y[j].z = fmaf(wi, a.z, y[j].z);
-            y[j].w = fmaf(wi, a.w, y[j].w);
+        for (uint32_t k = 0; k < kJoinWarps; ++k) m = fmaxf(m, s_m[k]);
+    }
+    float l = 0.0f;
+    float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        const float w = ml[k].x == -INFINITY ? 0.0f : ex2(__fsub_rn(ml[k].x, m));
+        l = fmaf(w, ml[k].y, l);
+        const uint32_t i0 = sub + WPR * 32u * k;
+        const uint32_t n = i0 < chunks ? min(32u, (chunks - i0 + WPR - 1u) / WPR) : 0u;   // of this warp's, in this round
+#pragma unroll 1
+        for (uint32_t j0 = 0; j0 < n; j0 += 8u) {
+#pragma unroll
+            for (uint32_t half = 0; half < 2u; ++half) {
+                const uint32_t d = 4u * lane + 128u * half;
+                if (128u * half >= hd) break;
+                float4 a[8];
+                float f[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    f[j] = __shfl_sync(0xFFFFFFFFu, w, j0 + j);
+                    a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (j0 + j < n && f[j] != 0.0f && d < hd)
+                        a[j] = __ldcg(reinterpret_cast<const float4*>(rec + at(i0 + WPR * (j0 + j)) * ld + d));
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    y[half].x = fmaf(f[j], a[j].x, y[half].x);
+                    y[half].y = fmaf(f[j], a[j].y, y[half].y);
+                    y[half].z = fmaf(f[j], a[j].z, y[half].z);
+                    y[half].w = fmaf(f[j], a[j].w, y[half].w);
+                }
+            }
         }
     }
+    l = warp_sum(l);
     if constexpr (WPR > 1u) {
 #pragma unroll
         for (uint32_t j = 0; j < 2u; ++j) {
