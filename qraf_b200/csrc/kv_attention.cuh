@@ -641,9 +641,9 @@ __device__ __forceinline__ KvaKeys slot_keys(const KvAttnParams& p, uint32_t h, 
 }
 
 // Own-row tile `idx` of R rows into the item; false where there is none, or its run
-// is padding or out of range.
+// is padding or out of range.  *seen: rows of the slot that the tile's last token sees.
 __device__ __forceinline__ bool own_item(const KvAttnParams& p, uint32_t idx, uint32_t R, KvaItem& it, uint32_t* slot,
-                                         uint32_t* len, uint32_t* n) {
+                                         uint32_t* len, uint32_t* n, uint32_t* seen) {
     uint32_t b, tile;
     if (!find_tile(p, idx, R, &b, &tile) || !run_ok(p, b, slot, len)) return false;
     const int32_t t0 = max(run_begin(p.runs, b), 0);
@@ -652,6 +652,8 @@ __device__ __forceinline__ bool own_item(const KvAttnParams& p, uint32_t idx, ui
     it.row0 = tile * R;
     it.rows = *n * p.group;
     it.t0 = t0;
+    const int32_t last = static_cast<int32_t>((min(it.rows, it.row0 + R) - 1u) / p.group);
+    *seen = min(*len, static_cast<uint32_t>(max(static_cast<int32_t>(*len) - static_cast<int32_t>(*n) + 1 + last, 0)));
     return true;
 }
 
@@ -679,13 +681,13 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
         idx -= p_items;
         const uint32_t q = idx / p.splits, s = idx - q * p.splits, tile_idx = q / H;
         it.h = q - tile_idx * H;
-        uint32_t slot, len, n, count;
-        if (!own_item(p, tile_idx, WIDE ? 16u : 8u, it, &slot, &len, &n)) return;
+        uint32_t slot, len, n, seen, count;
+        if (!own_item(p, tile_idx, WIDE ? 16u : 8u, it, &slot, &len, &n, &seen)) return;
         const uint32_t chunk = own_chunk(len, p.splits, &count);
         if (s >= max(count, p.part ? 0u : 1u)) return;   // with one chunk a row, an empty slot's rows still get their zeros
         it.a = slot_keys(p, it.h, slot, len, n);
         it.a.key0 = s * chunk;
-        it.a.key1 = min(len, it.a.key0 + chunk);
+        it.a.key1 = min(seen, it.a.key0 + chunk);   // not past key0: a record of nothing
         it.chunk = p.p_chunks + s;
     }
     kva_item<HDP, WIDE, false>(p, it, kva_smem);
@@ -720,9 +722,9 @@ __global__ void __launch_bounds__(32 * kKvaClusterWarps) kv_attention_cluster_ke
     it.stride = static_cast<uint64_t>(H) * hd;
     it.chunk = 0u;
     it.h = idx - tile_idx * H;
-    uint32_t slot, len, n;
-    if (!own_item(p, tile_idx, S::kRows, it, &slot, &len, &n)) return;   // the whole cluster
-    const uint32_t pre = (p.prefix_len + S::kKeys - 1u) / S::kKeys, own = (len + S::kKeys - 1u) / S::kKeys;
+    uint32_t slot, len, n, seen;
+    if (!own_item(p, tile_idx, S::kRows, it, &slot, &len, &n, &seen)) return;   // the whole cluster
+    const uint32_t pre = (p.prefix_len + S::kKeys - 1u) / S::kKeys, own = (seen + S::kKeys - 1u) / S::kKeys;
     const uint32_t s0 = (pre + own) * me / W, s1 = (pre + own) * (me + 1u) / W;   // steps of this warp
     it.spans = 0u;
     if (s0 < min(s1, pre)) {
@@ -734,7 +736,7 @@ __global__ void __launch_bounds__(32 * kKvaClusterWarps) kv_attention_cluster_ke
     if (s1 > max(s0, pre)) {
         KvaKeys k = slot_keys(p, it.h, slot, len, n);
         k.key0 = (max(s0, pre) - pre) * S::kKeys;
-        k.key1 = min(len, (s1 - pre) * S::kKeys);
+        k.key1 = min(seen, (s1 - pre) * S::kKeys);
         if (it.spans) it.b = k;
         else it.a = k;
         ++it.spans;

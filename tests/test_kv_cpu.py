@@ -56,16 +56,17 @@ def test_attention_refuses():
     kv = _kv()
 
     def call(kv=kv, prefix=None, prefix_slot=0, prefix_len=0, q=A, out=A, type=0, q_ld=256, out_ld=256, n=2, heads=4, slots=A,
-             lens=A, cu=None, count=2, max_len=64):
+             lens=A, cu=None, count=2, max_len=64, scale=1.0):
         return qb.lib.qraf_cuda_kv_attention(C.byref(kv) if kv is not None else None, prefix, prefix_slot, prefix_len, q, out,
-                                             type, q_ld, out_ld, n, heads, slots, lens, cu, count, max_len, 1.0, None, 0, None)
+                                             type, q_ld, out_ld, n, heads, slots, lens, cu, count, max_len, scale, None, 0, None)
 
     assert call(type=9) == qb.ERR_UNSUPPORTED
     assert call(prefix_len=1 << 31) == qb.ERR_UNSUPPORTED
     assert call(n=0) == qb.OK
     for kw, text in (({"kv": None}, "NULL"), ({"heads": 0}, "multiple"), ({"heads": 3}, "multiple"), ({"max_len": 65}, "max_len"),
                      ({"q": None}, "NULL"), ({"out": A + 1}, "aligned"), ({"q_ld": 255}, "stride"), ({"out_ld": 8}, "stride"),
-                     ({"count": 1}, "without cu"), ({"lens": None}, "NULL")):
+                     ({"count": 1}, "without cu"), ({"lens": None}, "NULL"),
+                     ({"scale": float("nan")}, "finite"), ({"scale": float("inf")}, "finite")):
         assert call(**kw) == qb.ERR_INVALID, kw
         assert text in qb.last_error(), kw
 
