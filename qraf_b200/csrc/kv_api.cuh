@@ -358,7 +358,8 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     rc = check_runs(slots_dev, lens_dev, count, n, cu_dev);
     if (rc) return rc;
     if (!q_dev || !out_dev) return fail(QRAF_ERR_INVALID, "q or out is NULL");
-    if (!std::isfinite(scale)) return fail(QRAF_ERR_INVALID, "scale %g is not finite", static_cast<double>(scale));
+    if (!std::isfinite(scale * 1.44269504088896340736f))
+        return fail(QRAF_ERR_INVALID, "scale %g is not finite in units of log2(e)", static_cast<double>(scale));
     if (!element_aligned(q_dev, type) || !element_aligned(out_dev, type))
         return fail(QRAF_ERR_INVALID, "q or out is not aligned to its element type");
     const uint64_t row = static_cast<uint64_t>(heads) * kv->head_dim;
