@@ -694,7 +694,7 @@ __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem
 }
 
 template <uint32_t HDP, bool WIDE>
-__global__ void __launch_bounds__(32, WIDE || HDP == 256u ? 8 : 11) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
+__global__ void __launch_bounds__(32, 8) kv_attention_kernel(const __grid_constant__ KvAttnParams p) {
     extern __shared__ __align__(16) uint8_t kva_smem[];
     pdl_launch_dependents();
     kva_cta<HDP, WIDE>(p, kva_smem);
