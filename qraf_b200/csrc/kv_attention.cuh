@@ -658,6 +658,12 @@ __device__ __forceinline__ bool own_item(const KvAttnParams& p, uint32_t idx, ui
 }
 
 // WIDE: prefix items and own rows in tiles of 16 rows, else own rows in tiles of 8.
+//
+// Measured on a B200 (64 sequences, 8 KV heads of 128, 8 query heads each, with the joining
+// kernel): up to 1024 rows a sequence 36.8 us, up to 4096 101 us, 3.7 TB/s of codes and
+// scales.  The loads alone take 76 us there: what bounds it is issuing some 900 instructions
+// a step of 32 keys, most of them turning codes into fp16 fragments.  Registers for eight
+// CTAs an SM at least: for eleven it took 112.
 template <uint32_t HDP, bool WIDE>
 __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem) {
     const uint32_t H = p.kv.kv_heads;
@@ -705,7 +711,8 @@ __global__ void __launch_bounds__(32, 8) kv_attention_kernel(const __grid_consta
 // Small calls, where latency counts: one launch, no workspace.  A cluster has a row
 // tile of one sequence and one KV head; its up to 32 warps take the steps of prefix
 // and own rows in equal shares, and join their records through distributed shared
-// memory.  The prefix is read once for every tile here, from L2.
+// memory.  The prefix is read once for every tile here, from L2.  Bound by latency: 9 us
+// on a B200 for 4 sequences of 16 / 2 heads behind 777 rows, 24 with the kernels below.
 constexpr uint32_t kKvaClusterWarps = 4;   // a CTA
 
 template <uint32_t HDP, bool WIDE>
@@ -784,7 +791,8 @@ __global__ void __launch_bounds__(32 * kKvaClusterWarps) kv_attention_cluster_ke
 // in chunk order.  WPR warps a row: one where a row has up to 16 chunks (then a CTA
 // joins eight rows), else eight, each with every eighth chunk; eight records are in
 // flight at a time.  The runs are looked up before the dependency wait: nothing that
-// they say is written by the kernels before.
+// they say is written by the kernels before.  Bound by latency and by reading the
+// records, from L2: with this order, 8 sequences behind 65536 rows went from 48 to 42 us.
 constexpr uint32_t kJoinFew = 16;
 
 template <uint32_t WPR>
