@@ -383,7 +383,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     ok = warp_wait(&m_ready[4u * (px & 1u) + (warp & 3u)], px >> 1 & 1u);
                     if (!ok) break;
                     const float before = s_m[(px & 1u) * 128u + r];
-                    if (t % p.pre_term == 0u) {   // a term of the sum is full: O starts anew, with this tile's maximum
+                    // never a lower one: the sum of weights runs on over the stretch's terms, and one
+                    // scaled up by 2^128 would overflow
+                    if (t % p.pre_term == 0u) {   // a term of O's sum is full: it starts anew
+                        m_now = fmaxf(before, mt);
                         ok = warp_wait(&pv_done[px & 1u], px >> 1 & 1u);
                         if (!ok) break;
                         tc_fence_after();

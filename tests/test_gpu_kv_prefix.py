@@ -1,0 +1,86 @@
+"""kv_attention's prefix tiles where a CTA has many of them: sums that start anew, widely spread and
+peaked scores, against 64-bit forms."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import qraf_b200 as qb
+from test_gpu_kv import DTYPES, _filled, _gen, _i32, _tensor, check, quantise
+
+pytestmark = pytest.mark.gpu
+
+# 160 tokens of 16 query heads a KV head are 20 tiles of 128 rows, and with 7 KV heads 140 (tile, head)
+# units: one CTA has a whole unit, so every key of the prefix
+SEQS, KV_HEADS, GROUP, DIM = 160, 7, 16, 64
+
+
+def prefix64(q, prefix, n, scale):
+    """(out, tolerance) of the prefix alone, in 64 bits: attention64's bound, but the weighted sum is
+    formed 16 keys and one of two parts at a time (n / 8 accumulations, each off by at most a last bit)
+    and joined from at most 64 records, whatever the type."""
+    import torch
+
+    q64 = q.double().view(q.shape[0], KV_HEADS, GROUP, DIM)
+    k, v = (getattr(prefix, s)[0, :n].double() * getattr(prefix, s + "_scale")[0, :n].double().unsqueeze(-1) for s in "kv")
+    out, tol = torch.empty_like(q64), torch.empty_like(q64)
+    for h in range(KV_HEADS):
+        s = torch.einsum("tgd,kd->tgk", q64[:, h], k[:, h]) * scale
+        a = (torch.einsum("tgd,kd->tgk", q64[:, h].abs(), k[:, h].abs()) * abs(scale)).amax(-1, keepdim=True)
+        p = torch.softmax(s, -1)
+        out[:, h] = p @ v[:, h]
+        ds = a * (2 * DIM / 16 + 8) * 2.0 ** -23
+        floor = n * v[:, h].abs().max() * 2.0 ** -31
+        tol[:, h] = (p @ v[:, h].abs()) * (2 * ds + 2.0 ** -21 + (n / 8 + 64) * 2.0 ** -23) + floor
+    return out.view(q.shape).cpu().numpy(), tol.view(q.shape).cpu().numpy()
+
+
+def _attend(q, prefix, n, cuda, **kw):
+    """The call with own slots of no rows; the prefix is on tiles: three launches."""
+    cache = qb.KvCache(1, 16, KV_HEADS, DIM)
+    slots = _i32([0] * len(q), cuda)
+    before = qb.launch_count()
+    got = qb.kv_attention(q, cache, slots, slots * 0, prefix=prefix, prefix_len=n, **kw)
+    assert qb.launch_count() - before == 3
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [5120, 8970])
+def test_sorted_scores_over_many_sums(cuda, dtype, n):
+    """Keys sorted by their scores, falling (each new sum starts far below the maximum so far) and
+    rising, over 40 and 71 tiles: the falls reach several hundred binary orders."""
+    import torch
+
+    rng = _gen(n)
+    prefix = _filled(rng, 1, n, KV_HEADS, DIM, cuda)
+    base = rng.standard_normal(DIM)
+    q = _tensor(base + 0.1 * rng.standard_normal((SEQS, KV_HEADS * GROUP, DIM)), cuda, dtype)
+    for falling in (True, False):
+        s = torch.einsum("d,nhd->nh", torch.from_numpy(base).to(cuda).float(), prefix.k[0].float() * prefix.k_scale[0].unsqueeze(-1))
+        for h in range(KV_HEADS):
+            at = s[:, h].argsort(descending=falling)
+            for t in (prefix.k, prefix.k_scale, prefix.v, prefix.v_scale):
+                t[0, :, h] = t[0, at, h]
+        for scale in (1.0, 2.0, 4.0):
+            check(_attend(q, prefix, n, cuda, scale=scale), *prefix64(q, prefix, n, scale), dtype)
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [90, 120, 125, 126, 127, 128, 130, 300])
+@pytest.mark.parametrize("place", [5, 5000])
+def test_one_key_far_above_the_others(cuda, dtype, gap, place):
+    """A key in the first or the last tile that scores `gap` binary orders above the level of the
+    others: every row is that key's value."""
+    import torch
+
+    n, rng = 5120, _gen(gap)
+    prefix = _filled(rng, 1, n, KV_HEADS, DIM, cuda)
+    base = np.sign(rng.standard_normal(DIM))
+    q = _tensor(base * (1 + 0.01 * rng.random((SEQS, KV_HEADS * GROUP, 1))), cuda, dtype)
+    prefix.k_scale.mul_(0.01)
+    prefix.k[0, place] = torch.from_numpy((127 * base).astype(np.int8)).to(cuda)
+    prefix.k_scale[0, place] = gap * np.log(2.0) / (127 * DIM)
+    check(_attend(q, prefix, n, cuda, scale=1.0), *prefix64(q, prefix, n, 1.0), dtype)
+    assert qb.device_status() == qb.OK

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import qraf_b200 as qb
@@ -90,3 +91,58 @@ def test_sampling_refuses():
     for kw in ({"target": None}, {"draft": None}, {"tokens": None}, {"u": None}, {"last": None}, {"out": None}, {"acc": None},
                {"vocab": 0}, {"t_row": 15}, {"d_row": 15}, {"t_seq": 15}, {"d_seq": 15}, {"target": A + 2}):
         assert verify(**kw) == qb.ERR_INVALID, kw
+
+
+def _prefix_stretch(scores, term, restart, lag=8.0):
+    """A row's way through one stretch of kv_prefix_kernel in fp32: (maximum, sum) that its records are
+    joined with.  scores: (maximum, sum of weights relative to it) of each tile, binary; restart: the
+    maximum referred to from a new sum on, of the one before and the tile's."""
+    f32 = np.float32
+
+    def ex2(x):   # 2^x, flushed to zero below the normal range as on the device
+        with np.errstate(over="ignore"):
+            y = np.exp2(f32(x), dtype=np.float32)
+        return y if y >= np.finfo(f32).tiny else f32(0)
+
+    m = [f32(-np.inf)] * 2   # of the two warpgroups, which take the tiles in turn
+    total = [f32(0)] * 2
+    before, records = None, []
+    for t, (mt, weight) in enumerate(scores):
+        mt = f32(mt)
+        if t == 0:
+            now = mt
+        elif t % term == 0:
+            records.append((before, f32(0)))   # what was summed leaves; its weights stay in the sum
+            now = f32(restart(before, mt))
+        else:
+            now = mt if mt > before + f32(lag) else before
+        g = t & 1
+        if now != m[g]:
+            with np.errstate(over="ignore", invalid="ignore"):
+                total[g] = f32(0) if m[g] == -np.inf else total[g] * ex2(m[g] - now)
+        m[g] = before = now
+        total[g] = total[g] + f32(weight) * ex2(mt - now)
+    end = f32(0)
+    with np.errstate(over="ignore", invalid="ignore"):
+        for g in range(2):
+            if m[g] > -np.inf:
+                end = end + total[g] * ex2(m[g] - before)
+        records.append((before, end))
+        top = max(r[0] for r in records)
+        return top, sum(ex2(r[0] - top) * r[1] for r in records)
+
+
+@pytest.mark.parametrize("gap", [0, 90, 120, 126, 127, 128, 130, 300, 2000])
+@pytest.mark.parametrize("tiles,term", [(40, 32), (40, 8), (71, 32), (9, 8)])
+def test_a_sum_that_starts_anew_keeps_its_weights(gap, tiles, term):
+    """A first tile `gap` binary orders above all later ones: the joined sum of weights is its own (and
+    the others', where they are not too small), relative to its maximum.  With a maximum that falls to a
+    tile's own the sum is zero or not a number once 2^-gap is below the normal range."""
+    scores = [(gap, 1.0)] + [(0.0, 1.0)] * (tiles - 1)
+    want = 1.0 + (tiles - 1) * 2.0 ** -gap
+    top, total = _prefix_stretch(scores, term, max)
+    assert top == gap and abs(total - want) < 1e-5 * want
+    top, total = _prefix_stretch(scores[::-1], term, max)
+    assert top == gap and abs(total - want) < 1e-5 * want
+    _, wrong = _prefix_stretch(scores, term, lambda before, mt: mt)
+    assert (gap <= 126) == (abs(wrong - want) < 1e-4 * want)
