@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 const uint32_t valid = key1 - (key0 + t * kPreKeys);
                 const float ymax = valid >= kPreKeys ? pre_max<false>(s_col, ks, kPreKeys) : pre_max<true>(s_col, ks, valid);
                 const float mt = __fmul_rn(ymax, rf);
-                // the maximum that the row refers to from this tile on
-                float m_now = mt > -INFINITY ? mt : 0.0f, alpha = 1.0f;
+                // the maximum that the row refers to from this tile on (-inf while every score was)
+                float m_now = mt > -INFINITY ? mt : -INFINITY, alpha = 1.0f;
                 if (t > 0u) {
                     const uint32_t px = x - 1u;
                     ok = warp_wait(&m_ready[4u * (px & 1u) + (warp & 3u)], px >> 1 & 1u);
@@ -407,10 +407,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                     tc_fence_after();
                     pre_scale_row<HDP>(o_col, alpha);
                 }
-                if (m_now != m) l = m == -INFINITY ? 0.0f : __fmul_rn(l, ex2(__fsub_rn(m, m_now)));
+                if (m_now != m) l = __fmul_rn(l, ex2(__fsub_rn(m, m_now)));
                 m = m_now;
-                l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<PP, false>(s_col, ks, ks + 128, kPreKeys, rf, m)
-                                                   : pre_weights<PP, true>(s_col, ks, ks + 128, valid, rf, m));
+                const float m_use = m > -INFINITY ? m : 0.0f;   // nothing seen yet: every weight 2^-inf = 0
+                l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<PP, false>(s_col, ks, ks + 128, kPreKeys, rf, m_use)
+                                                   : pre_weights<PP, true>(s_col, ks, ks + 128, valid, rf, m_use));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&p_ready[b]);
@@ -677,9 +678,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 const float m_end = s_m[((x0 - 1u) & 1u) * 128u + r];
                 float sum = 0.0f;
 #pragma unroll
-                for (uint32_t i = 0; i < 2u; ++i)
-                    if (s_ml[i * 256u + r] > -INFINITY)
-                        sum = fmaf(s_ml[i * 256u + 128u + r], ex2(__fsub_rn(s_ml[i * 256u + r], m_end)), sum);
+                for (uint32_t i = 0; i < 2u; ++i) {
+                    const float mi = s_ml[i * 256u + r];
+                    sum = fmaf(s_ml[i * 256u + 128u + r], mi == m_end ? 1.0f : ex2(__fsub_rn(mi, m_end)), sum);
+                }
                 *reinterpret_cast<float4*>(dst + hd) = make_float4(m_end, sum, 0.0f, 0.0f);
             }
             tc_fence_before();

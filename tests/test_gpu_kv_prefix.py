@@ -84,3 +84,25 @@ def test_one_key_far_above_the_others(cuda, dtype, gap, place):
     prefix.k_scale[0, place] = gap * np.log(2.0) / (127 * DIM)
     check(_attend(q, prefix, n, cuda, scale=1.0), *prefix64(q, prefix, n, 1.0), dtype)
     assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), 3e38])
+@pytest.mark.parametrize("dead", [128, 200, 1500])
+def test_a_prefix_that_begins_with_scores_of_minus_infinity(cuda, dtype, bad, dead):
+    """Whole tiles whose scores are below every fp32 number, before keys some 300 binary orders below
+    zero: the rows are what those keys give, as if the others were not there."""
+    import torch
+
+    n, rng = 2000, _gen(dead)
+    prefix = _filled(rng, 1, n, KV_HEADS, DIM, cuda)
+    base = np.sign(rng.standard_normal(DIM))
+    k = torch.from_numpy((-127 * base).astype(np.int8)).to(cuda)
+    prefix.k[0] = torch.where(prefix.k[0] % 3 == 0, 0, k)
+    prefix.k_scale.fill_(300 * np.log(2.0) / (127 * DIM * 2 / 3))
+    prefix.k[0, :dead] = k
+    prefix.k_scale[0, :dead] = bad
+    q = _tensor(base * (1 + 0.01 * rng.random((SEQS, KV_HEADS * GROUP, 1))), cuda, dtype)
+    rest = qb.KvCache.from_tensors(*(t[:, dead:].clone() for t in (prefix.k, prefix.v, prefix.k_scale, prefix.v_scale)))
+    check(_attend(q, prefix, n, cuda, scale=1.0), *prefix64(q, rest, n - dead, 1.0), dtype)
+    assert qb.device_status() == qb.OK
