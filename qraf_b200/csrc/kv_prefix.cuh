@@ -8,8 +8,9 @@
 //     O += P V   (tcgen05, P in TMEM, V in shared memory)
 // The codes become fp16 exactly; Q and P are split into hi + lo of two fp16, each
 // part an MMA of its own into the same fp32 accumulator.  The queries of 16-bit
-// activations are exact in one part; for bf16 the weights take one part too: their
-// rounding, 2^-12 of themselves, is an eighth of the output's own.
+// activations are exact in one part.  The weights take two whatever the type: in one
+// they are off by 2^-12 of themselves, which moved a tenth of the outputs of bf16 calls
+// (8 sequences behind 65536 rows) to a neighbouring number.
 //
 // Two softmax warpgroups take the tiles in turn.  S becomes P in place (a thread owns
 // a row, so it overwrites only what it has read) in one of three TMEM buffers, so
@@ -31,8 +32,6 @@
 // 8192 keys, f32, with the join: 57 us, 300 TFLOP/s of the formula's.
 #pragma once
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "kv_attention.cuh"
 #include "matmul_tc.cuh"
@@ -50,8 +49,7 @@ constexpr int32_t kPreUp = 7;           // weights of p = 1 are below 2^7
 // Parts of the queries (16-bit ones are exact in one) and of the weights.
 template <typename Q>
 constexpr uint32_t pre_q_parts() { return sizeof(Q) == 4u ? 2u : 1u; }
-template <typename Q>
-constexpr uint32_t pre_p_parts() { return std::is_same<Q, __nv_bfloat16>::value ? 1u : 2u; }
+constexpr uint32_t kPreParts = 2;
 
 // The tensor cores' fp32 accumulator truncates: every accumulation may lose a last bit, and
 // always toward zero.  So the lower parts' products go first (into small sums); O is
@@ -159,7 +157,7 @@ __device__ __forceinline__ float pre_max(uint32_t s_col, const float* ks, uint32
 
 // The row's weights, relative to the maximum m, in the place of its scores (the hi
 // parts of 32 keys, then their lo parts); returns the sum of exp(s - m).
-template <uint32_t PP, bool MASK>
+template <bool MASK>
 __device__ __forceinline__ float pre_weights(uint32_t s_col, const float* ks, const float* vs, uint32_t valid, float rf, float m) {
     const float2 rf2 = make_float2(rf, rf), m2 = make_float2(-m, -m), neg = make_float2(-1.0f, -1.0f);
     float2 sum = make_float2(0.0f, 0.0f);
@@ -187,15 +185,13 @@ __device__ __forceinline__ float pre_weights(uint32_t s_col, const float* ks, co
                 const float2 w = f2_mul(p, vv);
                 const __half2 h = __floats2half2_rn(w.x, w.y);
                 hi[(j + i) / 2u] = *reinterpret_cast<const uint32_t*>(&h);
-                if constexpr (PP == 2u) {
-                    const float2 d = f2_fma(__half22float2(h), neg, w);
-                    const __half2 r = __floats2half2_rn(d.x, d.y);
-                    lo[(j + i) / 2u] = *reinterpret_cast<const uint32_t*>(&r);
-                }
+                const float2 d = f2_fma(__half22float2(h), neg, w);
+                const __half2 r = __floats2half2_rn(d.x, d.y);
+                lo[(j + i) / 2u] = *reinterpret_cast<const uint32_t*>(&r);
             }
         }
         tmem_st16(s_col + 32u * c, hi);
-        if constexpr (PP == 2u) tmem_st16(s_col + 32u * c + 16u, lo);
+        tmem_st16(s_col + 32u * c + 16u, lo);
     }
     tmem_wait_st();
     return __fadd_rn(sum.x, sum.y);
@@ -248,7 +244,7 @@ __device__ __forceinline__ void bulk_s2g(float* dst, const float* src, uint32_t 
 // Q: the type of q and out.
 template <uint32_t HDP, typename Q>
 __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_constant__ KvAttnParams p) {
-    constexpr uint32_t QP = pre_q_parts<Q>(), PP = pre_p_parts<Q>();
+    constexpr uint32_t QP = pre_q_parts<Q>();
     using S = PreShape<HDP, QP>;
     extern __shared__ uint8_t pre_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pre_smem_raw) + 1023u) & ~uintptr_t(1023));
@@ -316,7 +312,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
             return __fmul_rn(pow2_bits(static_cast<int32_t>(most) - kPreUp + 1),
-                             fmaf(static_cast<float>(tiles * PP), kPreLoss, 1.0f));
+                             fmaf(static_cast<float>(tiles * kPreParts), kPreLoss, 1.0f));
         };
 
         if (warp < kPreWarpXf) {
@@ -410,8 +406,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 if (m_now != m) l = __fmul_rn(l, ex2(__fsub_rn(m, m_now)));
                 m = m_now;
                 const float m_use = m > -INFINITY ? m : 0.0f;   // nothing seen yet: every weight 2^-inf = 0
-                l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<PP, false>(s_col, ks, ks + 128, kPreKeys, rf, m_use)
-                                                   : pre_weights<PP, true>(s_col, ks, ks + 128, valid, rf, m_use));
+                l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<false>(s_col, ks, ks + 128, kPreKeys, rf, m_use)
+                                                   : pre_weights<true>(s_col, ks, ks + 128, valid, rf, m_use));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&p_ready[b]);
@@ -624,10 +620,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 tc_fence_after();
                 if (tc_elect_one()) {
 #pragma unroll 1
-                    for (uint32_t part = 0; part < PP; ++part)
+                    for (uint32_t part = 0; part < kPreParts; ++part)
 #pragma unroll 4
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
-                            pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * (PP - 1u - part) + 8u * (k & 1u),
+                            pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * (kPreParts - 1u - part) + 8u * (k & 1u),
                                        tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
                                        t % p.pre_term + part + k > 0u);
                     tc_commit(&pv_done[sl]);

@@ -106,3 +106,47 @@ def test_a_prefix_that_begins_with_scores_of_minus_infinity(cuda, dtype, bad, de
     rest = qb.KvCache.from_tensors(*(t[:, dead:].clone() for t in (prefix.k, prefix.v, prefix.k_scale, prefix.v_scale)))
     check(_attend(q, prefix, n, cuda, scale=1.0), *prefix64(q, rest, n - dead, 1.0), dtype)
     assert qb.device_status() == qb.OK
+
+
+def _peaked(cuda, dtype, n, places):
+    """Queries that each attend to one key alone: (q, prefix, exact outputs).  Token t's key lies 300
+    binary orders above its next, so the answer is that key's value."""
+    import torch
+
+    rng, m = _gen(n), len(places)
+    prefix = _filled(rng, 1, n, KV_HEADS, DIM, cuda)
+    prefix.k_scale.mul_(2.0 ** -12)
+    base = np.sign(rng.standard_normal((m, DIM)))
+    most = np.abs(base @ base.T - DIM * np.eye(m)).max()   # of another key's codes with a query
+    assert most < 0.8 * DIM
+    place = torch.tensor(places, device=cuda)
+    prefix.k[0, place] = torch.from_numpy(127 * base).to(cuda).to(torch.int8).unsqueeze(1)
+    prefix.k_scale[0, place] = 2000.0 / (127 * DIM)
+    of = np.arange(SEQS) % m
+    q = _tensor(np.broadcast_to(base[of, None], (SEQS, KV_HEADS * GROUP, DIM)), cuda, dtype)
+    v = prefix.v[0, place].double() * prefix.v_scale[0, place].double().unsqueeze(-1)
+    return q, prefix, v[torch.from_numpy(of).to(cuda)].repeat_interleave(GROUP, 1)
+
+
+def _check_rounded(got, want, rel, floor):
+    """got is want, off by at most rel of itself and floor, rounded once."""
+    import torch
+
+    tol = want.abs() * rel + floor
+    low, high = ((want + s * tol).to(got.dtype) for s in (-1, 1))
+    bad = ~((low <= got) & (got <= high))
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, worst {float(((got.double() - want).abs() / want.abs()).max()):.3g} of itself"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_of_peaked_rows_keep_22_bits(cuda, dtype):
+    """Rows that attend to one key behind a short prefix.  A weight w = p vs is rounded to fp32 (2^-24)
+    and split (the lower part's rounding: 2^-22 of w at most); its two products with a code are exact
+    and their sum loses a last bit (2^-23) at both accumulations; p is the same number in the sum of
+    weights, which the others do not reach; the join's division and two products round to 2^-24 each:
+    below 2^-20 together, and as much again for the correction of three tiles' accumulations.  Every
+    weight's lower part may end at 2^-31 of the largest vs."""
+    q, prefix, want = _peaked(cuda, dtype, 300, [0, 77, 128, 129, 200, 255, 256, 299])
+    floor = 127 * float(prefix.v_scale.max()) * 2.0 ** -31
+    _check_rounded(_attend(q, prefix, 300, cuda, scale=1.0), want, 2.0 ** -19, floor)
+    assert qb.device_status() == qb.OK
