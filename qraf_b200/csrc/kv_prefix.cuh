@@ -255,9 +255,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     float* s_m = reinterpret_cast<float*>(smem + S::kM);
     // by S buffer (three): the K tile and the scales are there, S is, P is; by tile parity:
-    // the V tile is there, O has it, a warp's rows have their maxima
+    // the V tile is there, O has it, a warp's rows have their maxima; by stretch: the query
+    // rows are there, O has all of its tiles
     uint64_t *k_ready = bars, *s_ready = bars + 3, *p_ready = bars + 6, *v_ready = bars + 9, *pv_done = bars + 11,
-             *m_ready = bars + 13 /* [2][4] */, *q_ready = bars + 21, *drain = bars + 22;
+             *m_ready = bars + 13 /* [2][4] */, *q_ready = bars + 21, *o_ready = bars + 22, *drain = bars + 23;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t hd = p.kv.hd, H = p.kv.kv_heads, G = p.group;
     const uint32_t rows = p.runs.n * G;
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             for (uint32_t j = 0; j < 4u; ++j) mbar_init(&m_ready[4u * i + j], 1);
         }
         mbar_init(q_ready, 8);
+        mbar_init(o_ready, 1);
         mbar_init(drain, 1);
         fence_mbar_init();
         s_fail = 0u;
@@ -627,6 +629,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                                        tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
                                        t % p.pre_term + part + k > 0u);
                     tc_commit(&pv_done[sl]);
+                    if (t + 1u == n) tc_commit(o_ready);
                 }
                 __syncwarp();
                 // the next S of this buffer overwrites the P that has just been used
@@ -634,15 +637,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             }
         }
         x0 += n;
-        q_phase ^= 1u;
         // ── the rows leave as records, by way of shared memory (over K and V) ──
         if (warp < kPreWarpXf && ok) {
-            ok = warp_wait(&pv_done[(x0 - 1u) & 1u], (x0 - 1u) >> 1 & 1u);   // the last, and so every one
+            // not pv_done of the last tile: a warp here knows only that the tile three before its own
+            // last is in O, so that one's parity may be that of the tile two before the last
+            ok = warp_wait(o_ready, q_phase);
             tc_fence_after();
             const uint32_t r = (warp & 3u) * 32u + lane;
             s_ml[wg * 256u + r] = m;   // -inf and 0 where the warpgroup had no tile
             s_ml[wg * 256u + 128u + r] = l;
         }
+        q_phase ^= 1u;
         if (!ok) s_fail = 1u;
         __syncthreads();
         if (s_fail) {   // a wait ran out (the status is raised): let the MMAs in flight end, then leave
