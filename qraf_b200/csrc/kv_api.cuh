@@ -116,9 +116,10 @@ bool prefix_on_tiles(uint64_t rows, uint64_t kv_heads, uint32_t hd, uint64_t pre
 
 struct KvaPlan {
     uint32_t row_tiles = 0, p_chunks = 0, p_chunk = 0, own_tiles = 0, splits = 0, own_wide = 0, pre_ctas = 0;
-    uint32_t pre_base = 0, pre_extra = 0, pre_term = 0, pre_terms = 0;
+    uint32_t pre_base = 0, pre_extra = 0;
     uint32_t cluster = 0;   // CTAs of a cluster: kv_attention_cluster_kernel has the call
-    uint64_t items = 0, part_bytes = 0;
+    uint64_t items = 0, part_bytes = 0;   // part_bytes: the workspace, records and
+    uint64_t sum_at = 0;                  // from this byte of it kv_prefix_kernel's sums (0: none)
 };
 
 // How a call's rows and keys are cut.  Items of a few hundred keys keep the 2 x SMs
@@ -193,14 +194,7 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         pl->pre_base = work / pl->pre_ctas;
         pl->pre_extra = work % pl->pre_ctas;
         // a unit's T tiles may start inside one CTA's range and end inside another's
-        const uint32_t ctas = std::min({T, pl->pre_ctas, (T + pl->pre_base - 1u) / pl->pre_base + 1u});
-        const uint32_t longest = std::min(T, pl->pre_base + (pl->pre_extra ? 1u : 0u));   // stretch
-        pl->pre_term = 16;
-        do {
-            pl->pre_term *= 2;
-            pl->pre_terms = (longest + pl->pre_term - 1u) / pl->pre_term;
-        } while (ctas * pl->pre_terms > kKvaMaxChunks / 2u && pl->pre_terms > 1u);
-        pl->p_chunks = ctas * pl->pre_terms;
+        pl->p_chunks = std::min({T, pl->pre_ctas, (T + pl->pre_base - 1u) / pl->pre_base + 1u});
         if (pl->p_chunks > kKvaMaxChunks / 2u) return fail(QRAF_ERR_UNSUPPORTED, "a GPU of %d SMs cuts the prefix too finely", sm_count);
     } else if (prefix_len) {
         pl->row_tiles = static_cast<uint32_t>((rows + 15u) / 16u);
@@ -220,6 +214,10 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
     pl->items = items;
     if (pl->p_chunks + pl->splits > 1u || pl->pre_ctas)
         pl->part_bytes = static_cast<uint64_t>(n) * heads * (pl->p_chunks + pl->splits) * (hd + 4u) * sizeof(float);
+    if (pl->pre_ctas && pl->pre_base + (pl->pre_extra ? 1u : 0u) > kPreTerm) {
+        pl->sum_at = pl->part_bytes;
+        pl->part_bytes += static_cast<uint64_t>(pl->pre_ctas) * kPreRows * (hd <= 64u ? 64u : 128u) * sizeof(float);
+    }
     return QRAF_OK;
 }
 
@@ -423,8 +421,7 @@ int qraf_cuda_kv_attention(const qraf_kv_t* kv, const qraf_kv_t* prefix, uint32_
     p.pre_ctas = pl.pre_ctas;
     p.pre_base = pl.pre_base;
     p.pre_extra = pl.pre_extra;
-    p.pre_term = pl.pre_term;
-    p.pre_terms = pl.pre_terms;
+    p.pre_sum = pl.sum_at ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace_dev) + pl.sum_at) : nullptr;
     p.chained = pl.pre_ctas ? 1u : 0u;
     p.part = pl.part_bytes ? static_cast<float*>(workspace_dev) : nullptr;
     const uint32_t hd = kv->head_dim;

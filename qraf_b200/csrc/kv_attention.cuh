@@ -42,6 +42,8 @@ constexpr uint32_t kKvaMaxChunks = 512;     // chunks of one row, prefix and own
 
 constexpr uint32_t kPreRows = 128;          // kv_prefix.cuh: query rows of a tile = MMA M
 constexpr uint32_t kPreKeys = 128;          // and keys of a tile
+constexpr uint32_t kPreTerm = 8;            // tiles of one sum on the tensor cores
+static_assert(kPreTerm % 2u == 0u, "the same warpgroup begins every sum");
 
 // kv_prefix_kernel's (unit, key tile) pairs, unit-major, are dealt out in contiguous
 // ranges of `base` pairs a CTA, one more for the first `extra`: the first pair of CTA c,
@@ -74,7 +76,7 @@ struct KvAttnParams {
     uint32_t p_chunks, p_chunk;   // its chunks (pre_ctas: records of a row at most) and keys in one
     uint32_t pre_ctas;       // CTAs of kv_prefix_kernel, which has the prefix then; 0: kv_attention_kernel has it
     uint32_t pre_base, pre_extra;   // its ranges
-    uint32_t pre_term, pre_terms;   // tiles in one sum, and the records of a row that a CTA may leave: one per sum
+    float* pre_sum;          // its CTAs' sums of finished terms, [128][64 or 128] each; nullptr: no stretch has two
     uint32_t chained;        // kv_attention_kernel was launched as kv_prefix_kernel's dependent
     uint32_t own_tiles, splits;              // own rows: row tiles over all runs (at most), chunks of each (at most)
     uint32_t own_wide;       // the kernel with tiles of 16 rows, else 8
@@ -812,22 +814,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const _
         live = b >= 0 && run_ok(p, static_cast<uint32_t>(b), &slot, &len);
         if (live && p.splits) own_chunk(len, p.splits, &own);
     }
-    uint32_t pre = p.p_chunks, tile0 = 0, T = 0, c0 = 0;
-    if (p.pre_ctas) {   // the CTAs whose ranges meet this row's unit
-        T = (p.prefix_len + kPreKeys - 1u) / kPreKeys;
-        const uint32_t h = head / p.group;
-        tile0 = (h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows) * T;
-        c0 = pre_owner(p.pre_base, p.pre_extra, tile0);
-        pre = (pre_owner(p.pre_base, p.pre_extra, tile0 + T - 1u) - c0 + 1u) * p.pre_terms;
+    uint32_t pre = p.p_chunks;
+    if (p.pre_ctas) {   // the CTAs whose ranges meet this row's unit leave a record each
+        const uint32_t T = (p.prefix_len + kPreKeys - 1u) / kPreKeys, h = head / p.group;
+        const uint32_t tile0 = (h * p.row_tiles + (t * p.group + head - h * p.group) / kPreRows) * T;
+        pre = pre_owner(p.pre_base, p.pre_extra, tile0 + T - 1u) - pre_owner(p.pre_base, p.pre_extra, tile0) + 1u;
     }
-    // whether record i of the prefix was left: a CTA leaves one per pre_term tiles of its stretch
-    auto left = [&](uint32_t i) {
-        if (!p.pre_ctas || i >= pre) return true;
-        const uint32_t c = c0 + i / p.pre_terms;
-        const uint32_t a = max(tile0, pre_start(p.pre_base, p.pre_extra, c));
-        const uint32_t b = min(tile0 + T, pre_start(p.pre_base, p.pre_extra, c + 1u));
-        return i % p.pre_terms * p.pre_term < b - a;
-    };
     const uint32_t chunks = live ? pre + own : 0u;
     auto at = [&](uint32_t i) { return i < pre ? i : p.p_chunks + (i - pre); };   // record of chunk i
     const uint64_t ld = hd + 4u;
@@ -839,7 +831,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const _
 #pragma unroll
     for (uint32_t k = 0; k < kMine; ++k) {
         const uint32_t i = sub + WPR * (lane + 32u * k);
-        ml[k] = i < chunks && left(i) ? __ldcg(reinterpret_cast<const float2*>(rec + at(i) * ld + hd)) : make_float2(-INFINITY, 0.0f);
+        ml[k] = i < chunks ? __ldcg(reinterpret_cast<const float2*>(rec + at(i) * ld + hd)) : make_float2(-INFINITY, 0.0f);
         m = fmaxf(m, ml[k].x);
     }
 #pragma unroll

@@ -29,7 +29,7 @@
 // Measured on a B200: the MMAs of one tile take about 8 x 80 cycles a part for S and
 // 8 x 73 for O (N = 128, K = 16 each), in two parts about 2700 cycles; a tile takes some
 // 4350, bound by the warps that turn codes into fp16.  512 rows of 8 KV heads of 128 behind
-// 8192 keys, f32, with the join: 57 us, 300 TFLOP/s of the formula's.
+// 8192 keys, f32, with the join: 58 us, 300 TFLOP/s of the formula's.
 #pragma once
 
 #include "common.cuh"
@@ -50,14 +50,6 @@ constexpr int32_t kPreUp = 7;           // weights of p = 1 are below 2^7
 template <typename Q>
 constexpr uint32_t pre_q_parts() { return sizeof(Q) == 4u ? 2u : 1u; }
 constexpr uint32_t kPreParts = 2;
-
-// The tensor cores' fp32 accumulator truncates: every accumulation may lose a last bit, and
-// always toward zero.  So the lower parts' products go first (into small sums); O is
-// lengthened by what it loses on the average (measured on a B200: 1.0e-7 of itself a tile and
-// part, 8 accumulations; without this 16 tiles came out 3e-6 short); and O starts anew every
-// p.pre_term tiles (32 where that keeps a row's records below 256), its sum so far leaving as
-// a record.
-constexpr float kPreLoss = 1.0e-7f;
 
 template <uint32_t HDP, uint32_t QP>
 struct PreShape {
@@ -197,23 +189,39 @@ __device__ __forceinline__ float pre_weights(uint32_t s_col, const float* ks, co
     return __fadd_rn(sum.x, sum.y);
 }
 
-// The row's output so far, in numbers, to its record (with the maximum that it refers to and
-// no sum of weights: that is in the stretch's last record).
-template <uint32_t HDP>
-__device__ __forceinline__ void pre_flush_row(uint32_t o_col, float* rec, uint32_t hd, float unit, float m) {
+// The tensor cores' fp32 accumulator truncates: every accumulation may lose a last bit, and
+// always toward zero (measured on a B200: evenly weighted keys lose 1.0e-7 of the sum a tile
+// and part, 8 accumulations).  So the lower parts' products go first (into small sums), and O
+// starts anew every kPreTerm tiles: its sum so far is added, rounded to nearest, to the CTA's
+// own sums (p.pre_sum), which stay in L2.  512 rows of 8 KV heads behind 8192 keys (16 tiles a
+// CTA), off the 64-bit answer and time of the kernels: 4 tiles 1.1e-6, 64 us; 8 tiles 1.8e-6,
+// 59 us; 16 tiles 3.4e-6, 59 us.  Plain fp32 is off by 1.8e-6.
+
+// o times alpha plus v times unit (a power of two).
+__device__ __forceinline__ float4 pre_add4(float4 o, float alpha, const float* v, float unit) {
+    return make_float4(fmaf(o.x, alpha, __fmul_rn(v[0], unit)), fmaf(o.y, alpha, __fmul_rn(v[1], unit)),
+                       fmaf(o.z, alpha, __fmul_rn(v[2], unit)), fmaf(o.w, alpha, __fmul_rn(v[3], unit)));
+}
+
+// Where a CTA's sums have columns c .. c + 4 of row r: a warp's rows next to each other.
+__device__ __forceinline__ float4* pre_sum_at(float4* sums, uint32_t c, uint32_t r) { return sums + (c / 4u) * kPreRows + r; }
+
+// The row's output so far, in numbers, added to its sums times alpha (FIRST: to nothing).
+template <uint32_t HDP, bool FIRST>
+__device__ __forceinline__ void pre_add_row(uint32_t o_col, float4* sums, uint32_t r, uint32_t hd, float unit, float alpha) {
 #pragma unroll 1
     for (uint32_t c = 0; c < HDP; c += 32u) {
         float v[32];
         tmem_ld32(o_col + c, v);
         tmem_wait_ld();
-        if (!rec) continue;
+        float4 old[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 32u; j += 4u)
-            if (c + j < hd)
-                *reinterpret_cast<float4*>(rec + c + j) =
-                    make_float4(__fmul_rn(v[j], unit), __fmul_rn(v[j + 1u], unit), __fmul_rn(v[j + 2u], unit), __fmul_rn(v[j + 3u], unit));
+        for (uint32_t j = 0; j < 8u; ++j)
+            old[j] = FIRST || c + 4u * j >= hd ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(pre_sum_at(sums, c + 4u * j, r));
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j)
+            if (c + 4u * j < hd) __stcg(pre_sum_at(sums, c + 4u * j, r), pre_add4(old[j], alpha, v + 4u * j, unit));
     }
-    if (rec) *reinterpret_cast<float2*>(rec + hd) = make_float2(m, 0.0f);
 }
 
 // The row's output so far times alpha.
@@ -297,25 +305,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
     uint32_t x0 = 0u;   // tiles of the CTA's stretches before this one: tile t is the CTA's tile x0 + t
     uint32_t q_phase = 0u;
     bool ok = true;
+    float4* sums = reinterpret_cast<float4*>(p.pre_sum) + static_cast<uint64_t>(blockIdx.x) * (kPreRows * HDP / 4u);
     for (uint32_t w = pre_start(p.pre_base, p.pre_extra, blockIdx.x); w < w1;) {
         const uint32_t unit = w / T, tile0 = w - unit * T, n = min(T - tile0, w1 - w);
         const uint32_t h = unit / p.row_tiles, row0 = (unit - h * p.row_tiles) * kPreRows;
         const uint32_t key0 = tile0 * kPreKeys, key1 = min(p.prefix_len, (tile0 + n) * kPreKeys);
         float m = -INFINITY, l = 0.0f;       // of a softmax thread: its sum, and the maximum that it refers to
         const uint32_t wg = warp >> 2;       // softmax warpgroup: tiles of this parity (of the stretch)
-        const uint32_t first_rec = (blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T)) * p.pre_terms;
-        auto record = [&](uint32_t r, uint32_t term) -> float* {   // of the tile's row r; nullptr past the last row
+        float m_sum = -INFINITY;             // and of its row's sums of earlier terms
+        const uint32_t rec_at = blockIdx.x - pre_owner(p.pre_base, p.pre_extra, unit * T);
+        auto record = [&](uint32_t r) -> float* {   // of the tile's row r; nullptr past the last row
             const uint32_t row = row0 + r, t = row / G, head = h * G + (row - t * G);
-            return row < rows ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + first_rec + term) * (hd + 4u)
+            return row < rows ? p.part + ((static_cast<uint64_t>(t) * p.heads + head) * (p.p_chunks + p.splits) + rec_at) * (hd + 4u)
                               : nullptr;
         };
-        auto unit_factor = [&](uint32_t tiles) {   // the sum of that many tiles to numbers
+        auto unit_factor = [&]() {   // O to numbers
             uint32_t most = 14u;
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) most = max(most, s_unit[i]);
-            return __fmul_rn(pow2_bits(static_cast<int32_t>(most) - kPreUp + 1),
-                             fmaf(static_cast<float>(tiles * kPreParts), kPreLoss, 1.0f));
+            return pow2_bits(static_cast<int32_t>(most) - kPreUp + 1);
         };
+        auto rescale = [](float from, float to) { return from == to ? 1.0f : ex2(__fsub_rn(from, to)); };   // from <= to, -inf too
 
         if (warp < kPreWarpXf) {
             // ── the query rows: 16 a warp, all of its loads in flight ──
@@ -375,21 +385,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 const float ymax = valid >= kPreKeys ? pre_max<false>(s_col, ks, kPreKeys) : pre_max<true>(s_col, ks, valid);
                 const float mt = __fmul_rn(ymax, rf);
                 // the maximum that the row refers to from this tile on (-inf while every score was)
-                float m_now = mt > -INFINITY ? mt : -INFINITY, alpha = 1.0f;
+                float m_now = mt > -INFINITY ? mt : -INFINITY, alpha = 1.0f, before = -INFINITY;
                 if (t > 0u) {
                     const uint32_t px = x - 1u;
                     ok = warp_wait(&m_ready[4u * (px & 1u) + (warp & 3u)], px >> 1 & 1u);
                     if (!ok) break;
-                    const float before = s_m[(px & 1u) * 128u + r];
+                    before = s_m[(px & 1u) * 128u + r];
                     // never a lower one: the sum of weights runs on over the stretch's terms, and one
                     // scaled up by 2^128 would overflow
-                    if (t % p.pre_term == 0u) {   // a term of O's sum is full: it starts anew
+                    if (t % kPreTerm == 0u) {   // O starts anew
                         m_now = fmaxf(before, mt);
-                        ok = warp_wait(&pv_done[px & 1u], px >> 1 & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
-                        pre_flush_row<HDP>(o_col, record(r, t / p.pre_term - 1u), hd, unit_factor(p.pre_term), before);
-                        tc_fence_before();
                     } else if (mt > __fadd_rn(before, kPreLag)) {
                         alpha = ex2(__fsub_rn(before, mt));
                     } else {
@@ -410,6 +415,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 const float m_use = m > -INFINITY ? m : 0.0f;   // nothing seen yet: every weight 2^-inf = 0
                 l = __fadd_rn(l, valid >= kPreKeys ? pre_weights<false>(s_col, ks, ks + 128, kPreKeys, rf, m_use)
                                                    : pre_weights<true>(s_col, ks, ks + 128, valid, rf, m_use));
+                if (t > 0u && t % kPreTerm == 0u) {   // the term before leaves O
+                    ok = warp_wait(&pv_done[(x - 1u) & 1u], (x - 1u) >> 1 & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (t == kPreTerm) pre_add_row<HDP, true>(o_col, sums, r, hd, unit_factor(), 0.0f);
+                    else pre_add_row<HDP, false>(o_col, sums, r, hd, unit_factor(), rescale(m_sum, before));
+                    m_sum = before;
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(&p_ready[b]);
@@ -627,7 +640,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                         for (uint32_t k = 0; k < kPreKeys / 16u; ++k)
                             pre_mma_ts(tmem + 384u, tmem + b * 128u + 32u * (k >> 1) + 16u * (kPreParts - 1u - part) + 8u * (k & 1u),
                                        tc_smem_desc(base + S::kV + sl * S::kKTile + (k >> 2) * (HDP * 128u) + (k & 3u) * 32u), idesc_o,
-                                       t % p.pre_term + part + k > 0u);
+                                       t % kPreTerm + part + k > 0u);
                     tc_commit(&pv_done[sl]);
                     if (t + 1u == n) tc_commit(o_ready);
                 }
@@ -646,6 +659,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
             const uint32_t r = (warp & 3u) * 32u + lane;
             s_ml[wg * 256u + r] = m;   // -inf and 0 where the warpgroup had no tile
             s_ml[wg * 256u + 128u + r] = l;
+            if (wg == 0u) s_m[(x0 & 1u) * 128u + r] = m_sum;   // the slot of the tile before the last: that has been read
         }
         q_phase ^= 1u;
         if (!ok) s_fail = 1u;
@@ -661,7 +675,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         float* jo = reinterpret_cast<float*>(smem + S::kK);   // [128][HDP + 4]
         if (warp < kPreWarpXf) {   // each warpgroup has half of the columns
             const uint32_t r = (warp & 3u) * 32u + lane;
-            const float unit_f = unit_factor((n - 1u) % p.pre_term + 1u);
+            const float unit_f = unit_factor();
+            const float m_end = s_m[((x0 - 1u) & 1u) * 128u + r], alpha = rescale(s_m[(x0 & 1u) * 128u + r], m_end);
             const uint32_t o_col = tmem + (((warp & 3u) * 32u) << 16) + 384u;
             float* dst = jo + r * S::kJoinLd;
 #pragma unroll 1
@@ -669,19 +684,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
                 float v[32];
                 tmem_ld32(o_col + c, v);
                 tmem_wait_ld();
+                float4 old[8];
 #pragma unroll
-                for (uint32_t k = 0; k < 32u; k += 4u)
-                    if (c + k < hd)
-                        *reinterpret_cast<float4*>(dst + c + k) = make_float4(__fmul_rn(v[k], unit_f), __fmul_rn(v[k + 1u], unit_f),
-                                                                              __fmul_rn(v[k + 2u], unit_f), __fmul_rn(v[k + 3u], unit_f));
+                for (uint32_t k = 0; k < 8u; ++k)
+                    old[k] = n > kPreTerm && c + 4u * k < hd ? __ldcg(pre_sum_at(sums, c + 4u * k, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k)
+                    if (c + 4u * k < hd) *reinterpret_cast<float4*>(dst + c + 4u * k) = pre_add4(old[k], alpha, v + 4u * k, unit_f);
             }
             if (wg == 0u) {
-                const float m_end = s_m[((x0 - 1u) & 1u) * 128u + r];
                 float sum = 0.0f;
 #pragma unroll
                 for (uint32_t i = 0; i < 2u; ++i) {
-                    const float mi = s_ml[i * 256u + r];
-                    sum = fmaf(s_ml[i * 256u + 128u + r], mi == m_end ? 1.0f : ex2(__fsub_rn(mi, m_end)), sum);
+                    sum = fmaf(s_ml[i * 256u + 128u + r], rescale(s_ml[i * 256u + r], m_end), sum);
                 }
                 *reinterpret_cast<float4*>(dst + hd) = make_float4(m_end, sum, 0.0f, 0.0f);
             }
@@ -690,7 +705,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefix_kernel(const __grid_
         }
         __syncthreads();
         if (warp < 4u) {   // one bulk copy a row
-            if (float* rec = record(tid, (n - 1u) / p.pre_term)) bulk_s2g(rec, jo + tid * S::kJoinLd, hd + 4u);
+            if (float* rec = record(tid)) bulk_s2g(rec, jo + tid * S::kJoinLd, hd + 4u);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // written: K and V tiles may come, the CTA may end
         }

@@ -144,9 +144,46 @@ def test_weights_of_peaked_rows_keep_22_bits(cuda, dtype):
     and split (the lower part's rounding: 2^-22 of w at most); its two products with a code are exact
     and their sum loses a last bit (2^-23) at both accumulations; p is the same number in the sum of
     weights, which the others do not reach; the join's division and two products round to 2^-24 each:
-    below 2^-20 together, and as much again for the correction of three tiles' accumulations.  Every
-    weight's lower part may end at 2^-31 of the largest vs."""
+    below 2^-20 together, and as much again to spare.  Every weight's lower part may end at 2^-31 of
+    the largest vs."""
     q, prefix, want = _peaked(cuda, dtype, 300, [0, 77, 128, 129, 200, 255, 256, 299])
     floor = 127 * float(prefix.v_scale.max()) * 2.0 ** -31
     _check_rounded(_attend(q, prefix, 300, cuda, scale=1.0), want, 2.0 ** -19, floor)
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [300, 5120])
+def test_peaked_rows_are_as_exact_as_their_weight(cuda, dtype, n):
+    """One key has a row's weight, in the first tile, in the last, or between, and the tensor cores add
+    exact zeros for the others: the same steps as above, with nothing for their accumulations, and a
+    term's sum added to the record (2^-24)."""
+    last = (n - 1) // 128 * 128
+    q, prefix, want = _peaked(cuda, dtype, n, [0, 77, 127, 128, 200, n // 2, last, n - 1])
+    floor = 127 * float(prefix.v_scale.max()) * 2.0 ** -31
+    _check_rounded(_attend(q, prefix, n, cuda, scale=1.0), want, 2.0 ** -20, floor)
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("n", [5120, 20481])
+def test_even_weights_lose_nothing_with_length(cuda, n):
+    """Keys of about the same weight and positive values, so that nothing cancels.  In a term of 8 tiles
+    O grows evenly over 8 x 16 accumulations, each losing at most a last bit of its size: 64 x 2^-23.
+    The terms' additions, and the sum of weights' (64 pairs a tile, growing likewise, and a tile's sum
+    to the ones before), round to nearest: at most (n / 1024 + 32 + n / 256) / 2 x 2^-23 in their mean
+    growth.  Weights are off by 2^-21 and twice the scores' bound ((2 dim / 16 + 8) 2^-23 of sum |q| |k|
+    here), the rest by 8 x 2^-23."""
+    import torch
+
+    rng = _gen(n)
+    prefix = _filled(rng, 1, n, KV_HEADS, DIM, cuda)
+    prefix.v.copy_(prefix.v.abs().clamp_(min=30))
+    q = _tensor(0.02 * rng.standard_normal((SEQS, KV_HEADS * GROUP, DIM)), cuda)
+    got = _attend(q, prefix, n, cuda, scale=DIM ** -0.5).double().cpu().numpy()
+    want, _ = prefix64(q, prefix, n, DIM ** -0.5)
+    k = prefix.k[0].double().abs() * prefix.k_scale[0].double().unsqueeze(-1)
+    a = float((q.double().abs().amax(1).amax(0) @ k.amax(0).amax(0))) * DIM ** -0.5
+    rel = (64 + (n / 1024 + 32 + n / 256) / 2 + 4 + 2 * a * (2 * DIM / 16 + 8) + 8) * 2.0 ** -23
+    off = np.abs(got - want) / want
+    assert off.max() <= rel, f"{off.max():.3g}, mean {off.mean():.3g}, against {rel:.3g}"
     assert qb.device_status() == qb.OK
