@@ -468,9 +468,9 @@ int qraf_cuda_decoder_share_prefix(qraf_decoder_t d, uint32_t slot, uint32_t len
  * at most max_slots), stores their K and V, attends causally (each token sees the
  * prefix, its slot's rows and its run's tokens up to itself) and leaves every token's
  * logits in logits_dev[n][vocab].  Rows behind the last run are not cached, and what
- * their logits hold is unspecified.  A run whose slot or positions are out of range
- * raises the device status.  The first call of a shape allocates; make one before
- * capturing. */
+ * their logits hold is unspecified.  A run whose slot or positions, the last one's
+ * too, are out of range raises the device status, and nothing of it is stored.  The
+ * first call of a shape allocates; make one before capturing. */
 int qraf_cuda_decoder_step_runs(qraf_decoder_t d, uint32_t n, const int32_t* tokens_dev, const int32_t* slots_dev,
                                 const int32_t* starts_dev, const int32_t* cu_dev, uint32_t count, float* logits_dev, int mode,
                                 void* stream);

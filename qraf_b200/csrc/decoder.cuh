@@ -537,32 +537,24 @@ struct RopeStoreParams {
     const float2* rope;      // [max_seq][hd / 2]
     KvView kv;               // one layer of the int8 cache
     KvRuns runs;             // firsts = position of each run's first token
-    uint32_t heads, max_seq, prefix_len, prefix_slot;
+    const int32_t* lens;     // [runs]: dec_run_lens_kernel's
+    uint32_t heads, prefix_len;
 };
 
-// Row of the slot that holds a run's position, and whether the run may be carried out:
-// behind a shared prefix a slot's rows begin where the prefix ends, and the prefix's own
-// slot takes no tokens.
-__device__ __forceinline__ bool run_row(int32_t slot, int32_t pos, uint32_t prefix_len, uint32_t prefix_slot, uint32_t slots,
-                                        uint32_t max_seq, uint32_t* row) {
-    const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < slots && pos >= static_cast<int32_t>(prefix_len) &&
-                    static_cast<uint32_t>(pos) < max_seq && !(prefix_len && static_cast<uint32_t>(slot) == prefix_slot);
-    *row = ok ? static_cast<uint32_t>(pos) - prefix_len : 0u;
-    return ok;
-}
-
-// Rows that each run's slot holds after the step (-1: the run is refused), for
-// kv_attention; raises the status for runs out of range.
+// Rows that each run's slot holds after the step (-1: the run is padding or refused, and
+// nothing of it is carried out), for the two kernels that follow; raises the status for runs
+// out of range.  Behind a shared prefix a slot's rows begin where the prefix ends, and the
+// prefix's own slot takes no tokens.
 __global__ void __launch_bounds__(256) dec_run_lens_kernel(KvRuns runs, uint32_t prefix_len, uint32_t prefix_slot,
                                                            uint32_t slots, uint32_t max_seq, int32_t* __restrict__ lens) {
     const uint32_t b = blockIdx.x * blockDim.x + threadIdx.x;
     if (b >= runs.count) return;
     const int32_t n = runs.cu ? runs.cu[b + 1u] - runs.cu[b] : 1, slot = runs.slots[b], pos = runs.firsts[b];
-    uint32_t row;
-    const bool ok = run_row(slot, pos, prefix_len, prefix_slot, slots, max_seq, &row) && n >= 0 &&
-                    static_cast<uint32_t>(n) <= max_seq - static_cast<uint32_t>(pos);
+    const bool ok = slot >= 0 && static_cast<uint32_t>(slot) < slots && pos >= static_cast<int32_t>(prefix_len) &&
+                    static_cast<uint32_t>(pos) < max_seq && !(prefix_len && static_cast<uint32_t>(slot) == prefix_slot) &&
+                    n >= 0 && static_cast<uint32_t>(n) <= max_seq - static_cast<uint32_t>(pos);
     if (!ok && slot != -1) raise_error(kErrBadLaunch);
-    lens[b] = ok ? static_cast<int32_t>(row) + n : -1;
+    lens[b] = ok ? pos - static_cast<int32_t>(prefix_len) + n : -1;
 }
 
 // One token a CTA: q and k rotated, k and v quantised into the cache
@@ -570,10 +562,10 @@ __global__ void __launch_bounds__(256) dec_run_lens_kernel(KvRuns runs, uint32_t
 __global__ void __launch_bounds__(256) dec_rope_store_kernel(const RopeStoreParams a) {
     const uint32_t t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = a.kv.hd, half = hd / 2u;
     const int32_t b = find_run(a.runs, static_cast<int32_t>(t));
-    if (b < 0) return;
-    const int32_t first = run_begin(a.runs, b), pos = a.runs.firsts[b] + (static_cast<int32_t>(t) - first), slot = a.runs.slots[b];
-    uint32_t row;
-    if (a.runs.firsts[b] < 0 || !run_row(slot, pos, a.prefix_len, a.prefix_slot, a.kv.slots, a.max_seq, &row)) return;
+    if (b < 0 || a.lens[b] < 0) return;
+    const int32_t i = static_cast<int32_t>(t) - run_begin(a.runs, b), pos = a.runs.firsts[b] + i, slot = a.runs.slots[b];
+    const uint32_t row = static_cast<uint32_t>(pos) - a.prefix_len;
+    if (i < 0 || row >= static_cast<uint32_t>(a.lens[b])) return;   // an unsorted cu
     const float2* cs = a.rope + static_cast<size_t>(pos) * half;
     const uint32_t kv_heads = a.kv.kv_heads;
     for (uint32_t u = warp; u < a.heads + 2u * kv_heads; u += 8u) {
@@ -1245,9 +1237,8 @@ int qraf_cuda_decoder_step_runs(qraf_decoder_t d, uint32_t n, const int32_t* tok
         a.kv = view_of(kv);
         a.runs = runs;
         a.heads = d->heads;
-        a.max_seq = d->max_seq;
+        a.lens = d->lens;
         a.prefix_len = d->prefix_len;
-        a.prefix_slot = d->prefix_slot;
         (dec_rope_store_kernel<<<n, 256, 0, st>>>(a), count_launch());
         QRAF_CUDA_TRY(cudaGetLastError());
         const uint64_t q_dim = static_cast<uint64_t>(d->heads) * d->hd;

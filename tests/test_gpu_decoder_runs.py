@@ -235,3 +235,29 @@ def test_refusals(tmp_path, cuda, oracle_lib):
         dec.step_runs(one, one, one, logits=torch.zeros(1, vocab + 1, device=cuda))
     assert dec.step_runs(one[:0], one[:0], one[:0]).shape == (0, vocab)
     dec.close()
+
+
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_a_refused_run_stores_nothing(tmp_path, cuda, oracle_lib, prefix):
+    """A run that ends past the last position, by one or by many, with others in the same step: the
+    status is raised, no row of its slot is written, not even those that would fit, and the others give
+    what they give without it."""
+    path, vocab = _model(tmp_path, oracle_lib, layers=1, heads=8, kv_heads=2, max_seq=64)
+    rng = np.random.default_rng(6)
+    prompt, good = ([int(t) for t in rng.integers(0, vocab, n)] for n in (20, 5))
+    dec = qb.Decoder(path, max_slots=40, max_seq=64, kv_int8=True)
+    if prefix:
+        _runs(dec, cuda, [prompt], [9], [0], qb.MODE_EXACT)
+        dec.share_prefix(9, prefix)
+    want = _runs(dec, cuda, [good], [1], [prefix], qb.MODE_EXACT)
+    cache = dec.layer_cache(0)
+    for slot, (length, start) in enumerate(((5, 60), (9, 60), (2, 63)), 2):
+        bad = [int(t) for t in rng.integers(0, vocab, length)]
+        got = _runs(dec, cuda, [bad, good], [slot, 1], [start, prefix], qb.MODE_EXACT)
+        assert qb.device_status() == qb.ERR_INVALID and qb.device_status() == qb.OK
+        assert got[length:].tobytes() == want.tobytes()
+        for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+            assert not t[slot].any()
+    _runs(dec, cuda, [[1, 2, 3, 4]], [2], [60], qb.MODE_EXACT)   # one that fits to the last position
+    assert cache.k_scale[2, 60 - prefix:64 - prefix].all() and qb.device_status() == qb.OK
+    dec.close()
