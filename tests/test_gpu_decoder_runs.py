@@ -261,3 +261,35 @@ def test_a_refused_run_stores_nothing(tmp_path, cuda, oracle_lib, prefix):
     _runs(dec, cuda, [[1, 2, 3, 4]], [2], [60], qb.MODE_EXACT)   # one that fits to the last position
     assert cache.k_scale[2, 60 - prefix:64 - prefix].all() and qb.device_status() == qb.OK
     dec.close()
+
+
+def test_the_guides_serving_example(tmp_path, cuda, oracle_lib, monkeypatch):
+    """The serving example of the integration guide, run as it stands: what it calls `tokens` and
+    `accepted` are those."""
+    import re
+    from pathlib import Path
+
+    import torch
+
+    from test_gpu_sampling import verify64
+
+    text = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "verify_drafts(" in b]
+    assert len(blocks) == 1
+    path, vocab = _model(tmp_path, oracle_lib, layers=1, heads=8, kv_heads=2, max_seq=4096)
+    Path(path).rename(tmp_path / "model-q8.qraf")
+    monkeypatch.chdir(tmp_path)
+    rng = np.random.default_rng(7)
+    q = rng.random((2, 3, vocab)).astype(np.float32) + 0.1
+    q /= q.sum(-1, keepdims=True)
+    drafts = rng.integers(0, vocab, (2, 3)).astype(np.int32)
+    u, last = (rng.random(n).astype(np.float32) for n in ((2, 3), 2))
+    lines = np.concatenate([rng.integers(0, vocab, (2, 1)).astype(np.int32), drafts], 1)
+    at = {"prompt": _i32([int(t) for t in rng.integers(0, vocab, 30)], cuda), "drafted": torch.from_numpy(lines.reshape(-1)).to(cuda),
+          "starts": _i32([30, 33], cuda), "q": torch.from_numpy(q).to(cuda), "drafts": torch.from_numpy(drafts).to(cuda),
+          "u": torch.from_numpy(u).to(cuda), "u_last": torch.from_numpy(last).to(cuda)}
+    exec(compile(blocks[0], "INTEGRATION.md", "exec"), at)
+    want = verify64(at["p"].view(2, 4, -1).cpu().numpy(), q, drafts, u, last)
+    assert np.array_equal(at["tokens"].cpu().numpy(), want[0]) and np.array_equal(at["accepted"].cpu().numpy(), want[1])
+    at["dec"].close()
+    assert qb.device_status() == qb.OK
