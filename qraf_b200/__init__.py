@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 
 import numpy as np
 
@@ -348,6 +349,7 @@ class Decoder:
         self._h = h
         v, hd, l, ms, mq = (C.c_uint32() for _ in range(5))
         check(_get_lib().qraf_cuda_decoder_info(h, C.byref(v), C.byref(hd), C.byref(l), C.byref(ms), C.byref(mq)))
+        self._caches = weakref.WeakSet()   # views of its cache
         self.vocab, self.hidden, self.layers = v.value, hd.value, l.value
         self.max_slots, self.max_seq = ms.value, mq.value
 
@@ -390,10 +392,13 @@ class Decoder:
         check(_get_lib().qraf_cuda_decoder_share_prefix(self._h, slot, length))
 
     def layer_cache(self, layer: int) -> "KvCache":
-        """One layer of the int8 cache for kv_store, kv_load and kv_attention; it keeps the decoder."""
+        """One layer of the int8 cache for kv_store, kv_load and kv_attention; it keeps the decoder, until
+        that is closed: the operators then refuse it, and tensors taken from it must not be used."""
         d = qraf_kv_t()
         check(_get_lib().qraf_cuda_decoder_kv(self._h, layer, C.byref(d)))
-        return KvCache._of_desc(d, self)
+        cache = KvCache._of_desc(d, self)
+        self._caches.add(cache)
+        return cache
 
     def kv_read(self, slot: int, layer: int, pos: int, kv_heads: int, head_dim: int):
         """One cache row: (k, v) float32 [kv_heads * head_dim], or with the int8 cache
@@ -413,6 +418,8 @@ class Decoder:
     def close(self) -> None:
         if self._h:
             h, self._h = self._h, C.c_void_p()
+            for cache in self._caches:
+                cache._detach()
             check(_get_lib().qraf_cuda_decoder_close(h))
 
     def __del__(self):
@@ -730,16 +737,29 @@ class KvCache:
             class _Holder:
                 __cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (getattr(d, name), False), "version": 3,
                                             "strides": strides}
+                owner = keepalive   # the tensor keeps this object
 
             setattr(self, name, torch.as_tensor(_Holder(), device=f"cuda:{d.device}"))
         self._describe(d)
         return self
 
     def _describe(self, d: qraf_kv_t) -> None:
-        self.desc, self._ref = d, C.byref(d)
+        self.desc = d
         self.device, self._index = self.k.device, d.device
         self.slots, self.rows, self.kv_heads, self.head_dim = d.slots, d.rows, d.kv_heads, d.head_dim
         self._workspace = {}
+
+    @property
+    def _ref(self):
+        """The descriptor for a call of the library."""
+        if not self.desc.k:
+            raise ValueError("the decoder of this cache is closed")
+        return C.byref(self.desc)
+
+    def _detach(self) -> None:
+        """The memory behind the cache goes away."""
+        C.memset(C.byref(self.desc), 0, C.sizeof(self.desc))
+        self.k = self.v = self.k_scale = self.v_scale = None
 
 
 def kv_store(cache: KvCache, k, v, slots, starts, cu=None, stream=None) -> None:
@@ -749,13 +769,13 @@ def kv_store(cache: KvCache, k, v, slots, starts, cu=None, stream=None) -> None:
     rows contiguous, any stride between them.  Rows cu[b] .. cu[b + 1] go to rows starts[b] ..
     of slot slots[b] (int32 CUDA tensors; without cu, one row each); slot -1 and rows behind
     the last run are left out, and where two runs write one row the later one stays."""
-    heads, dim, index = cache.kv_heads, cache.head_dim, cache._index
+    ref, heads, dim, index = cache._ref, cache.kv_heads, cache.head_dim, cache._index
     n, ld_k = _rows_of(k, heads, dim, index, "k")
     m, ld_v = _rows_of(v, heads, dim, index, "v")
     if m != n or v.dtype != k.dtype:
         raise ValueError("k and v must have one type and length")
     slots_p, starts_p, cu_p, count = _runs_of(slots, starts, cu, n, index, "starts")
-    check(_get_lib().qraf_cuda_kv_store(cache._ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
+    check(_get_lib().qraf_cuda_kv_store(ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
                                         starts_p, cu_p, count, _stream_on(stream, index)))
 
 
@@ -764,7 +784,7 @@ def kv_load(cache: KvCache, slots, starts, cu=None, n=None, dtype=None, k=None, 
 
     n: the number of rows (needed with cu, unless k and v are given to be written);
     dtype: float32 (default), float16 or bfloat16.  Returns (k, v) [n, kv_heads, head_dim]."""
-    heads, dim, index = cache.kv_heads, cache.head_dim, cache._index
+    ref, heads, dim, index = cache._ref, cache.kv_heads, cache.head_dim, cache._index
     if (k is None) != (v is None):
         raise ValueError("k and v go together")
     if k is None:
@@ -780,7 +800,7 @@ def kv_load(cache: KvCache, slots, starts, cu=None, n=None, dtype=None, k=None, 
         if m != n or v.dtype != k.dtype:
             raise ValueError("k and v must have one type and length")
     slots_p, starts_p, cu_p, count = _runs_of(slots, starts, cu, n, index, "starts")
-    check(_get_lib().qraf_cuda_kv_load(cache._ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
+    check(_get_lib().qraf_cuda_kv_load(ref, k.data_ptr(), v.data_ptr(), _type_of(k.dtype), ld_k, ld_v, n, slots_p,
                                        starts_p, cu_p, count, _stream_on(stream, index)))
     return k, v
 
@@ -797,7 +817,7 @@ def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_sl
     prefix_slot of the KvCache `prefix`.  A token that sees nothing gets zeros; tokens of
     slot -1 or behind the last sequence keep what `out` holds.  max_len: no lens[b] is larger
     (default: the cache's rows).  scale: default head_dim ** -0.5.  Returns out, shaped like q."""
-    dim, index = cache.head_dim, cache._index
+    ref, dim, index = cache._ref, cache.head_dim, cache._index
     if q.dim() not in (2, 3):
         raise ValueError("q must be [n, heads, head_dim] or [n, heads * head_dim]")
     heads = q.shape[1] if q.dim() == 3 else q.shape[1] // dim
@@ -821,13 +841,13 @@ def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_sl
     size = cache._workspace.get(key)
     if size is None:   # bytes by shape; the memory itself belongs to the call
         b = C.c_uint64()
-        check(lib.qraf_cuda_kv_attention_workspace(cache._ref, prefix_len, n, heads, count, cu is not None, max_len,
+        check(lib.qraf_cuda_kv_attention_workspace(ref, prefix_len, n, heads, count, cu is not None, max_len,
                                                    C.byref(b)))
         if len(cache._workspace) > 4096:
             cache._workspace.clear()
         size = cache._workspace[key] = b.value
     ws = _empty(size, _torch().uint8, q, stream) if size else None
-    check(lib.qraf_cuda_kv_attention(cache._ref, prefix._ref if prefix_len else None, prefix_slot, prefix_len, q.data_ptr(),
+    check(lib.qraf_cuda_kv_attention(ref, prefix._ref if prefix_len else None, prefix_slot, prefix_len, q.data_ptr(),
                                      out.data_ptr(), _type_of(q.dtype), q_ld, out_ld, n, heads, slots_p, lens_p, cu_p, count,
                                      max_len, dim ** -0.5 if scale is None else scale, ws.data_ptr() if size else None, size,
                                      _stream_on(stream, index)))

@@ -293,3 +293,38 @@ def test_the_guides_serving_example(tmp_path, cuda, oracle_lib, monkeypatch):
     assert np.array_equal(at["tokens"].cpu().numpy(), want[0]) and np.array_equal(at["accepted"].cpu().numpy(), want[1])
     at["dec"].close()
     assert qb.device_status() == qb.OK
+
+
+def test_a_closed_decoders_cache_is_refused(tmp_path, cuda, oracle_lib):
+    """Views of a decoder's cache keep it; closing it takes their memory away, and every operator then
+    refuses them, as cache or as prefix, and so does the library their descriptor."""
+    import ctypes as C
+    import gc
+
+    import torch
+
+    path, vocab = _model(tmp_path, oracle_lib, layers=2, heads=8, kv_heads=2, max_seq=32)
+    dec = qb.Decoder(path, max_slots=4, max_seq=32, kv_int8=True)
+    scales = dec.layer_cache(1).k_scale
+    _runs(dec, cuda, [[1, 2, 3]], [1], [0], qb.MODE_EXACT)
+    cache = dec.layer_cache(1)
+    dim, one = cache.head_dim, _i32([1], cuda)
+    q, k = torch.zeros(1, 8, dim, device=cuda), torch.zeros(1, 2, dim, device=cuda)
+    want = cache.k_scale.clone()
+    del dec, cache
+    gc.collect()
+    assert torch.equal(scales, want) and scales[1, :3].all()   # a tensor alone keeps the decoder too
+    del scales
+    dec = qb.Decoder(path, max_slots=4, max_seq=32, kv_int8=True)
+    cache, own = dec.layer_cache(0), qb.KvCache(2, 8, 2, dim)
+    qb.kv_attention(q, cache, one, one)
+    dec.close()
+    for call in (lambda: qb.kv_store(cache, k, k, one, one), lambda: qb.kv_load(cache, one, one),
+                 lambda: qb.kv_attention(q, cache, one, one),
+                 lambda: qb.kv_attention(q, own, one, one, prefix=cache, prefix_len=4)):
+        with pytest.raises(ValueError, match="closed"):
+            call()
+    assert cache.k is None
+    assert qb.lib.qraf_cuda_kv_store(C.byref(cache.desc), k.data_ptr(), k.data_ptr(), 0, 2 * dim, 2 * dim, 1, one.data_ptr(),
+                                     one.data_ptr(), None, 1, None) == qb.ERR_INVALID
+    assert qb.device_status() == qb.OK
