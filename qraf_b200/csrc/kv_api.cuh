@@ -122,9 +122,9 @@ struct KvaPlan {
     uint64_t sum_at = 0;                  // from this byte of it kv_prefix_kernel's sums (0: none)
 };
 
-// How a call's rows and keys are cut.  Items of a few hundred keys keep the 2 x SMs
-// CTAs of the grid evenly busy; every chunk more costs each row one record of
-// (head_dim + 4) floats, written and read once.
+// How a call's rows and keys are cut.  Items of a few hundred keys keep the warps that run
+// at once evenly busy; every chunk more costs each row one record of (head_dim + 4) floats,
+// written and read once.
 int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t prefix_len, uint32_t count, bool ragged,
              uint32_t max_len, int sm_count, KvaPlan* pl) {
     const uint64_t G = heads / kv_heads, rows = static_cast<uint64_t>(n) * G;
@@ -137,16 +137,23 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
                                       : static_cast<uint64_t>(count) * ((G + R - 1u) / R);
         const uint64_t equal = ragged ? std::max<uint64_t>({1, rows / R, std::min(count, n)}) : tiles;   // for runs of equal lengths
         const uint64_t steps = (prefix_len + keys - 1u) / keys + (max_len + keys - 1u) / keys;
-        const uint64_t groups = equal * kv_heads, room = 2ull * static_cast<uint64_t>(sm_count);   // CTAs that run at once
+        const uint64_t groups = equal * kv_heads, sms = static_cast<uint64_t>(sm_count);
+        const uint64_t room = 2u * sms;   // CTAs that run at once
         uint32_t cl = 1;
         while (cl < 8u && steps > 4u * cl && 2u * cl * groups <= room) cl *= 2;   // a step a warp
-        // One launch where every cluster runs at once, unless a prefix makes the warps' shares
-        // long: it is read for every tile of rows here.  Measured on a B200 (us a call, cluster /
-        // the other kernels; 8 query heads a KV head of 128): 2 KV heads, 4 sequences, 512 own rows
-        // 8 / 12; 8 KV heads, 16 sequences, 2048 own rows 23 / 32; 2 KV heads, 64 sequences, 64 own
-        // rows behind 512 12 / 19, behind 2048 24 / 24; 16 behind 8192 25 / 22.
-        const uint64_t a_warp = (steps + 4u * cl - 1u) / (4u * cl);
-        if (groups * cl <= room && (!prefix_len || a_warp <= 8u)) {
+        // One launch where every cluster runs at once and the warps' shares are short.  A prefix is
+        // read for every tile of rows here; own rows alone go on longer where the clusters leave
+        // no SM empty.  Measured on a B200 (us a call, cluster / the other kernels; 8 query heads a
+        // KV head of 128): behind a prefix, 2 KV heads, 64 sequences of 64 own rows behind 512
+        // 12 / 19, behind 2048 24 / 24; 16 behind 8192 25 / 22.  Own rows alone, 2 KV heads, one
+        // sequence of 512 7.7 / 8.7, of 1024 8.9 / 10.2, of 2048 10.4 / 8.7, of 131072 183 / 31; 8 KV
+        // heads, 4 sequences (256 CTAs) of 2048 12.8 / 12.5, of 131072 254 / 234; 16 sequences
+        // (256 CTAs) of 2048 23.1 / 27.1, of 4096 38.6 / 41.5, of 8192 69.3 / 71.4, of 131072
+        // 1058 / 960.  Heads of 256, 2 KV heads, 16 sequences (256 CTAs) of 1024 17.2 / 17.8, of 2048
+        // 22.3 / 19.2.
+        const uint64_t a_warp = (steps + 4u * cl - 1u) / (4u * cl), share = a_warp * keys;
+        const bool brief = prefix_len ? a_warp <= 8u : share <= (hd <= 128u && groups * cl >= sms ? 512u : 32u);
+        if (groups * cl <= room && brief) {
             pl->own_wide = wide;
             pl->own_tiles = static_cast<uint32_t>(tiles);
             pl->cluster = cl;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import qraf_b200 as qb
-from test_gpu_kv import DTYPES, _filled, _gen, _i32, _tensor, check, quantise
+from test_gpu_kv import DTYPES, attention64, _filled, _gen, _i32, _tensor, check, quantise
 
 pytestmark = pytest.mark.gpu
 
@@ -186,4 +186,22 @@ def test_even_weights_lose_nothing_with_length(cuda, n):
     rel = (64 + (n / 1024 + 32 + n / 256) / 2 + 4 + 2 * a * (2 * DIM / 16 + 8) + 8) * 2.0 ** -23
     off = np.abs(got - want) / want
     assert off.max() <= rel, f"{off.max():.3g}, mean {off.mean():.3g}, against {rel:.3g}"
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("launches,seqs,heads,kv_heads,dim,rows,run", [
+    (1, 1, 16, 2, 128, 1024, 1), (2, 1, 16, 2, 128, 1025, 1), (2, 1, 64, 8, 128, 20000, 1), (2, 4, 16, 2, 64, 5000, 1),
+    (1, 16, 64, 8, 128, 2048, 1), (2, 16, 64, 8, 128, 9000, 1), (1, 1, 16, 2, 256, 1024, 1), (2, 1, 16, 2, 256, 1500, 1)])
+def test_long_own_rows_use_every_sm(cuda, launches, seqs, heads, kv_heads, dim, rows, run):
+    """Own rows without a prefix: one launch of clusters while they are short, or while the clusters
+    leave no SM empty, else the chunked kernel and its join."""
+    rng = _gen(rows)
+    cache = _filled(rng, seqs, rows, kv_heads, dim, cuda)
+    lens = [rows - 3 * b for b in range(seqs)]
+    q = _tensor(rng.standard_normal((seqs * run, heads, dim)), cuda)
+    args = q, cache, _i32(list(range(seqs)), cuda), _i32(lens, cuda), _i32([run * b for b in range(seqs + 1)], cuda) if run > 1 else None
+    before = qb.launch_count()
+    got = qb.kv_attention(*args)
+    assert qb.launch_count() - before == launches
+    check(got, *attention64(q, cache, list(range(seqs)), lens, [run] * seqs))
     assert qb.device_status() == qb.OK
