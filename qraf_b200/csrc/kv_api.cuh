@@ -138,7 +138,7 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         const uint64_t equal = ragged ? std::max<uint64_t>({1, rows / R, std::min(count, n)}) : tiles;   // for runs of equal lengths
         const uint64_t steps = (prefix_len + keys - 1u) / keys + (max_len + keys - 1u) / keys;
         const uint64_t groups = equal * kv_heads, sms = static_cast<uint64_t>(sm_count);
-        const uint64_t room = 2u * sms;   // CTAs that run at once
+        const uint64_t room = wide && hd > 128u ? sms : 2u * sms;   // CTAs that run at once: 132 KB of shared memory, or up to 100
         uint32_t cl = 1;
         while (cl < 8u && steps > 4u * cl && 2u * cl * groups <= room) cl *= 2;   // a step a warp
         // One launch where every cluster runs at once and the warps' shares are short.  A prefix is

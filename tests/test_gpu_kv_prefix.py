@@ -191,7 +191,8 @@ def test_even_weights_lose_nothing_with_length(cuda, n):
 
 @pytest.mark.parametrize("launches,seqs,heads,kv_heads,dim,rows,run", [
     (1, 1, 16, 2, 128, 1024, 1), (2, 1, 16, 2, 128, 1025, 1), (2, 1, 64, 8, 128, 20000, 1), (2, 4, 16, 2, 64, 5000, 1),
-    (1, 16, 64, 8, 128, 2048, 1), (2, 16, 64, 8, 128, 9000, 1), (1, 1, 16, 2, 256, 1024, 1), (2, 1, 16, 2, 256, 1500, 1)])
+    (1, 16, 64, 8, 128, 2048, 1), (2, 16, 64, 8, 128, 9000, 1), (1, 1, 16, 2, 256, 1024, 1), (2, 1, 16, 2, 256, 1500, 1),
+    (1, 4, 16, 2, 256, 500, 5), (2, 4, 16, 2, 256, 900, 5)])
 def test_long_own_rows_use_every_sm(cuda, launches, seqs, heads, kv_heads, dim, rows, run):
     """Own rows without a prefix: one launch of clusters while they are short, or while the clusters
     leave no SM empty, else the chunked kernel and its join."""
