@@ -438,7 +438,11 @@ int qraf_cuda_kv_load(const qraf_kv_t* kv, void* k_dev, void* v_dev, uint32_t ty
  * apart; they may not overlap.  max_len: no lens_dev[b] is larger (at most kv->rows;
  * one that is raises the device status and leaves its rows as they were); the work
  * is cut for that length.  Sums, maxima and the running output are fp32 and the
- * products at fp32 accuracy whatever the type.
+ * products at fp32 accuracy whatever the type: a query row is held in 22 bits of its
+ * largest element, a key's weight (its probability times its V scale) in 22 bits of
+ * itself, but no finer than 2^-31 of the largest V scale that the row sees.  So where
+ * the V scales of a head lie more than 2^9 apart, a row that attends to keys of small
+ * ones is exact relative to the largest, not to itself.
  * workspace_dev: qraf_cuda_kv_attention_workspace's bytes for the same shape
  * (16-byte aligned; NULL where that is 0), written by the call: calls that may run
  * at the same time, replays of captured ones among them, need one each. */

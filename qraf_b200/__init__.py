@@ -816,7 +816,8 @@ def kv_attention(q, cache: KvCache, slots, lens, cu=None, prefix=None, prefix_sl
     i of m sees the first lens[b] - m + 1 + i of them after the prefix_len rows of slot
     prefix_slot of the KvCache `prefix`.  A token that sees nothing gets zeros; tokens of
     slot -1 or behind the last sequence keep what `out` holds.  max_len: no lens[b] is larger
-    (default: the cache's rows).  scale: default head_dim ** -0.5.  Returns out, shaped like q."""
+    (default: the cache's rows).  scale: default head_dim ** -0.5.  Weights are exact to 22 bits of
+    themselves or 2^-31 of the largest V scale that the row sees.  Returns out, shaped like q."""
     ref, dim, index = cache._ref, cache.head_dim, cache._index
     if q.dim() not in (2, 3):
         raise ValueError("q must be [n, heads, head_dim] or [n, heads * head_dim]")

@@ -168,7 +168,9 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
     const uint32_t R = pl->own_wide ? 16u : 8u;
     const uint64_t own_tiles = ragged ? (rows + static_cast<uint64_t>(std::min(count, n)) * (R - 1u)) / R
                                       : static_cast<uint64_t>(count) * ((G + R - 1u) / R);
-    // warps (CTAs) that run at once, by registers and shared memory
+    // Warps (CTAs) to fill: what the chunk counts below were measured with, not the kernels'
+    // residency, which by registers and shared memory is 16 an SM (tiles of 16 rows: 12) for heads up
+    // to 64, 10 (8) up to 128 and 8 (6) above.
     const uint64_t slots = (pl->own_wide || hd > 128u ? 8ull : 11ull) * static_cast<uint64_t>(sm_count);
     uint64_t items = 0;
     if (max_len) {
