@@ -206,3 +206,102 @@ def test_long_own_rows_use_every_sm(cuda, launches, seqs, heads, kv_heads, dim, 
     assert qb.launch_count() - before == launches
     check(got, *attention64(q, cache, list(range(seqs)), lens, [run] * seqs))
     assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("launches,seqs,heads,kv_heads,dim,n", [(1, 70, 16, 2, 128, 700), (3, 90, 24, 3, 96, 1100), (1, 80, 16, 2, 48, 513),
+                                                                (3, 70, 16, 2, 128, 4111), (3, 150, 8, 2, 48, 1900),
+                                                                (2, 200, 16, 2, 256, 700), (2, 200, 16, 2, 64, 0)])
+def test_rows_that_allow_no_wide_access(cuda, dtype, launches, seqs, heads, kv_heads, dim, n):
+    """q and out column slices with odd offsets and odd strides, own slots and the prefix layers of a larger
+    cache, on each plan; what lies around out stays."""
+    import torch
+
+    rng = _gen(dim)
+    rows, layers, width = 40, 3, heads * dim
+
+    def layer(slots, length):
+        k, v = (torch.from_numpy(rng.integers(-127, 128, (slots, layers, length, kv_heads, dim)).astype(np.int8)).to(cuda) for _ in "kv")
+        ks, vs = (_tensor(rng.random((slots, layers, length, kv_heads)) * 0.02 + 0.001, cuda) for _ in "kv")
+        return qb.KvCache.from_tensors(k[:, 1], v[:, 1], ks[:, 1], vs[:, 1])
+
+    cache, prefix = layer(seqs, rows), layer(3, n + 5) if n else None
+    joined = _tensor(rng.standard_normal((seqs, width + 7)), cuda, dtype)
+    q = joined[:, 1:1 + width]
+    around = torch.full((seqs, width + 9), 7.0, device=cuda, dtype=q.dtype)
+    out = around[:, 3:3 + width]
+    slots, lens = [int(v) for v in rng.permutation(seqs)], [int(v) for v in rng.integers(0, rows + 1, seqs)]
+    before = qb.launch_count()
+    qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_slot=2 if n else 0, prefix_len=n, out=out)
+    assert qb.launch_count() - before == launches or not n
+    assert (around[:, :3] == 7).all() and (around[:, 3 + width:] == 7).all()
+    shape = (seqs, heads, dim)
+    check(out.reshape(shape), *attention64(q.reshape(shape), cache, slots, lens, [1] * seqs, prefix, 2, n), dtype)
+    assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,n,rows", [(3, 16, 2, 128, 100, 20), (70, 16, 2, 128, 1500, 20), (200, 16, 2, 256, 700, 20),
+                                                            (200, 16, 2, 64, 0, 300), (16, 16, 2, 128, 30000, 20)])
+def test_what_is_not_a_number_stays_so(cuda, dtype, seqs, heads, kv_heads, dim, n, rows):
+    """A query of NaN, one with an infinity, and a K scale of NaN that some rows see make those rows' heads
+    NaN and leave every other one as it is, on each plan."""
+    import torch
+
+    rng = _gen(seqs)
+    cache, prefix = _filled(rng, seqs, rows, kv_heads, dim, cuda), _filled(rng, 1, n, kv_heads, dim, cuda) if n else None
+    q = _tensor(rng.standard_normal((seqs, heads, dim)), cuda, dtype)
+    slots, lens = list(range(seqs)), [rows] * seqs
+    want, tol = attention64(q, cache, slots, lens, [1] * seqs, prefix, 0, n)
+    lost = torch.zeros(seqs, heads, dtype=torch.bool)
+    q[0] = float("nan")
+    lost[0] = True
+    q[1, 3] = float("inf")
+    lost[1, 3] = True
+    q[2, 5, 7] = float("nan")
+    lost[2, 5] = True
+    cache.k_scale[1, rows - 1, 1] = float("nan")
+    lost[1, heads // 2:] = True
+    got = qb.kv_attention(q, cache, _i32(slots, cuda), _i32(lens, cuda), prefix=prefix, prefix_len=n).cpu()
+    assert got[lost].isnan().all()
+    keep = ~lost
+    check(got[keep], want[keep.numpy()], tol[keep.numpy()], dtype)
+    assert qb.device_status() == qb.OK
+
+
+def test_two_streams_behind_one_prefix(cuda):
+    """Two batches behind the same prefix, at the same time on two streams, eagerly and as captured
+    calls, with several sums a stretch: each gives what it gives alone."""
+    import torch
+
+    rng = _gen(31)
+    seqs, heads, kv_heads, dim, n = 64, 64, 8, 128, 9000
+    prefix = _filled(rng, 1, n, kv_heads, dim, cuda)
+    sides = []
+    for i in range(2):
+        cache = _filled(rng, seqs, 30, kv_heads, dim, cuda)
+        q = _tensor(rng.standard_normal((seqs, heads, dim)), cuda, "float32" if i else "bfloat16")
+        args = q, cache, _i32(list(range(seqs)), cuda), _i32([int(v) for v in rng.integers(0, 31, seqs)], cuda)
+        sides.append((args, qb.kv_attention(*args, prefix=prefix, prefix_len=n)))
+    streams = [torch.cuda.Stream(cuda) for _ in sides]
+    torch.cuda.synchronize()
+    outs = [[] for _ in sides]
+    for _ in range(5):
+        for (args, _), st, got in zip(sides, streams, outs):
+            got.append(qb.kv_attention(*args, prefix=prefix, prefix_len=n, stream=st))
+    torch.cuda.synchronize()
+    graphs = []
+    for (args, _), st in zip(sides, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = qb.kv_attention(*args, prefix=prefix, prefix_len=n)
+        graphs.append((g, out))
+    for _ in range(5):
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, want), got, (_, replayed) in zip(sides, outs, graphs):
+        assert all(torch.equal(g, want) for g in got) and torch.equal(replayed, want)
+    del graphs
+    assert qb.device_status() == qb.OK
