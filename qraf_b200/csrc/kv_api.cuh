@@ -147,12 +147,13 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         // KV head of 128): behind a prefix, 2 KV heads, 64 sequences of 64 own rows behind 512
         // 12 / 19, behind 2048 24 / 24; 16 behind 8192 25 / 22.  Own rows alone, 2 KV heads, one
         // sequence of 512 7.7 / 8.7, of 1024 8.9 / 10.2, of 2048 10.4 / 8.7, of 131072 183 / 31; 8 KV
-        // heads, 4 sequences (256 CTAs) of 2048 12.8 / 12.5, of 131072 254 / 234; 16 sequences
+        // heads, 4 sequences (256 CTAs) of 2048 12.8 / 12.5, of 32768 70.9 / 70.0 (of 1024 where 32768
+        // are allowed 11.1 / 12.2), of 131072 254 / 234; 16 sequences
         // (256 CTAs) of 2048 23.1 / 27.1, of 4096 38.6 / 41.5, of 8192 69.3 / 71.4, of 131072
         // 1058 / 960.  Heads of 256, 2 KV heads, 16 sequences (256 CTAs) of 1024 17.2 / 17.8, of 2048
         // 22.3 / 19.2.
         const uint64_t a_warp = (steps + 4u * cl - 1u) / (4u * cl), share = a_warp * keys;
-        const bool brief = prefix_len ? a_warp <= 8u : share <= (hd <= 128u && groups * cl >= sms ? 512u : 32u);
+        const bool brief = prefix_len ? a_warp <= 8u : share <= (hd <= 128u && groups * cl >= sms ? 1024u : 32u);
         if (groups * cl <= room && brief) {
             pl->own_wide = wide;
             pl->own_tiles = static_cast<uint32_t>(tiles);
