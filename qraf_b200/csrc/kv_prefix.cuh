@@ -27,8 +27,8 @@
 // record per row (output, maximum, sum) for the joining kernel.
 //
 // Measured on a B200: the MMAs of one tile take about 8 x 80 cycles a part for S and
-// 8 x 73 for O (N = 128, K = 16 each), in two parts about 2700 cycles; a tile takes some
-// 4350, bound by the warps that turn codes into fp16.  512 rows of 8 KV heads of 128 behind
+// 8 x 73 for O (N = 128, K = 16 each), in two parts about 2400; a tile takes some 4400,
+// bound by the warps that turn codes into fp16.  512 rows of 8 KV heads of 128 behind
 // 8192 keys, f32, with the join: 58 us, 300 TFLOP/s of the formula's.
 #pragma once
 
