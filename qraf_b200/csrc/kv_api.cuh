@@ -146,14 +146,13 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         // no SM empty.  Measured on a B200 (us a call, cluster / the other kernels; 8 query heads a
         // KV head of 128): behind a prefix, 2 KV heads, 64 sequences of 64 own rows behind 512
         // 12 / 19, behind 2048 24 / 24; 16 behind 8192 25 / 22.  Own rows alone, 2 KV heads, one
-        // sequence of 512 7.7 / 8.7, of 1024 8.9 / 10.2, of 2048 10.4 / 8.7, of 131072 183 / 31; 8 KV
-        // heads, 4 sequences (256 CTAs) of 2048 12.8 / 12.5, of 32768 70.9 / 70.0 (of 1024 where 32768
-        // are allowed 11.1 / 12.2), of 131072 254 / 234; 16 sequences
-        // (256 CTAs) of 2048 23.1 / 27.1, of 4096 38.6 / 41.5, of 8192 69.3 / 71.4, of 131072
-        // 1058 / 960.  Heads of 256, 2 KV heads, 16 sequences (256 CTAs) of 1024 17.2 / 17.8, of 2048
-        // 22.3 / 19.2.
+        // sequence of 512 8.0 / 8.8, of 1024 9.2 / 10.2, of 2048 11.0 / 8.9, of 131072 229 / 32; 4 runs
+        // of 5 tokens (160 CTAs) of 8192 36 / 39, of 32768 104 / 95; 8 KV heads, 16 sequences (256
+        // CTAs) of 2048 25.9 / 27.6, of 4096 44.4 / 42.8, of 131072 1140 / 965; 4 sequences (256 CTAs)
+        // of 1024 10.9 / 11.4, of 8192 27.6 / 24.5 (of 1024 where 32768 are allowed 11.0 / 12.3).  Heads
+        // of 256, 2 KV heads, 16 sequences (256 CTAs) of 1024 17.2 / 18.0, of 2048 22.1 / 19.6.
         const uint64_t a_warp = (steps + 4u * cl - 1u) / (4u * cl), share = a_warp * keys;
-        const bool brief = prefix_len ? a_warp <= 8u : share <= (hd <= 128u && groups * cl >= sms ? 1024u : 32u);
+        const bool brief = prefix_len ? a_warp <= 8u : share <= (hd <= 128u && groups * cl >= sms ? 256u : 32u);
         if (groups * cl <= room && brief) {
             pl->own_wide = wide;
             pl->own_tiles = static_cast<uint32_t>(tiles);
@@ -178,8 +177,8 @@ int plan_kva(uint32_t n, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_
         // About one round of them, counting the tiles that runs of equal lengths would have:
         // the nearest whole number of chunks, or behind kv_prefix_kernel, whose SMs come free one
         // by one, the next larger.  Measured on a B200 (us a call, 3 / 4 chunks; 64 sequences, 8 KV
-        // heads of 128): own rows up to 1024 36.7 / 39.0, up to 4096 101.5 / 103.1; up to 1024
-        // behind a prefix of 8192 87.9 / 82.9.
+        // heads of 128): own rows up to 1024 37.5 / 39.9, up to 4096 106.3 / 108.5; up to 1024
+        // behind a prefix of 8192 92.8 / 86.3.
         const uint64_t groups = std::max<uint64_t>({1, rows / R, std::min(count, n)}) * kv_heads;
         const uint64_t by_len = (max_len + kKvaMinChunk - 1ull) / kKvaMinChunk;
         const uint64_t round = tiles ? slots + groups - 1u : slots + groups / 2u;

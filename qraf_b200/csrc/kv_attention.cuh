@@ -13,7 +13,10 @@
 // on the tensor cores at fp32 accuracy by splitting only the other operand: a
 // query row is scaled by a power of two and written as hi + lo of two fp16 (22
 // bits), and each weight p_t vs_t likewise, relative to the largest vs met.  The
-// four products accumulate in fp32; maxima, sums and the running output are fp32.
+// four products accumulate in fp32; maxima, sums and the running output are fp32.  The
+// tensor cores' accumulator truncates toward zero, so it takes the products of 16 keys
+// only, and the running output is added to outside of it, rounded to nearest: left in it,
+// 4096 evenly weighted keys came out 1.8e-5 short, 16384 9.2e-5 (measured on a B200).
 //
 // Work.  The rows of a work item (up to 16 of one KV head) meet one chunk of keys:
 // a chunk of the prefix, with rows of any sequences, so the prefix is read once
@@ -100,6 +103,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same product alone.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Two codes (bytes SEL of w, already with the sign bit flipped: code + 128) as
@@ -312,9 +323,12 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
         }
     }
 
-    float o[S::kOut][4];
+    // the output: per tile two columns of the lane's RT rows
+    float2 o[S::kOut][RT];
 #pragma unroll
-    for (uint32_t i = 0; i < S::kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    for (uint32_t i = 0; i < S::kOut; ++i)
+#pragma unroll
+        for (uint32_t e = 0; e < RT; ++e) o[i][e] = make_float2(0.0f, 0.0f);
     float run_m[RT], run_l[RT];
     int32_t vref[RT];   // the output's unit is 2^(vref - 140), every V scale seen is below 2^(vref - 126)
 #pragma unroll
@@ -451,14 +465,9 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
             }
             if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
-                for (uint32_t i = 0; i < S::kOut; ++i) {
-                    const float2 a = f2_mul(make_float2(o[i][0], o[i][1]), make_float2(down[0], down[0]));
-                    const float2 b = f2_mul(make_float2(o[i][2], o[i][3]), make_float2(down[RT - 1u], down[RT - 1u]));
-                    o[i][0] = a.x;
-                    o[i][1] = a.y;
-                    o[i][2] = b.x;
-                    o[i][3] = b.y;
-                }
+                for (uint32_t i = 0; i < S::kOut; ++i)
+#pragma unroll
+                    for (uint32_t e = 0; e < RT; ++e) o[i][e] = f2_mul(o[i][e], make_float2(down[e], down[e]));
             }
             uint32_t ph[RT][S::kTiles], pl[RT][S::kTiles];
 #pragma unroll
@@ -525,8 +534,17 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                                               {codes_f16<0x4342u>(a23), codes_f16<0x4342u>(b23)}};
 #pragma unroll
                     for (uint32_t j = 0; j < 4u; ++j) {
-                        mma_f16(o[4u * w + j], a, b[j][0], b[j][1]);
-                        if constexpr (WIDE) mma_f16(o[4u * w + j], al, b[j][0], b[j][1]);
+                        float d[4];
+                        float2(&y)[RT] = o[4u * w + j];
+                        if constexpr (WIDE) {
+                            mma_f16_new(d, al, b[j][0], b[j][1]);
+                            mma_f16(d, a, b[j][0], b[j][1]);
+                            y[0] = f2_add(y[0], make_float2(d[0], d[1]));
+                            y[RT - 1u] = f2_add(y[RT - 1u], make_float2(d[2], d[3]));
+                        } else {
+                            mma_f16_new(d, a, b[j][0], b[j][1]);
+                            y[0] = f2_add(y[0], f2_add(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
+                        }
                     }
                 }
             }
@@ -573,8 +591,8 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                 float y[4];
 #pragma unroll
                 for (uint32_t j = 0; j < 4u; ++j) {
-                    const float* a = o[4u * w + j];
-                    y[j] = __fmul_rn(WIDE ? a[2u * e + b] : __fadd_rn(a[b], a[2u + b]), f);
+                    const float2 a = o[4u * w + j][e];
+                    y[j] = __fmul_rn(b ? a.y : a.x, f);
                 }
                 const float4 v = make_float4(y[0], y[1], y[2], y[3]);
                 if (rec) *reinterpret_cast<float4*>(rec + d) = v;
@@ -662,10 +680,11 @@ __device__ __forceinline__ bool own_item(const KvAttnParams& p, uint32_t idx, ui
 // WIDE: prefix items and own rows in tiles of 16 rows, else own rows in tiles of 8.
 //
 // Measured on a B200 (64 sequences, 8 KV heads of 128, 8 query heads each, with the joining
-// kernel): up to 1024 rows a sequence 36.8 us, up to 4096 101 us, 3.7 TB/s of codes and
-// scales.  The loads alone take 76 us there: what bounds it is issuing some 900 instructions
-// a step of 32 keys, most of them turning codes into fp16 fragments.  Registers for eight
-// CTAs an SM at least: for eleven it took 112.
+// kernel): up to 1024 rows a sequence 37.5 us, up to 4096 106 us, 3.6 TB/s of codes and
+// scales.  The loads alone take 76 us there: what bounds it is issuing some 950 instructions
+// a step of 32 keys, most of them turning codes into fp16 fragments (64 are the additions to
+// the output: left in the tensor cores' accumulator it was 101 us, and short).  Registers for
+// eight CTAs an SM at least: for eleven it took a tenth longer.
 template <uint32_t HDP, bool WIDE>
 __device__ __forceinline__ void kva_cta(const KvAttnParams& p, uint8_t* kva_smem) {
     const uint32_t H = p.kv.kv_heads;
@@ -713,8 +732,8 @@ __global__ void __launch_bounds__(32, 8) kv_attention_kernel(const __grid_consta
 // Small calls, where latency counts: one launch, no workspace.  A cluster has a row
 // tile of one sequence and one KV head; its up to 32 warps take the steps of prefix
 // and own rows in equal shares, and join their records through distributed shared
-// memory.  The prefix is read once for every tile here, from L2.  Bound by latency: 9 us
-// on a B200 for 4 sequences of 16 / 2 heads behind 777 rows, 24 with the kernels below.
+// memory.  The prefix is read once for every tile here, from L2.  Bound by latency: 9.5
+// us on a B200 for 4 sequences of 16 / 2 heads behind 777 rows, 24 with the kernels below.
 constexpr uint32_t kKvaClusterWarps = 4;   // a CTA
 
 template <uint32_t HDP, bool WIDE>

@@ -305,3 +305,41 @@ def test_two_streams_behind_one_prefix(cuda):
         assert all(torch.equal(g, want) for g in got) and torch.equal(replayed, want)
     del graphs
     assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,rows,n", [(1700, 8, 1, 64, 4096, 0), (1300, 16, 1, 128, 2048, 0), (900, 4, 2, 256, 2000, 0),
+                                                            (400, 16, 4, 256, 16, 3000), (16, 64, 8, 128, 2000, 0)])
+def test_own_rows_lose_nothing_with_length(cuda, seqs, heads, kv_heads, dim, rows, n):
+    """Keys of about the same weight and positive values, in chunks of up to thousands of keys (every
+    warp has work without cutting finer), in one launch, and behind a prefix by 16 rows.  Sums round to
+    nearest, which has no preferred sign: over thousands of rows the mean of the signed errors is far
+    below a last bit (2^-23).  Left in the tensor cores' accumulator, a sum of k keys loses some
+    4e-9 k of itself."""
+    import torch
+
+    rng = _gen(dim)
+
+    def cache_of(slots, length):
+        c = qb.KvCache(slots, length, kv_heads, dim)
+        c.k.random_(-127, 128)
+        c.v.random_(30, 128)
+        c.k_scale.uniform_(0.005, 0.01)
+        c.v_scale.uniform_(0.005, 0.01)
+        return c
+
+    torch.manual_seed(dim)
+    cache, prefix = cache_of(seqs, rows), cache_of(1, n) if n else None
+    q = _tensor(0.02 * rng.standard_normal((seqs, heads, dim)), cuda)
+    got = qb.kv_attention(q, cache, _i32(list(range(seqs)), cuda), _i32([rows] * seqs, cuda), prefix=prefix, prefix_len=n)
+    off = []
+    for t in range(0, seqs, max(1, seqs * heads // 2400)):
+        k, v = (getattr(cache, s)[t].double() * getattr(cache, s + "_scale")[t].double().unsqueeze(-1) for s in "kv")
+        if n:
+            far = [getattr(prefix, s)[0].double() * getattr(prefix, s + "_scale")[0].double().unsqueeze(-1) for s in "kv"]
+            k, v = torch.cat([far[0], k]), torch.cat([far[1], v])
+        s = torch.einsum("hgd,khd->hgk", q[t].double().view(kv_heads, -1, dim), k) * dim ** -0.5
+        want = torch.einsum("hgk,khd->hgd", torch.softmax(s, -1), v).reshape(heads, dim)
+        off.append((got[t].double() - want) / want)
+    off = torch.stack(off)
+    assert off.mean().abs() < 2.0 ** -23, f"mean {float(off.mean()):.3g}, worst {float(off.abs().max()):.3g}"
+    assert qb.device_status() == qb.OK
