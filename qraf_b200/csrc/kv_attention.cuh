@@ -14,9 +14,10 @@
 // query row is scaled by a power of two and written as hi + lo of two fp16 (22
 // bits), and each weight p_t vs_t likewise, relative to the largest vs met.  The
 // four products accumulate in fp32; maxima, sums and the running output are fp32.  The
-// tensor cores' accumulator truncates toward zero, so it takes the products of 16 keys
-// only, and the running output is added to outside of it, rounded to nearest: left in it,
-// 4096 evenly weighted keys came out 1.8e-5 short, 16384 9.2e-5 (measured on a B200).
+// tensor cores' accumulator truncates toward zero, so it takes the products of 16 keys,
+// or of 64 dimensions of a score, and the running output and the scores are added to
+// outside of it, rounded to nearest: left in it, 4096 evenly weighted keys came out
+// 1.8e-5 short, 16384 9.2e-5 (measured on a B200).
 //
 // Work.  The rows of a work item (up to 16 of one KV head) meet one chunk of keys:
 // a chunk of the prefix, with rows of any sequences, so the prefix is read once
@@ -365,12 +366,11 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
             const uint8_t* vc = kc + S::kKeys * HDP;
             const float* scales = reinterpret_cast<const float*>(vc + S::kKeys * HDP);
             // ── scores ──
-            float s[S::kTiles][4];
-#pragma unroll
-            for (uint32_t t = 0; t < S::kTiles; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+            float2 s[S::kTiles][RT];   // two keys of the lane's RT rows; 64 dims at a time in the accumulator
 #pragma unroll
             for (uint32_t j = 0; j < HDP / 64u; ++j) {
                 uint4 kr[S::kTiles];
+                float acc[S::kTiles][4];
                 const bool in = 64u * j + 16u * c < hd;
 #pragma unroll
                 for (uint32_t t = 0; t < S::kTiles; ++t)
@@ -392,9 +392,22 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                     for (uint32_t t = 0; t < S::kTiles; ++t) {
                         const uint32_t w = (i == 0u ? kr[t].x : i == 1u ? kr[t].y : i == 2u ? kr[t].z : kr[t].w) ^ 0x80808080u;
                         const uint32_t b0 = codes_f16<0x4140u>(w), b1 = codes_f16<0x4342u>(w);
-                        mma_f16(s[t], a, b0, b1);
-                        if constexpr (WIDE) mma_f16(s[t], al, b0, b1);
+                        if constexpr (WIDE) {
+                            if (i == 0u) mma_f16_new(acc[t], al, b0, b1);
+                            else mma_f16(acc[t], al, b0, b1);
+                            mma_f16(acc[t], a, b0, b1);
+                        } else {
+                            if (i == 0u) mma_f16_new(acc[t], a, b0, b1);
+                            else mma_f16(acc[t], a, b0, b1);
+                        }
                     }
+                }
+#pragma unroll
+                for (uint32_t t = 0; t < S::kTiles; ++t) {
+                    const float2 d0 = make_float2(acc[t][0], acc[t][1]), d1 = make_float2(acc[t][2], acc[t][3]);
+                    const float2 y = WIDE ? d0 : f2_add(d0, d1);
+                    s[t][0] = j ? f2_add(s[t][0], y) : y;
+                    if constexpr (WIDE) s[t][RT - 1u] = j ? f2_add(s[t][RT - 1u], d1) : d1;
                 }
             }
 
@@ -417,9 +430,7 @@ __device__ __forceinline__ void kva_item(const KvAttnParams& p, const KvaItem& i
                 const float2 vv = *reinterpret_cast<const float2*>(scales + S::kKeys + 8u * t + 2u * c);
 #pragma unroll
                 for (uint32_t e = 0; e < RT; ++e) {
-                    const float2 dot = WIDE ? make_float2(s[t][2u * e], s[t][2u * e + 1u])
-                                            : f2_add(make_float2(s[t][0], s[t][1]), make_float2(s[t][2], s[t][3]));
-                    const float2 v = f2_mul(dot, f2_mul(ks, make_float2(rf[e], rf[e])));
+                    const float2 v = f2_mul(s[t][e], f2_mul(ks, make_float2(rf[e], rf[e])));
                     x[e][2u * t] = v.x;
                     x[e][2u * t + 1u] = v.y;
                     vs[e][2u * t] = vv.x;

@@ -343,3 +343,36 @@ def test_own_rows_lose_nothing_with_length(cuda, seqs, heads, kv_heads, dim, row
     off = torch.stack(off)
     assert off.mean().abs() < 2.0 ** -23, f"mean {float(off.mean()):.3g}, worst {float(off.abs().max()):.3g}"
     assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,rows", [(3, 8, 1, 256, 300), (200, 16, 2, 256, 300), (3, 16, 1, 128, 700), (300, 8, 2, 192, 64)])
+def test_scores_of_sharp_rows(cuda, seqs, heads, kv_heads, dim, rows):
+    """Scores of some 100 that are sums of like signs, where what a score loses counts in full: two keys
+    of the same score but for a few last bits, and their values opposite, so that the output is the
+    difference of two weights of a half.  A score is off by at most the 8 accumulations of each 64 of its
+    products (2^-23 of their sum each), dim / 64 additions and four roundings beside (2^-24 each) and the
+    queries' 22 bits (2^-22): (8 + dim / 128 + 6) 2^-23 of sum |q| |k| together."""
+    import torch
+
+    rng = _gen(dim)
+    cache = qb.KvCache(seqs, rows, kv_heads, dim)
+    codes = torch.from_numpy(rng.integers(90, 128, (seqs, 2, kv_heads, dim)).astype(np.int8)).to(cuda)
+    at = [rows // 3, rows - 1]
+    cache.k[:, at] = codes
+    cache.k_scale.fill_(1e-6)
+    cache.k_scale[:, at] = 100.0 / (108 * dim)
+    v = torch.from_numpy(rng.integers(1, 128, (seqs, kv_heads, dim)).astype(np.int8)).to(cuda)
+    cache.v[:, at[0]], cache.v[:, at[1]] = v, -v
+    cache.v_scale.fill_(0.01)
+    q = _tensor(1 + 0.05 * rng.random((seqs, heads, dim)), cuda)
+    got = qb.kv_attention(q, cache, _i32(list(range(seqs)), cuda), _i32([rows] * seqs, cuda), scale=1.0).double()
+    group = heads // kv_heads
+    k = codes.double() * cache.k_scale[:, at].double().unsqueeze(-1)
+    s = torch.einsum("thgd,tkhd->thgk", q.double().view(seqs, kv_heads, group, dim), k)
+    w = torch.softmax(s, -1)
+    size = (v.double() * float(cache.v_scale[0, 0, 0]))[:, :, None]
+    want = ((w[..., 0] - w[..., 1]).unsqueeze(-1) * size).reshape(seqs, heads, dim)
+    ds = s.max() * (8 + dim / 128 + 6) * 2.0 ** -23
+    tol = (size * (ds + 2.0 ** -20)).expand(-1, -1, group, -1).reshape(seqs, heads, dim)
+    assert ((got - want).abs() <= tol).all(), f"{float(((got - want).abs() / tol).max()):.3g} of the bound"
+    assert qb.device_status() == qb.OK
