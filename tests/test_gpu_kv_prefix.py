@@ -376,3 +376,30 @@ def test_scores_of_sharp_rows(cuda, seqs, heads, kv_heads, dim, rows):
     tol = (size * (ds + 2.0 ** -20)).expand(-1, -1, group, -1).reshape(seqs, heads, dim)
     assert ((got - want).abs() <= tol).all(), f"{float(((got - want).abs() / tol).max()):.3g} of the bound"
     assert qb.device_status() == qb.OK
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,n", [(3, 16, 2, 128, 0), (500, 16, 2, 64, 0), (3, 16, 2, 128, 100), (64, 64, 8, 128, 9000),
+                                                       (200, 16, 2, 256, 700), (7, 8, 1, 32, 300000)])
+def test_a_prefix_and_no_own_rows_at_all(cuda, seqs, heads, kv_heads, dim, n):
+    """max_len 0: the prefix alone on each plan, in a workspace of exactly the stated size that holds
+    anything beforehand, and zeros without one."""
+    import ctypes as C
+
+    import torch
+
+    rng = _gen(n)
+    cache, prefix = _filled(rng, seqs, 4, kv_heads, dim, cuda), _filled(rng, 1, max(n, 1), kv_heads, dim, cuda)
+    q = _tensor(rng.standard_normal((seqs, heads, dim)), cuda)
+    slots, lens = _i32(list(range(seqs)), cuda), _i32([0] * seqs, cuda)
+    want, tol = attention64(q, cache, list(range(seqs)), [0] * seqs, [1] * seqs, prefix, 0, n)
+    check(qb.kv_attention(q, cache, slots, lens, prefix=prefix, prefix_len=n, max_len=0), want, tol)
+    size = C.c_uint64()
+    qb.check(qb.lib.qraf_cuda_kv_attention_workspace(C.byref(cache.desc), n, seqs, heads, seqs, 0, 0, C.byref(size)))
+    room = torch.full((size.value + 512,), 0xFF, dtype=torch.uint8, device=cuda)   # NaN in every word
+    out = torch.full_like(q, 7.0)
+    qb.check(qb.lib.qraf_cuda_kv_attention(C.byref(cache.desc), C.byref(prefix.desc), 0, n, q.data_ptr(), out.data_ptr(), 0, heads * dim,
+                                           heads * dim, seqs, heads, slots.data_ptr(), lens.data_ptr(), None, seqs, 0, dim ** -0.5,
+                                           room.data_ptr() + 256, size.value, torch.cuda.current_stream().cuda_stream))
+    check(out, want, tol)
+    assert (room[:256] == 0xFF).all() and (room[256 + size.value:] == 0xFF).all()
+    assert qb.device_status() == qb.OK
